@@ -694,6 +694,56 @@ int mdt_refine_detections_post(const float *rois, const float *probs, const floa
                                const float *window_host, float min_confidence, int B, int pc, int dim, int n_classes, int M,
                                const float *dets, const long long *keep, float *result, unsigned char *valid, int *any_valid_scratch, void *stream);
 
+/* ------------------------------------------------------------------------- */
+/* Block-scaled numbers: activations kept in 8 bits, products in 4 bits        */
+/* ------------------------------------------------------------------------- */
+
+/*
+ * 32 consecutive values share one power of two 2^e (scale byte = e + 127).  With m the block's largest magnitude, e is the smallest exponent
+ * >= -127 with m <= Q * 2^e: Q = 255 (codes of a ReLU's output, unsigned), 127 (signed 8-bit codes, two's complement), 6 (4-bit codes: sign bit and
+ * the magnitudes 0, .5, 1, 1.5, 2, 3, 4, 6).  code = value * 2^-e rounded to the nearest code, ties to the even one; a positive ReLU output keeps at
+ * least the code 1, so code > 0 is the ReLU's mask exactly.  A block with an infinity or a NaN has scale byte 255 and reads back as NaN (its ReLU codes
+ * still hold the mask).  A code that was rounded up across the type's largest value reads back as that value.
+ */
+#define MDT_DTYPE_F32 0
+#define MDT_DTYPE_BF16 1
+#define MDT_DTYPE_F16 2
+
+/* n values in storage order <-> n code bytes (4-byte aligned) and ceil(n / 32) scale bytes; relu: values <= 0 get the code 0.  n <= 2^33. */
+int mdt_act8_quantize(const void *x, void *codes, void *scales, long long n, int dtype, int relu, void *stream);
+int mdt_act8_restore(const void *codes, const void *scales, void *x, long long n, int dtype, int relu, void *stream);
+
+/*
+ * mdt_bias_act_forward (same sums, same roundings, y may alias x) that also writes y's 8-bit copy: what a training step keeps of a layer's output in
+ * place of the fp32 map.  codes: n bytes, 4-byte aligned; scales: ceil(n / 32) bytes, in storage order; relu selects the unsigned codes.
+ */
+int mdt_bias_act_act8_forward(float *y, const float *x, const float *bias, const float *residual /* or NULL */, void *codes, void *scales,
+                              long long n, int channels, long long inner, int relu, void *stream);
+
+/*
+ * Backward pass of y = act(conv1x1(x, w) + bias (+ residual)) on channels-last rows from the 8-bit copies of x and y:
+ *   g = gy * (y code > 0)  (y_codes NULL: g = gy),   gx[v][i] = sum_o g[v][o] * w[o][i],   gw[o][i] = sum_v g[v][o] * x^[v][i],   gbias[o] = sum_v g[v][o]
+ * with fp32 products and sums in a fixed order (deterministic).  w: [c_out][c_in]; x_codes / x_scales: n_voxels * c_in values in storage order, x_relu their
+ * kind; gx, gw, gbias, g may each be NULL (not wanted).  A non-finite gradient gives non-finite results (an infinity may become a NaN).
+ */
+size_t mdt_conv1x1_act8_backward_workspace_bytes(long long n_voxels, int c_in, int c_out);
+int mdt_conv1x1_act8_backward(const float *gy, const float *w, const void *x_codes, const void *x_scales, int x_relu, const void *y_codes /* or NULL */,
+                              float *gx, float *gw, float *gbias, float *g, long long n_voxels, int c_in, int c_out,
+                              void *workspace, size_t workspace_bytes, void *stream);
+
+/* rows of k values <-> codes [rows][ceil(k / 32) * 16 bytes] (two a byte, the even value in the low half; 4-byte aligned) and scales [rows][ceil(k / 32)];
+ * a row's last block is padded with zeros */
+int mdt_mx4_quantize(const void *x, void *codes, void *scales, long long rows, long long k, int dtype, void *stream);
+int mdt_mx4_dequantize(const void *codes, const void *scales, void *x, long long rows, long long k, int dtype, void *stream);
+
+/*
+ * y[r][j] = act(sum_i x4[r][i] * w4[j][i] + bias[j]): x4 = x rounded to 4-bit codes in the call, w4 the codes of w [n][k] (16-byte aligned); products and
+ * sums in fp32, one rounding to x's type at the end.  bias: fp32 [n] or NULL.  The box heads' products at inference.
+ */
+size_t mdt_mx4_linear_workspace_bytes(long long rows, long long k, int n);
+int mdt_mx4_linear(const void *x, int dtype, const void *w_codes, const void *w_scales, const float *bias /* or NULL */, void *y,
+                   long long rows, long long k, int n, int relu, void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

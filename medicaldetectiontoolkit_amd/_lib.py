@@ -102,6 +102,15 @@ _SIGNATURES = {
     "mdt_bias_grad_to_channels_last_workspace_bytes": (c_size_t, [c_int, c_int, c_longlong]),
     "mdt_bias_grad_to_channels_last": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_longlong, c_void_p, c_size_t, c_void_p]),
     "mdt_bias_act_backward_ticket": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_longlong, c_int, c_longlong, c_int, c_void_p, c_size_t, c_void_p, c_void_p]),
+    "mdt_act8_quantize": (c_int, [c_void_p, c_void_p, c_void_p, c_longlong, c_int, c_int, c_void_p]),
+    "mdt_act8_restore": (c_int, [c_void_p, c_void_p, c_void_p, c_longlong, c_int, c_int, c_void_p]),
+    "mdt_bias_act_act8_forward": (c_int, [c_void_p] * 6 + [c_longlong, c_int, c_longlong, c_int, c_void_p]),
+    "mdt_conv1x1_act8_backward_workspace_bytes": (c_size_t, [c_longlong, c_int, c_int]),
+    "mdt_conv1x1_act8_backward": (c_int, [c_void_p] * 4 + [c_int] + [c_void_p] * 5 + [c_longlong, c_int, c_int, c_void_p, c_size_t, c_void_p]),
+    "mdt_mx4_quantize": (c_int, [c_void_p, c_void_p, c_void_p, c_longlong, c_longlong, c_int, c_void_p]),
+    "mdt_mx4_dequantize": (c_int, [c_void_p, c_void_p, c_void_p, c_longlong, c_longlong, c_int, c_void_p]),
+    "mdt_mx4_linear_workspace_bytes": (c_size_t, [c_longlong, c_longlong, c_int]),
+    "mdt_mx4_linear": (c_int, [c_void_p, c_int] + [c_void_p] * 4 + [c_longlong, c_longlong, c_int, c_int, c_void_p, c_size_t, c_void_p]),
     "mdt_roi_levels": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p]),
     "mdt_rpn_sample_supported": (c_int, [c_int, c_int, c_int]),
     "mdt_rpn_sample_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),

@@ -1,0 +1,273 @@
+"""Block-scaled numbers (csrc/block_scaled.hip, act8_backward.hip, mx4_linear.hip): activations kept for the backward pass in 8 bits, and products in
+4 bits.
+
+32 consecutive values share one power of two 2^e (scale byte e + 127), the smallest with which no value of the block is clipped:
+max|x| <= Q * 2^e with Q = 255 for the outputs of a ReLU, 127 for signed values in 8 bits, 6 for the magnitudes 0, .5, 1, 1.5, 2, 3, 4, 6 of 4 bits.
+Values are rounded to the nearest code, ties to the even one: a kept value is off by at most half a step of its block, max / 255 (ReLU), max / 127
+(signed).  A positive ReLU output keeps at least the code 1, so the codes hold the ReLU's mask exactly.  A block with an infinity or a NaN reads
+back as NaN.
+
+  checkpoint8(x)                      -> Checkpoint8, .restore()      any float32 / bfloat16 / float16 tensor, 33 bytes for 32 values
+  bias_act_checkpoint8(h, bias, res)  -> (y, Checkpoint8 of y)        the convolution epilogue of utils/fused_epilogue.bias_act that keeps the copy
+  conv1x1_backward8(gy, w, x8, y8)    -> gradients of a 1x1(x1) layer from the kept copies of its input and its output
+  mx4_quantize(x) -> Mx4, .dequantize();  mx4_linear(x, w4, bias)     act(x W^T + bias) with both operands in 4 bits (inference)
+
+Like every operator of this package they run on the GPU only and are queued on the current stream of the tensors' device; a tensor that was made on
+another stream is the caller's to synchronise, as with any torch operator.  Their scratch memory comes from torch's allocator for each call, so
+calls on several streams and captured graphs do not share any."""
+import math
+
+import torch
+
+from .. import _lib
+
+BLOCK = 32
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _call(device, name, *args):
+    """the C entry on `device`'s current stream"""
+    fn = getattr(_lib.lib(), name)
+    idx = device.index
+    if idx == torch.cuda.current_device():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(idx))
+    else:
+        with torch.cuda.device(idx):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(idx))
+    if rc != 0:
+        _lib.check(rc, name)
+
+
+def _ptr(t):
+    return t.data_ptr() if t is not None else None
+
+
+def _float_tensor(x, name):
+    if x.dtype not in _DTYPES:
+        raise TypeError("%s: float32, bfloat16 or float16, not %s" % (name, x.dtype))
+    _lib.require_cuda(x, name)
+
+
+def _same_device(ref, **tensors):
+    for name, t in tensors.items():
+        if t is not None and t.device != ref:
+            raise ValueError("%s is on %s, the other operands on %s" % (name, t.device, ref))
+
+
+def _no_graph(what, *tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError("%s records no autograd graph: call it under torch.no_grad()" % what)
+
+
+def _channels_last_stride(shape):
+    """strides of a dense tensor whose axis 1 is the innermost"""
+    stride, s = [0] * len(shape), shape[1]
+    stride[1] = 1
+    for d in list(range(len(shape) - 1, 1, -1)) + [0]:
+        stride[d] = s
+        s *= shape[d]
+    return tuple(stride)
+
+
+def _row_stride(shape):
+    stride, s = [0] * len(shape), 1
+    for d in range(len(shape) - 1, -1, -1):
+        stride[d] = s
+        s *= shape[d]
+    return tuple(stride)
+
+
+def _rows_format(dim):
+    return torch.channels_last_3d if dim == 5 else torch.channels_last if dim == 4 else torch.contiguous_format
+
+
+def _dense(x):
+    """x, or a row-major copy where its storage is neither row-major nor channels-last; and whether its channels (axis 1) are innermost"""
+    if x.dim() in (4, 5) and x.is_contiguous(memory_format=_rows_format(x.dim())):
+        return x, True
+    if not x.is_contiguous():
+        x = x.contiguous()
+    return x, x.dim() == 2
+
+
+class Checkpoint8(object):
+    """An activation kept in 8 bits: `codes` (uint8, one a value, storage order) and `scales` (uint8, one for 32 codes).  `channels_last`: axis 1 is the
+    innermost of the storage (for two axes it always is)."""
+    __slots__ = ("codes", "scales", "shape", "relu", "dtype", "channels_last")
+
+    def __init__(self, codes, scales, shape, relu=False, dtype=torch.float32, channels_last=None):
+        shape = tuple(int(s) for s in shape)
+        n = math.prod(shape)
+        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or codes.numel() != n or scales.numel() != -(-n // BLOCK):
+            raise ValueError("Checkpoint8: %d uint8 codes and %d uint8 scales for shape %s, got %d %s and %d %s"
+                             % (n, -(-n // BLOCK), shape, codes.numel(), codes.dtype, scales.numel(), scales.dtype))
+        if not codes.is_contiguous() or not scales.is_contiguous() or codes.data_ptr() % 4 != 0:
+            raise ValueError("Checkpoint8: codes and scales are contiguous, the codes 4-byte aligned")
+        if dtype not in _DTYPES:
+            raise TypeError("Checkpoint8: float32, bfloat16 or float16, not %s" % dtype)
+        if channels_last is None:
+            channels_last = len(shape) == 2
+        elif (channels_last and len(shape) not in (2, 4, 5)) or (len(shape) == 2 and not channels_last):
+            raise ValueError("Checkpoint8: channels_last=%s does not describe %d axes" % (channels_last, len(shape)))
+        _same_device(codes.device, scales=scales)
+        self.codes, self.scales, self.shape, self.relu, self.dtype, self.channels_last = codes, scales, shape, bool(relu), dtype, bool(channels_last)
+
+    @property
+    def stride(self):
+        return _channels_last_stride(self.shape) if self.channels_last else _row_stride(self.shape)
+
+    def restore(self):
+        """the kept values, in the type, shape and storage order of the tensor they were taken from"""
+        _lib.require_cuda(self.codes, "Checkpoint8.codes")
+        x = torch.empty_strided(self.shape, self.stride, dtype=self.dtype, device=self.codes.device)
+        _call(x.device, "mdt_act8_restore", self.codes.data_ptr(), self.scales.data_ptr(), x.data_ptr(), x.numel(), _DTYPES[self.dtype], int(self.relu))
+        return x
+
+
+def _new_codes(n, device):
+    return torch.empty(n, dtype=torch.uint8, device=device), torch.empty(-(-n // BLOCK), dtype=torch.uint8, device=device)
+
+
+def checkpoint8(x, relu=False):
+    """x's values in 8 bits.  relu=True: x is the output of a ReLU (values <= 0 read back as 0) and is kept with twice the resolution."""
+    _float_tensor(x, "x")
+    x, cl = _dense(x.detach())
+    codes, scales = _new_codes(x.numel(), x.device)
+    _call(x.device, "mdt_act8_quantize", x.data_ptr(), codes.data_ptr(), scales.data_ptr(), x.numel(), _DTYPES[x.dtype], int(relu))
+    return Checkpoint8(codes, scales, x.shape, relu, x.dtype, cl)
+
+
+def bias_act_checkpoint8(h, bias, residual=None, relu=True, inplace=False):
+    """(y, Checkpoint8 of y), y = act(h + bias[c] (+ residual)): fused_epilogue.bias_act (the same roundings) with y's 8-bit copy from the same pass.
+    h: float32 [N, C, ...], row-major or channels-last; inplace: y overwrites h."""
+    _float_tensor(h, "h")
+    if h.dtype != torch.float32 or bias.dtype != torch.float32 or (residual is not None and residual.dtype != torch.float32):
+        raise TypeError("bias_act_checkpoint8: float32 operands")
+    if h.dim() < 2 or tuple(bias.shape) != (h.shape[1],) or (residual is not None and residual.shape != h.shape):
+        raise ValueError("bias_act_checkpoint8: bias %s and residual %s do not fit h %s"
+                         % (tuple(bias.shape), None if residual is None else tuple(residual.shape), tuple(h.shape)))
+    _same_device(h.device, bias=bias, residual=residual)
+    _no_graph("bias_act_checkpoint8", h, bias, residual)
+    x, cl = _dense(h)
+    if inplace and x is not h:
+        raise ValueError("bias_act_checkpoint8: inplace needs a dense row-major or channels-last h")
+    inner = 1 if cl else math.prod(x.shape[2:])
+    if residual is not None and residual.stride() != x.stride():
+        residual = residual.contiguous(memory_format=_rows_format(x.dim()) if cl else torch.contiguous_format)
+    if not bias.is_contiguous():
+        bias = bias.contiguous()
+    y = x if inplace else torch.empty_like(x)
+    codes, scales = _new_codes(x.numel(), x.device)
+    if x.numel():
+        _call(x.device, "mdt_bias_act_act8_forward", y.data_ptr(), x.data_ptr(), bias.data_ptr(), _ptr(residual), codes.data_ptr(), scales.data_ptr(), x.numel(),
+              int(x.shape[1]), inner, int(relu))
+    return y, Checkpoint8(codes, scales, x.shape, relu, x.dtype, cl)
+
+
+def conv1x1_backward8(gy, w, x8, y8=None, need_g=False, need_gx=True, need_gw=True):
+    """(gx, gw, gbias, g) of y = act(conv1x1(x, w) + bias (+ residual)) at unit stride, from the 8-bit copies of x and y.
+
+    gy: float32 [V, C_out] or [N, C_out, ...]; w: float32 [C_out, C_in(, 1, 1(, 1))]; x8: the kept input, channels innermost; y8: the kept ReLU output
+    (None: no activation).  g = gy * (y > 0) is the residual's gradient (None unless need_g); gx comes in x's shape and storage order."""
+    if gy.dtype != torch.float32 or w.dtype != torch.float32:
+        raise TypeError("conv1x1_backward8: float32 gradients and weights")
+    _lib.require_cuda(gy, "gy")
+    if w.dim() < 2 or math.prod(w.shape[2:]) != 1:
+        raise ValueError("conv1x1_backward8: a 1x1(x1) filter, not %s" % (tuple(w.shape),))
+    co, ci = int(w.shape[0]), int(w.shape[1])
+    shape = tuple(gy.shape)
+    if gy.dim() not in (2, 4, 5) or shape[1] != co or x8.shape != shape[:1] + (ci,) + shape[2:]:
+        raise ValueError("conv1x1_backward8: gy %s, w %s and x8 %s do not belong together" % (shape, tuple(w.shape), x8.shape))
+    if not x8.channels_last or (y8 is not None and not y8.channels_last):
+        raise ValueError("conv1x1_backward8: the kept maps have their channels innermost")
+    if y8 is not None and (y8.shape != shape or not y8.relu):
+        raise ValueError("conv1x1_backward8: y8 is the kept ReLU output of gy's shape")
+    _same_device(gy.device, w=w, x8=x8.codes, y8=None if y8 is None else y8.codes)
+    dev = gy.device
+    gy = gy.detach()
+    mf = _rows_format(gy.dim())
+    if not gy.is_contiguous(memory_format=mf):
+        gy = gy.contiguous(memory_format=mf)
+    wm = w.detach().reshape(co, ci)
+    if not wm.is_contiguous():
+        wm = wm.contiguous()
+    V = gy.numel() // co
+    gx = torch.empty_strided(x8.shape, x8.stride, dtype=torch.float32, device=dev) if need_gx else None
+    gw = torch.empty(co, ci, dtype=torch.float32, device=dev) if need_gw else None
+    gbias = torch.empty(co, dtype=torch.float32, device=dev)
+    write_g = need_g and y8 is not None
+    g = torch.empty_like(gy) if write_g else None
+    ws = torch.empty(_lib.lib().mdt_conv1x1_act8_backward_workspace_bytes(V, ci, co), dtype=torch.uint8, device=dev)
+    _call(dev, "mdt_conv1x1_act8_backward", gy.data_ptr(), wm.data_ptr(), x8.codes.data_ptr(), x8.scales.data_ptr(), int(x8.relu), _ptr(y8.codes if y8 is not None else None),
+          _ptr(gx), _ptr(gw), gbias.data_ptr(), _ptr(g), V, ci, co, ws.data_ptr(), ws.numel())
+    return gx, (gw.view(w.shape) if gw is not None else None), gbias, (g if write_g else gy if need_g else None)
+
+
+class Mx4(object):
+    """Rows in 4 bits: `codes` uint8 [..., ceil(k / 32) * 16] (two a byte, the even value in the low half), `scales` uint8 [..., ceil(k / 32)]; blocks run along
+    the last axis of length k."""
+    __slots__ = ("codes", "scales", "k", "dtype")
+
+    def __init__(self, codes, scales, k, dtype=torch.float32):
+        k = int(k)
+        kb = -(-k // BLOCK)
+        if k < 1 or codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or codes.dim() < 1 or codes.shape[-1] != 16 * kb \
+                or tuple(scales.shape) != tuple(codes.shape[:-1]) + (kb,):
+            raise ValueError("Mx4: uint8 codes [..., %d] and scales [..., %d] for rows of %d, got %s %s and %s %s"
+                             % (16 * kb, kb, k, tuple(codes.shape), codes.dtype, tuple(scales.shape), scales.dtype))
+        if not codes.is_contiguous() or not scales.is_contiguous() or codes.data_ptr() % 16 != 0:
+            raise ValueError("Mx4: codes and scales are contiguous, the codes 16-byte aligned")
+        if dtype not in _DTYPES:
+            raise TypeError("Mx4: float32, bfloat16 or float16, not %s" % dtype)
+        _same_device(codes.device, scales=scales)
+        self.codes, self.scales, self.k, self.dtype = codes, scales, k, dtype
+
+    @property
+    def shape(self):
+        return tuple(self.codes.shape[:-1]) + (self.k,)
+
+    def dequantize(self):
+        """the values the codes stand for, in the type of the tensor they were taken from"""
+        _lib.require_cuda(self.codes, "Mx4.codes")
+        x = torch.empty(self.shape, dtype=self.dtype, device=self.codes.device)
+        _call(x.device, "mdt_mx4_dequantize", self.codes.data_ptr(), self.scales.data_ptr(), x.data_ptr(), x.numel() // self.k, self.k, _DTYPES[self.dtype])
+        return x
+
+
+def mx4_quantize(x):
+    """x's rows (last axis) in 4 bits"""
+    _float_tensor(x, "x")
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError("mx4_quantize: rows of at least one value, not %s" % (tuple(x.shape),))
+    x = x.detach()
+    if not x.is_contiguous():
+        x = x.contiguous()
+    k = int(x.shape[-1])
+    kb = -(-k // BLOCK)
+    codes = torch.empty(x.shape[:-1] + (16 * kb,), dtype=torch.uint8, device=x.device)
+    scales = torch.empty(x.shape[:-1] + (kb,), dtype=torch.uint8, device=x.device)
+    _call(x.device, "mdt_mx4_quantize", x.data_ptr(), codes.data_ptr(), scales.data_ptr(), x.numel() // k, k, _DTYPES[x.dtype])
+    return Mx4(codes, scales, k, x.dtype)
+
+
+def mx4_linear(x, w4, bias=None, relu=False):
+    """act(x W^T + bias) in x's type: x [..., K] (float32, bfloat16 or float16) is rounded to 4 bits in the call, w4 = mx4_quantize(W) for W [N, K]; products and
+    sums in float32.  bias: [N], taken in float32.  For inference: no autograd graph."""
+    _float_tensor(x, "x")
+    if len(w4.shape) != 2 or x.dim() < 1 or x.shape[-1] != w4.k or (bias is not None and tuple(bias.shape) != (w4.shape[0],)):
+        raise ValueError("mx4_linear: x %s, W %s and bias %s do not fit" % (tuple(x.shape), w4.shape, None if bias is None else tuple(bias.shape)))
+    _same_device(x.device, w4=w4.codes, bias=bias)
+    _no_graph("mx4_linear", x, bias)
+    n, k = w4.shape
+    if not x.is_contiguous():
+        x = x.contiguous()
+    if bias is not None and (bias.dtype != torch.float32 or not bias.is_contiguous()):
+        bias = bias.float().contiguous()
+    rows = x.numel() // k
+    y = torch.empty(x.shape[:-1] + (n,), dtype=x.dtype, device=x.device)
+    if y.numel() == 0:
+        return y
+    ws = torch.empty(_lib.lib().mdt_mx4_linear_workspace_bytes(rows, k, n), dtype=torch.uint8, device=x.device)
+    _call(x.device, "mdt_mx4_linear", x.data_ptr(), _DTYPES[x.dtype], w4.codes.data_ptr(), w4.scales.data_ptr(), _ptr(bias), y.data_ptr(), rows, k, n, int(relu), ws.data_ptr(),
+          ws.numel())
+    return y

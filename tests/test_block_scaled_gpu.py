@@ -1,0 +1,456 @@
+"""Block-scaled operators (utils/block_scaled.py) against the formats' and the formulas' definition in 64 bits.
+
+Codes and kept values are compared bit for bit.  Products are compared twice: on small integers, where every product and sum is exact in fp32 and the
+result has to be equal (a missing or a doubled term shows), and on floats within the rounding errors counted beside each test."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from medicaldetectiontoolkit_amd.utils import block_scaled as bs
+from medicaldetectiontoolkit_amd.utils import fused_epilogue as fe
+
+pytestmark = pytest.mark.gpu
+
+GRID = np.array([0, 0.5, 1, 1.5, 2, 3, 4, 6])
+BIG = {torch.float32: float(np.finfo(np.float32).max), torch.bfloat16: 3.3895313892515355e38, torch.float16: 65504.0}
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+# ---- the definition --------------------------------------------------------------------------------------------------------------
+def scale_bytes(m, q):
+    """the smallest e >= -127 with m <= q 2^e, searched from below the answer"""
+    e = np.full(m.shape, -127.0)
+    fin = np.isfinite(m)
+    mm = np.where(fin, m, 0.0)
+    pos = mm > 0
+    e[pos] = np.maximum(-127, np.floor(np.log2(mm[pos] / q)) - 1)
+    for _ in range(4):
+        e = np.where(mm > q * np.exp2(e), e + 1, e)
+    return np.where(fin, e + 127, 255).astype(np.int64)
+
+
+def half_even(t):
+    return np.rint(t)          # numpy rounds halves to even
+
+
+def kept8(x, relu, big):
+    """codes, scale bytes and values of the flat float64 array x"""
+    n = x.size
+    p = np.concatenate([x, np.zeros(-n % 32)]).reshape(-1, 32)
+    mag = np.where(p < 0, 0.0, p) if relu else np.abs(p)
+    bad = ~np.isfinite(mag).all(1)
+    m = np.where(bad, np.inf, np.where(np.isfinite(mag), mag, 0).max(1))
+    b = scale_bytes(m, 255.0 if relu else 127.0)
+    s = np.exp2(np.where(bad, 0, b - 127.0))[:, None]
+    with np.errstate(invalid="ignore"):
+        q = half_even(np.where(bad[:, None], 0.0, p / s))
+        if relu:
+            q = np.where(p > 0, np.maximum(q, 1), 0)
+    if relu:
+        q = np.where(bad[:, None], (p > 0).astype(float), q)
+    v = np.where(bad[:, None], np.nan, np.clip(q * s, -big, big))
+    return q.reshape(-1)[:n], b, v.reshape(-1)[:n]
+
+
+def kept4(x, big):
+    """values [r, k] and scale bytes [r, blocks] of float64 rows"""
+    r, k = x.shape
+    p = np.concatenate([x, np.zeros((r, -k % 32))], 1).reshape(r, -1, 32)
+    bad = ~np.isfinite(p).all(2)
+    m = np.where(bad, np.inf, np.abs(np.where(np.isfinite(p), p, 0)).max(2))
+    b = scale_bytes(m, 6.0)
+    s = np.exp2(np.where(bad, 0, b - 127.0))[..., None]
+    a = np.abs(np.where(bad[..., None], 0, p)) / s
+    q = np.zeros_like(a)
+    for c in range(1, 8):
+        mid = (GRID[c - 1] + GRID[c]) / 2
+        q = np.where((a >= mid) if c % 2 == 0 else (a > mid), GRID[c], q)
+    v = np.where(bad[..., None], np.nan, np.clip(np.copysign(q, p) * s, -big, big))
+    return v.reshape(r, -1)[:, :k], b
+
+
+def hard_values(n, dtype, seed):
+    """numbers of very different size, with the places where a format can go wrong"""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(n, generator=g) * torch.exp2(torch.randint(-12, 12, (n,), generator=g).float())
+    for start, vals in ((0, [0.0] * 32), (32, [255.0, 254.5, 0.5, 1.5, 2.5, -0.0, -3.0, 127.5]), (64, [127.0, 126.5, -127.0, 0.5, -0.5, 1.5]), (96, [127.00001, 1.0]),
+                        (128, [6.0, 5.0, 2.5, 3.5, 1.75, 0.25, 0.75, 1.25, -5.0]), (160, [6.00001, 0.3]), (192, [float("inf"), 1.0, -1.0]), (224, [float("nan"), 2.0, -2.0, 0.0]),
+                        (256, [-float("inf"), 3.0]), (288, [1e-40, 2e-41, -1e-42, 1e-45]), (320, [6.1e-5, 5.9e-8, -1e-7]), (352, [BIG[dtype], 1.0, -BIG[dtype] / 2, BIG[dtype] * 0.9]),
+                        (384, [1e-30, 1e30 if dtype != torch.float16 else 6e4])):
+        if start + 32 <= n:
+            x[start:start + 32] = 0
+            x[start:start + len(vals)] = torch.tensor(vals)
+    return x.to(dtype)
+
+
+def f64(t):
+    return t.detach().cpu().double().numpy()
+
+
+def same(got, want):
+    return np.array_equal(got, want, equal_nan=True)
+
+
+# ---- 8 bits ------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("relu", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [1, 7, 31, 32, 33, 100, 416, 1000, 70001])
+def test_checkpoint8_codes_scales_and_values(cuda, n, dtype, relu):
+    x = hard_values(n, dtype, n)
+    ck = bs.checkpoint8(x.to(cuda), relu=relu)
+    q, b, v = kept8(f64(x), relu, BIG[dtype])
+    codes = ck.codes.cpu().numpy()
+    fin = np.repeat(b, 32)[:n] != 255
+    assert same(np.where(fin | relu, codes if relu else codes.view(np.int8), 0), np.where(fin | relu, q, 0))
+    assert same(ck.scales.cpu().numpy(), b)
+    back = ck.restore()
+    assert back.dtype == dtype and back.shape == x.shape
+    assert same(f64(back), v)
+    if relu:
+        assert same(codes > 0, f64(x) > 0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_checkpoint8_large_tensor_takes_the_same_path_values(cuda, dtype):
+    """sizes on both sides of the switch to four groups a thread (2^21 groups of 16 bytes), not a multiple of anything"""
+    for n in (2 ** 21 * (4 if dtype == torch.float32 else 8) - 3, 2 ** 21 * (4 if dtype == torch.float32 else 8) + 37):
+        x = (torch.randn(n, generator=torch.Generator().manual_seed(3)) * 5).to(dtype)
+        for relu in (False, True):
+            ck = bs.checkpoint8(x.to(cuda), relu=relu)
+            q, b, v = kept8(f64(x), relu, BIG[dtype])
+            assert same(ck.scales.cpu().numpy(), b)
+            assert same(f64(ck.restore()), v)
+
+
+@pytest.mark.parametrize("shape", [(2, 3, 5, 7), (2, 18, 4, 6, 8), (1, 1, 9, 9), (3, 5), (4,), (2, 40, 1, 1, 1), (3, 0, 4, 4), (2, 4, 6)])
+@pytest.mark.parametrize("form", ["rows", "cl", "sliced", "transposed"])
+def test_checkpoint8_layouts(cuda, shape, form):
+    """blocks run along the storage; what is restored has the values, the shape and (for dense tensors) the strides of the original"""
+    x = torch.randn(shape, generator=torch.Generator().manual_seed(1)).to(cuda)
+    if form == "cl":
+        if x.dim() not in (4, 5):
+            pytest.skip("channels-last: 4 or 5 axes")
+        x = x.contiguous(memory_format=bs._rows_format(x.dim()))
+    elif form == "sliced":
+        x = torch.randn((2,) + shape, device=cuda).movedim(0, -1)[..., 0]
+    elif form == "transposed" and x.dim() >= 2:
+        x = x.transpose(0, -1)
+    ck = bs.checkpoint8(x)
+    back = ck.restore()
+    assert back.shape == x.shape
+    want = x if form == "cl" else x.contiguous()
+    assert back.numel() == 0 or back.stride() == want.stride() or 1 in shape
+    flat = want.movedim(1, -1).reshape(-1) if ck.channels_last and x.dim() > 2 else want.reshape(-1)
+    got = back.movedim(1, -1).reshape(-1) if ck.channels_last and x.dim() > 2 else back.reshape(-1)
+    assert same(f64(got), kept8(f64(flat), False, BIG[torch.float32])[2])
+
+
+def test_restore_of_every_code_and_scale(cuda):
+    """all 256 codes under all 256 scale bytes, saturation at the type's largest value included"""
+    codes = torch.arange(256, dtype=torch.uint8).repeat(256).to(cuda)
+    scales = torch.arange(256, dtype=torch.uint8).repeat_interleave(8).to(cuda)
+    b = np.arange(256).repeat(256).astype(float)
+    for relu in (False, True):
+        c = np.tile(np.arange(256), 256)
+        c = c if relu else c.astype(np.uint8).view(np.int8)
+        for dtype in DTYPES:
+            got = bs.Checkpoint8(codes, scales, (65536,), relu, dtype).restore()
+            exact = torch.from_numpy(np.where(b == 255, np.nan, np.clip(c * np.exp2(b - 127), -BIG[dtype], BIG[dtype])))
+            assert same(f64(got), f64(exact.to(dtype)))
+
+
+@pytest.mark.parametrize("relu", [True, False])
+@pytest.mark.parametrize("residual", [True, False])
+@pytest.mark.parametrize("form", ["cl", "rows"])
+@pytest.mark.parametrize("shape", [(2, 18, 8, 8, 16), (1, 1, 3, 5), (3, 7, 5, 3, 1), (2, 72, 33, 31), (1, 300, 1, 1), (8, 18, 32, 32, 128), (5, 3), (4, 36, 1, 0, 3)])
+def test_bias_act_checkpoint8(cuda, shape, form, residual, relu):
+    g = torch.Generator(device=cuda).manual_seed(7)
+    mf = bs._rows_format(len(shape)) if form == "cl" else torch.contiguous_format
+    h = torch.randn(shape, generator=g, device=cuda).contiguous(memory_format=mf)
+    r = torch.randn(shape, generator=g, device=cuda).contiguous(memory_format=mf) if residual else None
+    bias = torch.randn(shape[1], generator=g, device=cuda)
+    keep = h.clone()
+    y, ck = bs.bias_act_checkpoint8(h, bias, r, relu=relu)
+    assert torch.equal(h, keep) and y.stride() == h.stride()
+    want = fe.bias_act(h.clone(), bias, r, relu) if h.numel() and len(shape) > 2 else None
+    if want is None:
+        want = h + bias.view([1, -1] + [1] * (h.dim() - 2))
+        want = want + r if residual else want
+        want = want.clamp(min=0) if relu else want
+    assert torch.equal(y, want)
+    other = bs.checkpoint8(y, relu=relu)
+    assert torch.equal(ck.codes, other.codes) and torch.equal(ck.scales, other.scales)
+    y2, ck2 = bs.bias_act_checkpoint8(h, bias, r, relu=relu, inplace=True)
+    assert y2.data_ptr() == h.data_ptr() and torch.equal(h, y) and torch.equal(ck2.codes, ck.codes)
+
+
+def test_bias_act_checkpoint8_takes_a_residual_of_another_layout(cuda):
+    h = torch.randn(2, 6, 5, 7, device=cuda).contiguous(memory_format=torch.channels_last)
+    r = torch.randn(2, 6, 5, 7, device=cuda)
+    bias = torch.randn(12, device=cuda)[::2]
+    y, ck = bs.bias_act_checkpoint8(h, bias, r)
+    assert torch.equal(y, (h + bias.view(1, -1, 1, 1) + r).clamp(min=0))
+
+
+# ---- the backward pass of a 1x1 layer ----------------------------------------------------------------------------------------------
+SHAPES = [(1, 1, 1), (1, 18, 72), (5, 3, 3), (31, 18, 72), (33, 72, 18), (693, 18, 72), (700, 72, 18), (257, 37, 101), (64, 32, 32), (100, 65, 33), (4100, 36, 144), (2000, 144, 36),
+          (96, 200, 300), (513, 576, 144)]
+
+
+def layer(V, ci, co, integers, seed, cuda):
+    g = torch.Generator().manual_seed(seed)
+    if integers:
+        x = torch.randint(0, 16, (V, ci), generator=g).float()
+        gy = torch.randint(-8, 9, (V, co), generator=g).float()
+        w = torch.randint(-8, 9, (co, ci), generator=g).float()
+    else:
+        x = torch.randn(V, ci, generator=g).relu() * torch.exp(torch.randn(ci, generator=g))
+        gy = torch.randn(V, co, generator=g) * torch.exp(torch.randn(V, 1, generator=g) * 1.5 - 7)
+        w = torch.randn(co, ci, generator=g)
+    y = torch.randn(V, co, generator=g).relu()
+    return x.to(cuda), gy.to(cuda), w.to(cuda), y.to(cuda)
+
+
+def depth(V):
+    """additions one sum can pass through: each of the products of one fp32 chain and the joins of partial sums"""
+    return V + 64
+
+
+@pytest.mark.parametrize("relu", [True, False])
+@pytest.mark.parametrize("V,ci,co", SHAPES)
+def test_conv1x1_backward8_is_exact_on_integers(cuda, V, ci, co, relu):
+    x, gy, w, y = layer(V, ci, co, True, V + ci, cuda)
+    x8, y8 = bs.checkpoint8(x, relu=True), bs.checkpoint8(y, relu=True) if relu else None
+    assert torch.equal(x8.restore(), x)                       # 0 .. 15 are kept exactly
+    gx, gw, gb, g = bs.conv1x1_backward8(gy, w, x8, y8, need_g=True)
+    m = gy * (y > 0) if relu else gy
+    assert torch.equal(g, m)
+    md, xd, wd = m.cpu().double(), x.cpu().double(), w.cpu().double()
+    assert torch.equal(gx.cpu().double(), md @ wd)
+    assert torch.equal(gw.cpu().double(), md.t() @ xd)
+    assert torch.equal(gb.cpu().double(), md.sum(0))
+
+
+@pytest.mark.parametrize("signed", [False, True])
+@pytest.mark.parametrize("V,ci,co", SHAPES)
+def test_conv1x1_backward8_on_floats(cuda, V, ci, co, signed):
+    """gw: exact products (a bf16 input, a gradient cut exactly), so only the sums round, depth(3 V) times half a step of at most the summed magnitudes;
+    gx: the same over 6 C_out products, plus the pieces left out (2^-24 of each product, and as much again for the next order)"""
+    x, gy, w, y = layer(V, ci, co, False, V + co, cuda)
+    x = x - 0.3 if signed else x
+    x8, y8 = bs.checkpoint8(x, relu=not signed), bs.checkpoint8(y, relu=True)
+    gx, gw, gb, g = bs.conv1x1_backward8(gy, w, x8, y8)
+    assert g is None
+    md, xd, wd = (gy * (y > 0)).cpu().double(), x8.restore().cpu().double(), w.cpu().double()
+    eps = 2.0 ** -24
+    assert ((gw.cpu().double() - md.t() @ xd).abs() <= depth(3 * V) * eps * (md.abs().t() @ xd.abs())).all()
+    assert ((gx.cpu().double() - md @ wd).abs() <= (depth(6 * co) + 2) * eps * (md.abs() @ wd.abs())).all()
+    assert ((gb.cpu().double() - md.sum(0)).abs() <= depth(V) * eps * md.abs().sum(0)).all()
+
+
+def test_conv1x1_backward8_long_sum_keeps_fp32_accuracy(cuda):
+    """as many voxels as a first stage's maps: the error of a sum in 2-norm stays near one fp32 rounding"""
+    x, gy, w, y = layer(262144, 18, 72, False, 5, cuda)
+    x8, y8 = bs.checkpoint8(x, relu=True), bs.checkpoint8(y, relu=True)
+    gx, gw, gb, _ = bs.conv1x1_backward8(gy, w, x8, y8)
+    md, xd = (gy * (y > 0)).double(), x8.restore().double()
+    for got, want in ((gw, md.t() @ xd), (gx, md @ w.double()), (gb, md.sum(0))):
+        assert float((got.double() - want).norm() / want.norm()) < 1e-6
+    again = bs.conv1x1_backward8(gy, w, x8, y8)
+    assert torch.equal(again[0], gx) and torch.equal(again[1], gw) and torch.equal(again[2], gb)
+
+
+@pytest.mark.parametrize("shape", [(2, 72, 4, 6, 8), (3, 72, 9, 5)])
+def test_conv1x1_backward8_on_maps(cuda, shape):
+    """channels-last maps in, gradients in the maps' own shape and storage; a row-major gradient is taken, too"""
+    mf = bs._rows_format(len(shape))
+    ci, co = 18, shape[1]
+    x = torch.randint(0, 16, shape[:1] + (ci,) + shape[2:], device=cuda).float().contiguous(memory_format=mf)
+    gy = torch.randint(-8, 9, shape, device=cuda).float()
+    w = torch.randint(-8, 9, (co, ci) + (1,) * (len(shape) - 2), device=cuda).float()
+    y = torch.randn(shape, device=cuda).relu().contiguous(memory_format=mf)
+    x8, y8 = bs.checkpoint8(x, relu=True), bs.checkpoint8(y, relu=True)
+    wide = torch.zeros(w.shape[:1] + (2 * ci,) + w.shape[2:], device=cuda)
+    wide[:, ::2] = w
+    for a, f in ((gy, w), (gy.contiguous(memory_format=mf), w), (gy.repeat_interleave(2, 1)[:, ::2], wide[:, ::2])):
+        gx, gw, gb, g = bs.conv1x1_backward8(a, f, x8, y8, need_g=True)
+        m = gy * (y > 0)
+        conv = torch.nn.functional.conv3d if len(shape) == 5 else torch.nn.functional.conv2d
+        xc, wc = x.cpu().double().requires_grad_(), w.cpu().double().requires_grad_()
+        conv(xc, wc).backward(m.cpu().double())
+        assert torch.equal(gx.cpu().double(), xc.grad) and gx.stride() == x.stride()
+        assert torch.equal(gw.cpu().double(), wc.grad) and gw.shape == w.shape
+        assert torch.equal(g, m) and torch.equal(gb.cpu().double(), m.cpu().double().sum([d for d in range(m.dim()) if d != 1]))
+
+
+def test_conv1x1_backward8_wanted_parts_and_no_rows(cuda):
+    x, gy, w, y = layer(300, 20, 40, True, 1, cuda)
+    x8, y8 = bs.checkpoint8(x, relu=True), bs.checkpoint8(y, relu=True)
+    full = bs.conv1x1_backward8(gy, w, x8, y8, need_g=True)
+    for kw in (dict(need_gx=False), dict(need_gw=False), dict(need_gx=False, need_gw=False), dict(need_gx=False, need_g=True), dict(need_gx=False, need_gw=False, need_g=True)):
+        got = bs.conv1x1_backward8(gy, w, x8, y8, **kw)
+        assert (got[0] is None) == (not kw.get("need_gx", True)) and (got[1] is None) == (not kw.get("need_gw", True)) and (got[3] is None) == (not kw.get("need_g", False))
+        assert all(a is None or torch.equal(a, b) for a, b in zip(got, full))
+    none = bs.checkpoint8(torch.zeros(0, 20, device=cuda), relu=True)
+    gx, gw, gb, g = bs.conv1x1_backward8(torch.zeros(0, 40, device=cuda), w, none, None, need_g=True)
+    assert gx.shape == (0, 20) and not gw.any() and not gb.any() and g.shape == (0, 40)
+
+
+def test_conv1x1_backward8_masked_rows_hide_non_finite_gradients(cuda):
+    """where the ReLU was closed, an infinity or a NaN in gy leaves no trace; where it was open, it shows"""
+    x, gy, w, y = layer(100, 18, 72, True, 3, cuda)
+    y[10:20] = 0
+    x8, y8 = bs.checkpoint8(x, relu=True), bs.checkpoint8(y, relu=True)
+    want = bs.conv1x1_backward8(gy, w, x8, y8, need_g=True)
+    bad = gy.clone()
+    bad[10:15], bad[15:20] = float("inf"), float("nan")
+    for a, b in zip(bs.conv1x1_backward8(bad, w, x8, y8, need_g=True), want):
+        assert torch.equal(a, b)
+    y[0, 0] = 1.0
+    bad[0, 0] = float("inf")
+    gx, gw, gb, g = bs.conv1x1_backward8(bad, w, x8, bs.checkpoint8(y, relu=True), need_g=True)
+    assert not torch.isfinite(gx[0]).any() and torch.isfinite(gx[1:]).all() and not torch.isfinite(gw[0]).any() and torch.isfinite(gw[1:]).all() and not torch.isfinite(gb[0])
+
+
+# ---- 4 bits ------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,k", [(1, 1), (1, 31), (3, 32), (2, 33), (1, 416), (7, 100), (5, 1000), (130, 64), (2, 5292), (4099, 7)])
+def test_mx4_codes_and_values(cuda, rows, k, dtype):
+    x = hard_values(rows * k, dtype, k).view(rows, k)
+    m = bs.mx4_quantize(x.to(cuda))
+    v, b = kept4(f64(x), BIG[dtype])
+    assert m.codes.shape == (rows, -(-k // 32) * 16) and same(m.scales.cpu().numpy(), b)
+    got = m.dequantize()
+    assert got.dtype == dtype and same(f64(got), v)
+    lo, hi = m.codes.cpu().numpy() & 15, m.codes.cpu().numpy() >> 4
+    c = np.stack([lo, hi], -1).reshape(rows, -1)
+    assert not c[:, k:].any()                                            # the padding holds zeros
+    ok = np.repeat(b, 32, 1)[:, :k] != 255
+    val = np.where(c >= 8, -1, 1) * GRID[c & 7]
+    want = np.where(ok, v / np.exp2(np.repeat(b, 32, 1)[:, :k] - 127.0), 0)
+    clipped = np.abs(v) == BIG[dtype]
+    assert same(np.where(clipped, 0, val[:, :k]), np.where(clipped, 0, want))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_mx4_large(cuda, dtype):
+    x = (torch.randn(3001, 5291, generator=torch.Generator().manual_seed(0)) * 3).to(dtype)
+    v, b = kept4(f64(x), BIG[dtype])
+    m = bs.mx4_quantize(x.to(cuda))
+    assert same(m.scales.cpu().numpy(), b) and same(f64(m.dequantize()), v)
+
+
+def test_mx4_keeps_leading_axes_and_takes_any_strides(cuda):
+    x = torch.randn(3, 4, 70, device=cuda)
+    m = bs.mx4_quantize(x)
+    assert m.shape == (3, 4, 70) and torch.equal(m.dequantize(), bs.mx4_quantize(x.view(12, 70)).dequantize().view(3, 4, 70))
+    t = x.transpose(0, 2)
+    assert torch.equal(bs.mx4_quantize(t).dequantize(), bs.mx4_quantize(t.contiguous()).dequantize())
+    assert bs.mx4_quantize(x[:0]).dequantize().shape == (0, 4, 70)
+
+
+LINEAR = [(1, 1, 1), (1, 5292, 144), (3, 33, 5), (31, 64, 32), (33, 100, 33), (130, 5292, 144), (257, 31, 7), (64, 2048, 768), (1000, 144, 144), (515, 1000, 300), (129, 9408, 65)]
+
+
+@pytest.mark.parametrize("relu", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,k,n", LINEAR)
+def test_mx4_linear_is_exact_on_integers(cuda, rows, k, n, dtype, relu):
+    """rows of 0, +-1, +-2, +-3, +-4, +-6 are kept exactly and their sums are fp32 integers below 2^24: the result is the exact one, rounded once"""
+    g = torch.Generator().manual_seed(k + n)
+    vals = torch.tensor([0.0, 1, 2, 3, 4, 6, -1, -2, -3, -4, -6])
+    x, w = vals[torch.randint(0, 11, (rows, k), generator=g)], vals[torch.randint(0, 11, (n, k), generator=g)]
+    bias = torch.randint(-9, 9, (n,), generator=g).float()
+    y = bs.mx4_linear(x.to(dtype).to(cuda), bs.mx4_quantize(w.to(cuda)), bias.to(cuda), relu=relu)
+    want = x.double() @ w.double().t() + bias.double()
+    want = want.clamp(min=0) if relu else want
+    assert y.dtype == dtype and torch.equal(y.cpu(), want.to(dtype))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,k,n", LINEAR)
+def test_mx4_linear_on_floats(cuda, rows, k, n, dtype):
+    """products are exact (2 + 2 significant bits); k sums and the bias round in fp32, at most half a step of the summed magnitudes each; then one rounding
+    to the type"""
+    g = torch.Generator().manual_seed(rows + n)
+    x = (torch.randn(rows, k, generator=g) * torch.exp(torch.randn(k, generator=g))).to(dtype)
+    w, bias = torch.randn(n, k, generator=g) / math.sqrt(k), torch.randn(n, generator=g)
+    y = bs.mx4_linear(x.to(cuda), bs.mx4_quantize(w.to(cuda)), bias.to(cuda))
+    xv, wv = torch.from_numpy(kept4(f64(x), BIG[dtype])[0]), torch.from_numpy(kept4(f64(w), BIG[torch.float32])[0])
+    want = xv @ wv.t() + bias.double()
+    tol = (k + 64) * 2.0 ** -24 * (xv.abs() @ wv.abs().t() + bias.abs().double()) + torch.finfo(dtype).eps / 2 * want.abs()
+    assert ((y.cpu().double() - want).abs() <= tol * (1 + 1e-6)).all()
+
+
+def test_mx4_linear_shapes_strides_and_non_finite_rows(cuda):
+    w4 = bs.mx4_quantize(torch.randn(48, 70, device=cuda))
+    x = torch.randn(3, 4, 70, device=cuda)
+    y = bs.mx4_linear(x, w4)
+    assert y.shape == (3, 4, 48) and torch.equal(y.view(12, 48), bs.mx4_linear(x.view(12, 70), w4))
+    wide = torch.randn(12, 140, device=cuda)
+    assert torch.equal(bs.mx4_linear(wide[:, ::2], w4), bs.mx4_linear(wide[:, ::2].contiguous(), w4))
+    assert bs.mx4_linear(x[:0], w4).shape == (0, 4, 48)
+    assert torch.equal(bs.mx4_linear(x[1, 2], w4), y[1, 2])
+    bad = x.view(12, 70).clone()
+    bad[5, 40] = float("nan")
+    bad[7, 3] = float("inf")
+    z = bs.mx4_linear(bad, w4, relu=True)
+    assert torch.isnan(z[5]).all() and torch.isnan(z[7]).all()
+    keep = [i for i in range(12) if i not in (5, 7)]
+    assert torch.equal(z[keep], y.view(12, 48)[keep].clamp(min=0))
+    half = torch.randn(12, 71, device=cuda).to(torch.bfloat16)            # odd rows: only 2-byte alignment
+    w5 = bs.mx4_quantize(torch.randn(9, 71, device=cuda))
+    assert torch.equal(bs.mx4_linear(half, w5), bs.mx4_linear(half.clone(), w5)) and torch.equal(bs.mx4_linear(half[3:4], w5), bs.mx4_linear(half, w5)[3:4])
+
+
+# ---- streams, graphs -----------------------------------------------------------------------------------------------------------------
+def test_two_streams_at_once_do_not_share_scratch(cuda):
+    x, gy, w, y = layer(5000, 72, 18, True, 11, cuda)
+    x8, y8 = bs.checkpoint8(x, relu=True), bs.checkpoint8(y, relu=True)
+    a, w4 = torch.randn(200, 5292, device=cuda), bs.mx4_quantize(torch.randn(144, 5292, device=cuda))
+    want, lin = bs.conv1x1_backward8(gy, w, x8, y8), bs.mx4_linear(a, w4)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    outs = []
+    for rep in range(4):
+        for s in streams:
+            with torch.cuda.stream(s):
+                outs.append((bs.conv1x1_backward8(gy, w, x8, y8), bs.mx4_linear(a, w4)))
+    torch.cuda.synchronize()
+    for got, l in outs:
+        assert all(torch.equal(p, q) for p, q in zip(got[:3], want[:3])) and torch.equal(l, lin)
+
+
+def test_captured_and_replayed(cuda):
+    """the whole set in one graph, replayed on new inputs with eager calls of other sizes between the replays"""
+    V, ci, co = 600, 18, 72
+    h = torch.zeros(V, co, device=cuda)
+    bias, w = torch.randn(co, device=cuda), torch.randn(co, ci, device=cuda)
+    x, gy = torch.zeros(V, ci, device=cuda), torch.zeros(V, co, device=cuda)
+    wl = bs.mx4_quantize(torch.randn(40, co, device=cuda))
+
+    def step():
+        y, y8 = bs.bias_act_checkpoint8(h, bias)
+        x8 = bs.checkpoint8(x, relu=True)
+        gx, gw, gb, g = bs.conv1x1_backward8(gy, w, x8, y8, need_g=True)
+        return [y, y8.restore(), gx, gw, gb, g, bs.mx4_linear(y, wl), bs.mx4_quantize(gy).dequantize()]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    for rep in range(4):
+        for t in (h, gy):
+            t.copy_(torch.randn(t.shape, device=cuda))
+        x.copy_(torch.randn(x.shape, device=cuda).relu())
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [o.clone() for o in outs]
+        big = torch.randn(3000, 500, device=cuda)
+        bs.mx4_linear(big, bs.mx4_quantize(big[:700]))
+        assert all(torch.equal(a, b) for a, b in zip(got, step()))
