@@ -151,6 +151,224 @@ __global__ __launch_bounds__(THREADS) void dgrad_kernel(const float *__restrict_
     }
 }
 
+// floats of one wave's LDS tiles: 32 voxels of gradients (and a row's overhang), 32 of bf16 inputs (and theirs)
+__host__ __device__ constexpr int fused_wave_floats(int mt, int nt, int ci, int co) { return (32 * co + 32 * mt + (32 * ci + 32 * nt) / 2 + 3) / 4 * 4; }
+
+// ---- both products in one pass, for few channels --------------------------------------------------------------------------------------------
+// A wave takes 32 voxels at a time and needs no other wave: their 32 co gradients are one contiguous run, loaded 16 bytes a lane (the next run's loads
+// are issued before this one is multiplied), masked, stored as g where wanted, and put into the wave's own LDS tile as they are; their 32 ci input codes
+// are ci whole blocks.  From the tile gx takes rows (N = voxel, K = co, M = ci: a lane ends up with 4 consecutive channels of one voxel) and gw takes columns
+// (M = co, N = ci, K = voxel), both cut into bf16 pieces in registers; gw stays in registers over all of a wave's voxels.  Entries of the tiles behind co or
+// ci hold whatever follows in LDS: they only reach rows and columns that are not stored, except along gx's sum, where they are set to zero.
+template <int MT, int NT, bool A4>
+__global__ __launch_bounds__(THREADS, MT * NT <= 3 ? 2 : 1) void fused_kernel(const float *__restrict__ gy, const uint8_t *__restrict__ yc, const float *__restrict__ w,
+                                                                             const uint8_t *__restrict__ xc, const uint8_t *__restrict__ xs, float *__restrict__ gx,
+                                                                             float *__restrict__ g_out, float *__restrict__ part_w, float *__restrict__ part_b, long long V, int ci, int co,
+                                                                             int x_relu)
+{
+    extern __shared__ v4u smem[];
+    const int l = threadIdx.x & 63, wave = threadIdx.x >> 6, half = l >> 5, lo = l & 31;
+    const int KS = (co + 15) / 16;
+    v4u *wp = smem;                                                              // [NT][KS][3][64] pieces of W in fragment order
+    float *gs = reinterpret_cast<float *>(smem + NT * KS * 3 * 64) + wave * fused_wave_floats(MT, NT, ci, co);
+    uint16_t *xb = reinterpret_cast<uint16_t *>(gs + 32 * co + 32 * MT);
+    for (int t = threadIdx.x; t < NT * KS * 64; t += THREADS) {
+        const int ll = t & 63, n = (t / 64 / KS) * 32 + (ll & 31), k = (t / 64 % KS) * 16 + 8 * (ll >> 5);
+        float b[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) b[j] = n < ci && k + j < co ? w[(k + j) * ci + n] : 0.0f;
+        const Split8 B = split8(b);
+        v4u *to = wp + (t / 64) * 3 * 64 + ll;
+        to[0] = __builtin_bit_cast(v4u, B.hi);
+        to[64] = __builtin_bit_cast(v4u, B.mid);
+        to[128] = __builtin_bit_cast(v4u, B.lo);
+    }
+    __syncthreads();
+
+    const long long chunks = (V + 31) / 32, step = (long long)gridDim.x * WAVES;
+    long long chunk = (long long)blockIdx.x * WAVES + wave;
+    float G[4 * MT][4];
+    unsigned Y[4 * MT], X[4 * NT];
+    int S[4 * NT];
+    // lanes behind the run's end repeat its last 16 bytes (they store them to the same place again)
+    auto load = [&](long long c) {
+        const float *pg = gy + c * 32 * co;
+        const uint8_t *py = yc + c * 32 * co, *px = xc + c * 32 * ci, *ps = xs + c * ci;
+#pragma unroll
+        for (int q = 0; q < 4 * MT; ++q)
+            if (q * 8 < co) {
+                const int i = min(q * 64 + l, 8 * co - 1);
+                *reinterpret_cast<Io<float>::vec *>(G[q]) = *reinterpret_cast<const Io<float>::vec *>(pg + 4 * i);
+                Y[q] = yc != nullptr ? *reinterpret_cast<const unsigned *>(py + 4 * i) : 0x01010101u;
+            }
+#pragma unroll
+        for (int q = 0; q < 4 * NT; ++q)
+            if (q * 8 < ci) {
+                const int i = min(q * 64 + l, 8 * ci - 1);
+                X[q] = *reinterpret_cast<const unsigned *>(px + 4 * i);
+                S[q] = ps[i >> 3];
+            }
+    };
+    // the last chunk where it is short: value by value, straight into the tiles
+    auto fill_short = [&](long long c) {
+        for (int e = l; e < 32 * co; e += 64) {
+            const long long at = c * 32 * co + e;
+            float t = 0.0f;
+            if (at < V * co) {
+                t = yc == nullptr || yc[at] ? gy[at] : 0.0f;
+                if (g_out != nullptr) g_out[at] = t;
+            }
+            gs[e] = t;
+        }
+        for (int e = l; e < 32 * ci; e += 64) {
+            const long long at = c * 32 * ci + e;
+            xb[e] = at < V * ci ? (uint16_t)(__float_as_uint(code_value(xc[at], x_relu, xs[at >> 5])) >> 16) : (uint16_t)0;
+        }
+    };
+    v16f acc[MT][NT];
+    float bsum[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        bsum[m] = 0.0f;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) acc[m][n] = v16f{};
+    }
+    const long long full = V / 32;
+    if (chunk < full) load(chunk);
+    for (; chunk < chunks; chunk += step) {
+        if (chunk < full) {
+            float *pg = g_out + chunk * 32 * co;
+#pragma unroll
+            for (int q = 0; q < 4 * MT; ++q)
+                if (q * 8 < co) {
+                    const int i = min(q * 64 + l, 8 * co - 1);
+                    v4f t;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) t[j] = (Y[q] >> (8 * j) & 255u) ? G[q][j] : 0.0f;
+                    *reinterpret_cast<v4f *>(gs + 4 * i) = t;
+                    if (g_out != nullptr) *reinterpret_cast<Io<float>::vec *>(pg + 4 * i) = t;
+                }
+#pragma unroll
+            for (int q = 0; q < 4 * NT; ++q)
+                if (q * 8 < ci) {
+                    const int i = min(q * 64 + l, 8 * ci - 1);
+                    float t[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) t[j] = code_value(X[q] >> (8 * j) & 255u, x_relu, S[q]);
+                    uint2 p;
+                    p.x = pack_hi(t[0], t[1]);
+                    p.y = pack_hi(t[2], t[3]);
+                    *reinterpret_cast<uint2 *>(xb + 4 * i) = p;
+                }
+        } else {
+            fill_short(chunk);
+        }
+        if (chunk + step < full) load(chunk + step);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        // gx
+        v16f d[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) d[n] = v16f{};
+        for (int ks = 0; ks < KS; ++ks) {
+            const int k = ks * 16 + 8 * half;
+            const float *row = gs + lo * co + k;
+            float b[8];
+            if (A4) {
+                *reinterpret_cast<v4f *>(b) = *reinterpret_cast<const v4f *>(row);
+                *reinterpret_cast<v4f *>(b + 4) = *reinterpret_cast<const v4f *>(row + 4);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) b[j] = row[j];
+            }
+            if (ks * 16 + 16 > co) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) b[j] = k + j < co ? b[j] : 0.0f;
+            }
+            const Split8 B = split8(b);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const v4u *p = wp + (n * KS + ks) * 3 * 64 + l;
+                const v8bf hi = __builtin_bit_cast(v8bf, p[0]), mid = __builtin_bit_cast(v8bf, p[64]), low = __builtin_bit_cast(v8bf, p[128]);
+                d[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(low, B.hi, d[n], 0, 0, 0);
+                d[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(hi, B.lo, d[n], 0, 0, 0);
+                d[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(mid, B.mid, d[n], 0, 0, 0);
+                d[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(mid, B.hi, d[n], 0, 0, 0);
+                d[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(hi, B.mid, d[n], 0, 0, 0);
+                d[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(hi, B.hi, d[n], 0, 0, 0);
+            }
+        }
+        if (chunk * 32 + lo < V) {
+            float *row = gx + (chunk * 32 + lo) * ci;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int c = n * 32 + 8 * q + 4 * half;
+                    Io<float>::vec t;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) t[j] = d[n][4 * q + j];
+                    if (c + 4 <= ci) *reinterpret_cast<Io<float>::vec *>(row + c) = t;
+                    else
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) if (c + j < ci) row[c + j] = t[j];
+                }
+            }
+        }
+        // gw and gbias
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            const int v = ks * 16 + 8 * half;
+            v8bf B[NT];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                v4u p;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) p[q] = (unsigned)xb[(v + 2 * q) * ci + n * 32 + lo] | (unsigned)xb[(v + 2 * q + 1) * ci + n * 32 + lo] << 16;
+                B[n] = __builtin_bit_cast(v8bf, p);
+            }
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                float a[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) a[j] = gs[(v + j) * co + m * 32 + lo];
+                bsum[m] = bsum[m] + (((a[0] + a[1]) + (a[2] + a[3])) + ((a[4] + a[5]) + (a[6] + a[7])));
+                const Split8 A = split8(a);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A.lo, B[n], acc[m][n], 0, 0, 0);
+                    acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A.mid, B[n], acc[m][n], 0, 0, 0);
+                    acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A.hi, B[n], acc[m][n], 0, 0, 0);
+                }
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+    // the four waves' sums, in wave order
+    float *sum = reinterpret_cast<float *>(smem), *sumb = sum + 32 * 32 * MT * NT;
+#pragma unroll 1
+    for (int turn = 0; turn < WAVES; ++turn) {
+        __syncthreads();
+        if (wave != turn) continue;
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            const float b2 = bsum[m] + __shfl_xor(bsum[m], 32);
+            if (half == 0) sumb[m * 32 + lo] = turn == 0 ? b2 : sumb[m * 32 + lo] + b2;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    float *to = sum + ((m * 32 + 8 * (i / 4) + 4 * half + i % 4) * NT + n) * 32 + lo;
+                    *to = turn == 0 ? acc[m][n][i] : *to + acc[m][n][i];
+                }
+        }
+    }
+    __syncthreads();
+    for (int t = threadIdx.x; t < co * ci; t += THREADS) part_w[(long long)blockIdx.x * co * ci + t] = sum[(t / ci) * 32 * NT + t % ci];
+    for (int t = threadIdx.x; t < co; t += THREADS) part_b[(long long)blockIdx.x * co + t] = sumb[t];
+}
+
 // voxels a workgroup of wgrad_kernel sums: enough workgroups for the card, not so many that the partial sums outweigh the inputs
 inline long long wgrad_split(long long V, int ci, int co)
 {
@@ -162,6 +380,60 @@ inline long long wgrad_split(long long V, int ci, int co)
     return (per + 15) / 16 * 16;
 }
 
+struct FusedPlan { int mt, nt, lds, blocks; };
+
+// the one-pass kernel's plan, mt = 0 where it does not apply
+inline FusedPlan fused_plan(long long V, int ci, int co)
+{
+    FusedPlan p = {(co + 31) / 32, (ci + 31) / 32, 0, 0};
+    const int tiles = co <= 160 && ci <= 160 ? p.mt * p.nt : 99;
+    if (tiles > 10) return {0, 0, 0, 0};
+    const int ks = (co + 15) / 16;
+    p.lds = p.nt * ks * 3 * 1024 + WAVES * fused_wave_floats(p.mt, p.nt, ci, co) * 4;
+    const int sums = (1024 * tiles + 32 * p.mt) * 4;
+    if (p.lds < sums) p.lds = sums;
+    if (p.lds > 160 * 1024) return {0, 0, 0, 0};
+    const int per_cu = tiles <= 3 ? 2 : 1, fit = 160 * 1024 / p.lds, at_once = 256 * (fit < per_cu ? fit : per_cu);
+    const long long want = (V + 32 * WAVES - 1) / (32 * WAVES);
+    p.blocks = (int)(want < at_once ? want : at_once);
+    return p;
+}
+
+struct FusedArgs { const float *gy; const uint8_t *yc; const float *w; const uint8_t *xc, *xs; float *gx, *g, *part_w, *part_b; long long V; int ci, co, x_relu; };
+
+template <int MT, int NT>
+int fused_launch(const FusedPlan &p, const FusedArgs &a, hipStream_t s)
+{
+    const auto kernel = a.co % 4 == 0 ? fused_kernel<MT, NT, true> : fused_kernel<MT, NT, false>;
+    if (hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, p.lds) != hipSuccess) return MDT_ERR_LAUNCH_FAILED;
+    kernel<<<p.blocks, THREADS, p.lds, s>>>(a.gy, a.yc, a.w, a.xc, a.xs, a.gx, a.g, a.part_w, a.part_b, a.V, a.ci, a.co, a.x_relu);
+    return MDT_OK;
+}
+
+int fused_run(const FusedPlan &p, const FusedArgs &a, hipStream_t s)
+{
+    switch (p.mt * 10 + p.nt) {
+        case 11: return fused_launch<1, 1>(p, a, s);
+        case 12: return fused_launch<1, 2>(p, a, s);
+        case 13: return fused_launch<1, 3>(p, a, s);
+        case 14: return fused_launch<1, 4>(p, a, s);
+        case 15: return fused_launch<1, 5>(p, a, s);
+        case 21: return fused_launch<2, 1>(p, a, s);
+        case 22: return fused_launch<2, 2>(p, a, s);
+        case 23: return fused_launch<2, 3>(p, a, s);
+        case 24: return fused_launch<2, 4>(p, a, s);
+        case 25: return fused_launch<2, 5>(p, a, s);
+        case 31: return fused_launch<3, 1>(p, a, s);
+        case 32: return fused_launch<3, 2>(p, a, s);
+        case 33: return fused_launch<3, 3>(p, a, s);
+        case 41: return fused_launch<4, 1>(p, a, s);
+        case 42: return fused_launch<4, 2>(p, a, s);
+        case 51: return fused_launch<5, 1>(p, a, s);
+        case 52: return fused_launch<5, 2>(p, a, s);
+    }
+    return MDT_ERR_UNSUPPORTED;
+}
+
 }  // namespace
 
 extern "C" {
@@ -169,7 +441,10 @@ extern "C" {
 size_t mdt_conv1x1_act8_backward_workspace_bytes(long long n_voxels, int c_in, int c_out)
 {
     if (n_voxels < 1 || c_in < 1 || c_out < 1 || c_in > 65536 || c_out > 65536) return 256;
-    const long long per = wgrad_split(n_voxels, c_in, c_out), splits = (n_voxels + per - 1) / per;
+    const long long per = wgrad_split(n_voxels, c_in, c_out);
+    long long splits = (n_voxels + per - 1) / per;
+    const FusedPlan p = fused_plan(n_voxels, c_in, c_out);
+    if (p.blocks > splits) splits = p.blocks;
     return (size_t)(splits * ((long long)c_in * c_out + c_out)) * 4 + 256;
 }
 
@@ -183,6 +458,15 @@ int mdt_conv1x1_act8_backward(const float *gy, const float *w, const void *x_cod
     const long long per = n_voxels > 0 ? wgrad_split(n_voxels, c_in, c_out) : 16, splits = (n_voxels + per - 1) / per;
     if (sums && n_voxels > 0 && (workspace == nullptr || workspace_bytes < mdt_conv1x1_act8_backward_workspace_bytes(n_voxels, c_in, c_out))) return MDT_ERR_WORKSPACE_TOO_SMALL;
     const long long nw = (long long)c_in * c_out;
+    const FusedPlan p = n_voxels > 0 && gx && gw ? fused_plan(n_voxels, c_in, c_out) : FusedPlan{0, 0, 0, 0};
+    if (p.mt > 0) {
+        float *part_w = (float *)workspace, *part_b = part_w + p.blocks * nw;
+        const FusedArgs a = {gy, (const uint8_t *)y_codes, w, (const uint8_t *)x_codes, (const uint8_t *)x_scales, gx, g, part_w, part_b, n_voxels, c_in, c_out, x_relu};
+        const int rc = fused_run(p, a, s);
+        if (rc != MDT_OK) return rc;
+        reduce_kernel<<<dim3((unsigned)((nw + c_out + 31) / 32)), 256, 0, s>>>(part_w, part_b, gw, gbias, nw, c_out, p.blocks);
+        return launch_check();
+    }
     float *part_w = (float *)workspace, *part_b = part_w + splits * nw;
     if (n_voxels > 0 && (gx || g)) {
         const dim3 grid((unsigned)((n_voxels + 32 * WAVES - 1) / (32 * WAVES)), gx ? (unsigned)((c_in + 31) / 32) : 1u);
