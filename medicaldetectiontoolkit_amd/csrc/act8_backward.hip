@@ -151,27 +151,31 @@ __global__ __launch_bounds__(THREADS) void dgrad_kernel(const float *__restrict_
     }
 }
 
-// floats of one wave's LDS tiles: 32 voxels of gradients (and a row's overhang), 32 of bf16 inputs (and theirs)
-__host__ __device__ constexpr int fused_wave_floats(int mt, int nt, int ci, int co) { return (32 * co + 32 * mt + (32 * ci + 32 * nt) / 2 + 3) / 4 * 4; }
+// floats of one wave's LDS tiles: 32 voxels of gradients (and a row's overhang; gx's rows take the same place later), 32 of bf16 inputs (and theirs)
+__host__ __device__ constexpr int fused_rows_floats(int mt, int ci, int co) { return 32 * (co > ci ? co : ci) + 32 * mt; }
+__host__ __device__ constexpr int fused_wave_floats(int mt, int nt, int ci, int co) { return (fused_rows_floats(mt, ci, co) + (32 * ci + 32 * nt) / 2 + 3) / 4 * 4; }
 
 // ---- both products in one pass, for few channels --------------------------------------------------------------------------------------------
-// A wave takes 32 voxels at a time and needs no other wave: their 32 co gradients are one contiguous run, loaded 16 bytes a lane (the next run's loads
-// are issued before this one is multiplied), masked, stored as g where wanted, and put into the wave's own LDS tile as they are; their 32 ci input codes
-// are ci whole blocks.  From the tile gx takes rows (N = voxel, K = co, M = ci: a lane ends up with 4 consecutive channels of one voxel) and gw takes columns
-// (M = co, N = ci, K = voxel), both cut into bf16 pieces in registers; gw stays in registers over all of a wave's voxels.  Entries of the tiles behind co or
-// ci hold whatever follows in LDS: they only reach rows and columns that are not stored, except along gx's sum, where they are set to zero.
-template <int MT, int NT, bool A4>
+// A wave takes 32 voxels at a time and needs no other wave: their 32 co gradients are one contiguous run, loaded 16 bytes a lane, masked, and put into the
+// wave's own LDS tile as they are; their 32 ci input codes are ci whole blocks.  From the tile gw takes columns (M = co, N = ci, K = voxel) and gx takes rows
+// (M = ci, N = voxel, K = co), both cut into bf16 pieces in registers; gw stays in registers over all of a wave's voxels.  gx's tile replaces the gradients in LDS
+// and leaves as the contiguous run that it is, like g.
+// Loads and stores share one in-order counter: the next chunk's loads are issued before this chunk's stores and every chunk issues the same number of
+// stores, so that the wait for the loads does not wait for the stores behind them.
+// Entries of the tiles behind co or ci hold whatever follows in LDS: they only reach rows and columns that are not stored, except along gx's sum, where
+// they are set to zero.
+template <int MT, int NT, bool G_OUT>
 __global__ __launch_bounds__(THREADS, MT * NT <= 3 ? 2 : 1) void fused_kernel(const float *__restrict__ gy, const uint8_t *__restrict__ yc, const float *__restrict__ w,
                                                                              const uint8_t *__restrict__ xc, const uint8_t *__restrict__ xs, float *__restrict__ gx,
                                                                              float *__restrict__ g_out, float *__restrict__ part_w, float *__restrict__ part_b, long long V, int ci, int co,
                                                                              int x_relu)
 {
     extern __shared__ v4u smem[];
-    const int l = threadIdx.x & 63, wave = threadIdx.x >> 6, half = l >> 5, lo = l & 31;
+    const int l = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = l >> 5, lo = l & 31;
     const int KS = (co + 15) / 16;
     v4u *wp = smem;                                                              // [NT][KS][3][64] pieces of W in fragment order
     float *gs = reinterpret_cast<float *>(smem + NT * KS * 3 * 64) + wave * fused_wave_floats(MT, NT, ci, co);
-    uint16_t *xb = reinterpret_cast<uint16_t *>(gs + 32 * co + 32 * MT);
+    uint16_t *xb = reinterpret_cast<uint16_t *>(gs + fused_rows_floats(MT, ci, co));
     for (int t = threadIdx.x; t < NT * KS * 64; t += THREADS) {
         const int ll = t & 63, n = (t / 64 / KS) * 32 + (ll & 31), k = (t / 64 % KS) * 16 + 8 * (ll >> 5);
         float b[8];
@@ -185,29 +189,36 @@ __global__ __launch_bounds__(THREADS, MT * NT <= 3 ? 2 : 1) void fused_kernel(co
     }
     __syncthreads();
 
-    const long long chunks = (V + 31) / 32, step = (long long)gridDim.x * WAVES;
+    const long long chunks = (V + 31) / 32, full = V / 32, step = (long long)gridDim.x * WAVES;
     long long chunk = (long long)blockIdx.x * WAVES + wave;
-    float G[4 * MT][4];
+    v4f G[4 * MT];
     unsigned Y[4 * MT], X[4 * NT];
     int S[4 * NT];
-    // lanes behind the run's end repeat its last 16 bytes (they store them to the same place again)
+    // lanes behind the run's end repeat its last 16 bytes (and store them to the same place again)
+    auto at_gy = [&](unsigned lane, int q) { return min(q * 64 + lane, 8u * co - 1); };
+    auto at_x = [&](unsigned lane, int q) { return min(q * 64 + lane, 8u * ci - 1); };
+    // the lane's number, kept from the optimiser: it would hold every address that it computes from it in a register of its own over the loop
+    auto lane = [&] {
+        unsigned v = l;
+        asm volatile("" : "+v"(v));
+        return v;
+    };
     auto load = [&](long long c) {
+        const unsigned ln = lane();
+        if (yc != nullptr) {
+            const uint8_t *py = yc + c * 32 * co;
+#pragma unroll
+            for (int q = 0; q < 4 * MT; ++q) Y[q] = *reinterpret_cast<const unsigned *>(py + 4 * at_gy(ln, q));
+        }
+        const uint8_t *px = xc + c * 32 * ci, *ps = xs + c * ci;
+#pragma unroll
+        for (int q = 0; q < 4 * NT; ++q) {
+            X[q] = *reinterpret_cast<const unsigned *>(px + 4 * at_x(ln, q));
+            S[q] = ps[at_x(ln, q) >> 3];
+        }
         const float *pg = gy + c * 32 * co;
-        const uint8_t *py = yc + c * 32 * co, *px = xc + c * 32 * ci, *ps = xs + c * ci;
 #pragma unroll
-        for (int q = 0; q < 4 * MT; ++q)
-            if (q * 8 < co) {
-                const int i = min(q * 64 + l, 8 * co - 1);
-                *reinterpret_cast<Io<float>::vec *>(G[q]) = *reinterpret_cast<const Io<float>::vec *>(pg + 4 * i);
-                Y[q] = yc != nullptr ? *reinterpret_cast<const unsigned *>(py + 4 * i) : 0x01010101u;
-            }
-#pragma unroll
-        for (int q = 0; q < 4 * NT; ++q)
-            if (q * 8 < ci) {
-                const int i = min(q * 64 + l, 8 * ci - 1);
-                X[q] = *reinterpret_cast<const unsigned *>(px + 4 * i);
-                S[q] = ps[i >> 3];
-            }
+        for (int q = 0; q < 4 * MT; ++q) G[q] = *reinterpret_cast<const Io<float>::vec *>(pg + 4 * at_gy(ln, q));
     };
     // the last chunk where it is short: value by value, straight into the tiles
     auto fill_short = [&](long long c) {
@@ -216,7 +227,7 @@ __global__ __launch_bounds__(THREADS, MT * NT <= 3 ? 2 : 1) void fused_kernel(co
             float t = 0.0f;
             if (at < V * co) {
                 t = yc == nullptr || yc[at] ? gy[at] : 0.0f;
-                if (g_out != nullptr) g_out[at] = t;
+                if (G_OUT) g_out[at] = t;
             }
             gs[e] = t;
         }
@@ -224,6 +235,10 @@ __global__ __launch_bounds__(THREADS, MT * NT <= 3 ? 2 : 1) void fused_kernel(co
             const long long at = c * 32 * ci + e;
             xb[e] = at < V * ci ? (uint16_t)(__float_as_uint(code_value(xc[at], x_relu, xs[at >> 5])) >> 16) : (uint16_t)0;
         }
+    };
+    auto fence = [] {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
     };
     v16f acc[MT][NT];
     float bsum[MT];
@@ -233,39 +248,61 @@ __global__ __launch_bounds__(THREADS, MT * NT <= 3 ? 2 : 1) void fused_kernel(co
 #pragma unroll
         for (int n = 0; n < NT; ++n) acc[m][n] = v16f{};
     }
-    const long long full = V / 32;
     if (chunk < full) load(chunk);
     for (; chunk < chunks; chunk += step) {
-        if (chunk < full) {
-            float *pg = g_out + chunk * 32 * co;
+        const bool whole = chunk < full;
+        if (whole) {
+            const unsigned ln = lane();
 #pragma unroll
-            for (int q = 0; q < 4 * MT; ++q)
-                if (q * 8 < co) {
-                    const int i = min(q * 64 + l, 8 * co - 1);
-                    v4f t;
+            for (int q = 0; q < 4 * MT; ++q) {
+                if (yc != nullptr) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) t[j] = (Y[q] >> (8 * j) & 255u) ? G[q][j] : 0.0f;
-                    *reinterpret_cast<v4f *>(gs + 4 * i) = t;
-                    if (g_out != nullptr) *reinterpret_cast<Io<float>::vec *>(pg + 4 * i) = t;
+                    for (int j = 0; j < 4; ++j) G[q][j] = (Y[q] >> (8 * j) & 255u) ? G[q][j] : 0.0f;
                 }
+                *reinterpret_cast<v4f *>(gs + 4 * at_gy(ln, q)) = G[q];
+            }
 #pragma unroll
-            for (int q = 0; q < 4 * NT; ++q)
-                if (q * 8 < ci) {
-                    const int i = min(q * 64 + l, 8 * ci - 1);
-                    float t[4];
+            for (int q = 0; q < 4 * NT; ++q) {
+                float t[4];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) t[j] = code_value(X[q] >> (8 * j) & 255u, x_relu, S[q]);
-                    uint2 p;
-                    p.x = pack_hi(t[0], t[1]);
-                    p.y = pack_hi(t[2], t[3]);
-                    *reinterpret_cast<uint2 *>(xb + 4 * i) = p;
-                }
+                for (int j = 0; j < 4; ++j) t[j] = code_value(X[q] >> (8 * j) & 255u, x_relu, S[q]);
+                uint2 p;
+                p.x = pack_hi(t[0], t[1]);
+                p.y = pack_hi(t[2], t[3]);
+                *reinterpret_cast<uint2 *>(xb + 4 * at_x(ln, q)) = p;
+            }
         } else {
             fill_short(chunk);
         }
         if (chunk + step < full) load(chunk + step);
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
+        fence();
+        // gw and gbias
+        const unsigned lg = lane(), og = 8 * (lg >> 5) * co + (lg & 31), ox = 8 * (lg >> 5) * ci + (lg & 31);
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            v8bf B[NT];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                v4u p;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) p[q] = (unsigned)xb[ox + (ks * 16 + 2 * q) * ci + n * 32] | (unsigned)xb[ox + (ks * 16 + 2 * q + 1) * ci + n * 32] << 16;
+                B[n] = __builtin_bit_cast(v8bf, p);
+            }
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                float a[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) a[j] = gs[og + (ks * 16 + j) * co + m * 32];
+                bsum[m] = bsum[m] + (((a[0] + a[1]) + (a[2] + a[3])) + ((a[4] + a[5]) + (a[6] + a[7])));
+                const Split8 A = split8(a);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A.lo, B[n], acc[m][n], 0, 0, 0);
+                    acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A.mid, B[n], acc[m][n], 0, 0, 0);
+                    acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A.hi, B[n], acc[m][n], 0, 0, 0);
+                }
+            }
+        }
         // gx
         v16f d[NT];
 #pragma unroll
@@ -274,7 +311,7 @@ __global__ __launch_bounds__(THREADS, MT * NT <= 3 ? 2 : 1) void fused_kernel(co
             const int k = ks * 16 + 8 * half;
             const float *row = gs + lo * co + k;
             float b[8];
-            if (A4) {
+            if (co % 4 == 0) {
                 *reinterpret_cast<v4f *>(b) = *reinterpret_cast<const v4f *>(row);
                 *reinterpret_cast<v4f *>(b + 4) = *reinterpret_cast<const v4f *>(row + 4);
             } else {
@@ -298,52 +335,36 @@ __global__ __launch_bounds__(THREADS, MT * NT <= 3 ? 2 : 1) void fused_kernel(co
                 d[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(hi, B.hi, d[n], 0, 0, 0);
             }
         }
-        if (chunk * 32 + lo < V) {
-            float *row = gx + (chunk * 32 + lo) * ci;
+        if (G_OUT && whole) {
+            float *pg = g_out + chunk * 32 * co;
+            const unsigned ln = lane();
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
+            for (int q = 0; q < 4 * MT; ++q) *reinterpret_cast<Io<float>::vec *>(pg + 4 * at_gy(ln, q)) = *reinterpret_cast<const v4f *>(gs + 4 * at_gy(ln, q));
+        }
+        fence();
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int c = n * 32 + 8 * q + 4 * half;
-                    Io<float>::vec t;
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) t[j] = d[n][4 * q + j];
-                    if (c + 4 <= ci) *reinterpret_cast<Io<float>::vec *>(row + c) = t;
-                    else
+            for (int q = 0; q < 4; ++q) {
+                const int c = n * 32 + 8 * q + 4 * half;
+                float *to = gs + lo * ci + c;
+                if (ci % 4 == 0) {
+                    if (c < ci) *reinterpret_cast<v4f *>(to) = v4f{d[n][4 * q], d[n][4 * q + 1], d[n][4 * q + 2], d[n][4 * q + 3]};
+                } else {
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) if (c + j < ci) row[c + j] = t[j];
+                    for (int j = 0; j < 4; ++j) if (c + j < ci) to[j] = d[n][4 * q + j];
                 }
             }
+        fence();
+        float *px = gx + chunk * 32 * ci;
+        if (whole) {
+            const unsigned ln = lane();
+#pragma unroll
+            for (int q = 0; q < 4 * NT; ++q) *reinterpret_cast<Io<float>::vec *>(px + 4 * at_x(ln, q)) = *reinterpret_cast<const v4f *>(gs + 4 * at_x(ln, q));
+        } else {
+            for (int e = l; e < (V - chunk * 32) * ci; e += 64) px[e] = gs[e];
         }
-        // gw and gbias
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-            const int v = ks * 16 + 8 * half;
-            v8bf B[NT];
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                v4u p;
-#pragma unroll
-                for (int q = 0; q < 4; ++q) p[q] = (unsigned)xb[(v + 2 * q) * ci + n * 32 + lo] | (unsigned)xb[(v + 2 * q + 1) * ci + n * 32 + lo] << 16;
-                B[n] = __builtin_bit_cast(v8bf, p);
-            }
-#pragma unroll
-            for (int m = 0; m < MT; ++m) {
-                float a[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) a[j] = gs[(v + j) * co + m * 32 + lo];
-                bsum[m] = bsum[m] + (((a[0] + a[1]) + (a[2] + a[3])) + ((a[4] + a[5]) + (a[6] + a[7])));
-                const Split8 A = split8(a);
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A.lo, B[n], acc[m][n], 0, 0, 0);
-                    acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A.mid, B[n], acc[m][n], 0, 0, 0);
-                    acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A.hi, B[n], acc[m][n], 0, 0, 0);
-                }
-            }
-        }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
+        fence();
     }
     // the four waves' sums, in wave order
     float *sum = reinterpret_cast<float *>(smem), *sumb = sum + 32 * 32 * MT * NT;
@@ -404,7 +425,7 @@ struct FusedArgs { const float *gy; const uint8_t *yc; const float *w; const uin
 template <int MT, int NT>
 int fused_launch(const FusedPlan &p, const FusedArgs &a, hipStream_t s)
 {
-    const auto kernel = a.co % 4 == 0 ? fused_kernel<MT, NT, true> : fused_kernel<MT, NT, false>;
+    const auto kernel = a.g != nullptr ? fused_kernel<MT, NT, true> : fused_kernel<MT, NT, false>;
     if (hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, p.lds) != hipSuccess) return MDT_ERR_LAUNCH_FAILED;
     kernel<<<p.blocks, THREADS, p.lds, s>>>(a.gy, a.yc, a.w, a.xc, a.xs, a.gx, a.g, a.part_w, a.part_b, a.V, a.ci, a.co, a.x_relu);
     return MDT_OK;
