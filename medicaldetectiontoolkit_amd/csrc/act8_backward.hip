@@ -45,110 +45,313 @@ __device__ __forceinline__ Split8 split8(const float (&v)[8])
 
 __device__ __forceinline__ float code_value(unsigned c, bool is_relu, int b) { return (is_relu ? (float)c : (float)(int8_t)c) * scale_of(b); }
 
-// ---- gw and gbias: partial sums over ranges of voxels --------------------------------------------------------------------------------
-// matrix tile 32 x 32 (M = co, N = ci, K = 16 voxels): lane l holds row / column l % 32 and voxels 8 (l / 32) ...
-__global__ __launch_bounds__(THREADS) void wgrad_kernel(const float *__restrict__ gy, const uint8_t *__restrict__ yc, const uint8_t *__restrict__ xc, const uint8_t *__restrict__ xs,
-                                                        float *__restrict__ part_w, float *__restrict__ part_b, long long V, int ci, int co, int x_relu, long long per_split)
+// ---- any number of channels: one product a kernel, tiles through LDS ------------------------------------------------------------------------
+// Both kernels cut what they load into bf16 pieces once, put the pieces into LDS with the summed axis innermost (32 entries and 8 of padding a row: the
+// 16-byte reads and writes of neighbouring rows fall into different banks) and hold the next step's loads in registers meanwhile.  4 waves, WM x WN of
+// them with TM x TN matrix tiles of 32 x 32 each.
+constexpr int KSTEP = 32, KROW = KSTEP + 8;
+
+__device__ __forceinline__ v8bf row_of(const uint16_t *p) { return __builtin_bit_cast(v8bf, *reinterpret_cast<const v4u *>(p)); }
+
+// up to 4 consecutive values from p on, zeros behind `left`
+__device__ __forceinline__ v4f load4(const float *p, int left)
 {
-    __shared__ float s_acc[WAVES][32 * 32];
-    __shared__ float s_b[WAVES][64];
-    const int l = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int m = blockIdx.y * 32 + (l & 31), n = blockIdx.z * 32 + (l & 31);
-    const long long v0 = (long long)blockIdx.x * per_split, v1 = v0 + per_split < V ? v0 + per_split : V;
-    v16f acc = {};
-    float bsum = 0.0f;
-    for (long long v = v0 + wave * 16; v < v1; v += WAVES * 16) {
-        float g[8], x[8];
+    if (left >= 4) return *reinterpret_cast<const Io<float>::vec *>(p);
+    v4f v = {};
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const long long r = v + 8 * (l >> 5) + j;
-            const bool in = r < v1;
-            g[j] = in && m < co ? gy[r * co + m] : 0.0f;
-            if (yc != nullptr && in && m < co) g[j] = yc[r * co + m] ? g[j] : 0.0f;
-            const long long at = r * ci + n;
-            x[j] = in && n < ci ? code_value(xc[at], x_relu, xs[at >> 5]) : 0.0f;
-            bsum = bsum + g[j];
-        }
-        const Split8 a = split8(g);
-        v4u xb;
+    for (int j = 0; j < 3; ++j) if (j < left) v[j] = p[j];
+    return v;
+}
+__device__ __forceinline__ unsigned load4(const uint8_t *p, int left)
+{
+    typedef unsigned una __attribute__((aligned(1)));
+    if (left >= 4) return *reinterpret_cast<const una *>(p);
+    unsigned v = 0;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) xb[q] = pack_hi(x[2 * q], x[2 * q + 1]);
-        const v8bf b = __builtin_bit_cast(v8bf, xb);
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.lo, b, acc, 0, 0, 0);
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.mid, b, acc, 0, 0, 0);
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.hi, b, acc, 0, 0, 0);
-    }
+    for (int j = 0; j < 3; ++j) if (j < left) v |= (unsigned)p[j] << (8 * j);
+    return v;
+}
+__device__ __forceinline__ v4f masked(v4f g, unsigned m)
+{
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s_acc[wave][(8 * (i / 4) + 4 * (l >> 5) + i % 4) * 32 + (l & 31)] = acc[i];
-    s_b[wave][l] = bsum;
-    __syncthreads();
-    for (int t = threadIdx.x; t < 32 * 32; t += THREADS) {
-        const int o = blockIdx.y * 32 + t / 32, i = blockIdx.z * 32 + t % 32;
-        if (o < co && i < ci) part_w[((long long)blockIdx.x * co + o) * ci + i] = (s_acc[0][t] + s_acc[1][t]) + (s_acc[2][t] + s_acc[3][t]);
-    }
-    if (blockIdx.z == 0 && threadIdx.x < 32 && blockIdx.y * 32 + threadIdx.x < co) {
-        float s = 0.0f;
-        for (int w = 0; w < WAVES; ++w) s = s + (s_b[w][threadIdx.x] + s_b[w][threadIdx.x + 32]);
-        part_b[(long long)blockIdx.x * co + blockIdx.y * 32 + threadIdx.x] = s;
+    for (int j = 0; j < 4; ++j) g[j] = (m >> (8 * j) & 255u) ? g[j] : 0.0f;
+    return g;
+}
+// 4 floats -> 4 entries of each of the three pieces' planes
+__device__ __forceinline__ void put4(uint16_t *to, int plane, v4f v)
+{
+    float a = v[0], b = v[1], c = v[2], d = v[3];
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+        uint2 p;
+        p.x = round2(a, b);
+        p.y = round2(c, d);
+        *reinterpret_cast<uint2 *>(to + k * plane) = p;
     }
 }
 
-// out[e] = sum over the splits of part[split][e], 32 elements a workgroup and 8 ranges of splits, in a fixed order; elements [0, nw) are gw's, the rest gbias's
-__global__ __launch_bounds__(256) void reduce_kernel(const float *__restrict__ part_w, const float *__restrict__ part_b, float *__restrict__ gw, float *__restrict__ gb, long long nw,
-                                                     int nb, int splits)
+// gx (and g).  M = ci, N = voxel, K = co: a lane ends up with 4 consecutive channels of one voxel.
+template <int WM, int TM, int WN, int TN>
+__global__ __launch_bounds__(THREADS, 2) void dgrad_kernel(const float *__restrict__ gy, const uint8_t *__restrict__ yc, const float *__restrict__ w, float *__restrict__ gx,
+                                                           float *__restrict__ g_out, long long V, int ci, int co, int ci_tiles)
 {
-    __shared__ float s[8][32];
-    const int lane = threadIdx.x & 31, range = threadIdx.x >> 5;
-    const long long e = (long long)blockIdx.x * 32 + lane;
+    constexpr int BM = WM * TM * 32, BN = WN * TN * 32, GP = BN / 32, WG = BM / 64;
+    __shared__ uint16_t s_w[3 * BM * KROW], s_g[3 * BN * KROW];
+    const int t = threadIdx.x, l = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), half = l >> 5, lo = l & 31;
+    // the ci tiles of one range of voxels follow each other on one XCD (workgroups go to the 8 XCDs in turn), whose L2 then holds the range's gradients
+    const int xcd = blockIdx.x % 8, turn = blockIdx.x / 8, ct = turn % ci_tiles;
+    const long long v0 = ((long long)(turn / ci_tiles) * 8 + xcd) * BN;
+    if (v0 >= V) return;
+    const int c0 = ct * BM, gr = t >> 3, gk = (t & 7) * 4, wn = t % BM, wk = t / BM * 8;
+    v4f G[GP];
+    unsigned Y[GP];
+    float W[WG][8];
+    auto load = [&](int k0) {
+#pragma unroll
+        for (int i = 0; i < GP; ++i) {
+            const long long v = v0 + i * 32 + gr, at = (v < V ? v : V - 1) * co + k0 + gk;
+            const int left = co - k0 - gk;
+            G[i] = load4(gy + at, left);
+            Y[i] = yc != nullptr ? load4(yc + at, left) : 0x01010101u;
+        }
+#pragma unroll
+        for (int i = 0; i < WG; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int k = k0 + wk + i * (THREADS / BM) * 8 + j, n = c0 + wn;
+                W[i][j] = k < co && n < ci ? w[(long long)k * ci + n] : 0.0f;
+            }
+    };
+    v16f acc[TM][TN];
+#pragma unroll
+    for (int m = 0; m < TM; ++m)
+#pragma unroll
+        for (int n = 0; n < TN; ++n) acc[m][n] = v16f{};
+    const int wm = wave / WN * TM * 32, wv = wave % WN * TN * 32;
+    load(0);
+    for (int k0 = 0; k0 < co; k0 += KSTEP) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < GP; ++i) {
+            const v4f g = masked(G[i], Y[i]);
+            put4(s_g + (i * 32 + gr) * KROW + gk, BN * KROW, g);
+            if (g_out != nullptr && ct == 0) {
+                const long long v = v0 + i * 32 + gr;
+                float *to = g_out + v * co + k0 + gk;
+                const int left = co - k0 - gk;
+                if (v < V) {
+                    if (left >= 4) *reinterpret_cast<Io<float>::vec *>(to) = g;
+                    else
+#pragma unroll
+                        for (int j = 0; j < 3; ++j) if (j < left) to[j] = g[j];
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < WG; ++i) {
+            const Split8 p = split8(W[i]);
+            uint16_t *to = s_w + wn * KROW + wk + i * (THREADS / BM) * 8;
+            *reinterpret_cast<v4u *>(to) = __builtin_bit_cast(v4u, p.hi);
+            *reinterpret_cast<v4u *>(to + BM * KROW) = __builtin_bit_cast(v4u, p.mid);
+            *reinterpret_cast<v4u *>(to + 2 * BM * KROW) = __builtin_bit_cast(v4u, p.lo);
+        }
+        if (k0 + KSTEP < co) load(k0 + KSTEP);
+        __syncthreads();
+        if (gx == nullptr) continue;
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            v8bf A[TM][3], B[TN][3];
+#pragma unroll
+            for (int p = 0; p < 3; ++p) {
+#pragma unroll
+                for (int m = 0; m < TM; ++m) A[m][p] = row_of(s_w + (p * BM + wm + m * 32 + lo) * KROW + ks * 16 + 8 * half);
+#pragma unroll
+                for (int n = 0; n < TN; ++n) B[n][p] = row_of(s_g + (p * BN + wv + n * 32 + lo) * KROW + ks * 16 + 8 * half);
+            }
+            // small products first; each pass over the tiles leaves every accumulator time to settle
+#pragma unroll
+            for (int e = 0; e < 6; ++e) {
+                constexpr int PA[6] = {2, 0, 1, 1, 0, 0}, PB[6] = {0, 2, 1, 0, 1, 0};
+#pragma unroll
+                for (int m = 0; m < TM; ++m)
+#pragma unroll
+                    for (int n = 0; n < TN; ++n) acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[m][PA[e]], B[n][PB[e]], acc[m][n], 0, 0, 0);
+            }
+        }
+    }
+    if (gx == nullptr) return;
+#pragma unroll
+    for (int n = 0; n < TN; ++n) {
+        const long long v = v0 + wv + n * 32 + lo;
+        if (v >= V) continue;
+#pragma unroll
+        for (int m = 0; m < TM; ++m)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int c = c0 + wm + m * 32 + 8 * q + 4 * half;
+                float *to = gx + v * ci + c;
+                if (c + 4 <= ci) *reinterpret_cast<Io<float>::vec *>(to) = v4f{acc[m][n][4 * q], acc[m][n][4 * q + 1], acc[m][n][4 * q + 2], acc[m][n][4 * q + 3]};
+                else
+#pragma unroll
+                    for (int j = 0; j < 3; ++j) if (c + j < ci) to[j] = acc[m][n][4 * q + j];
+            }
+    }
+}
+
+// gw and gbias, partial sums over ranges of voxels.  M = co, N = ci, K = voxel: a thread loads 4 channels of 4 voxels and turns them in registers.
+template <int WM, int TM, int WN, int TN>
+__global__ __launch_bounds__(THREADS, 2) void wgrad_kernel(const float *__restrict__ gy, const uint8_t *__restrict__ yc, const uint8_t *__restrict__ xc, const uint8_t *__restrict__ xs,
+                                                           float *__restrict__ part_w, float *__restrict__ part_b, long long V, int ci, int co, int x_relu, long long per_split)
+{
+    constexpr int BM = WM * TM * 32, BN = WN * TN * 32, GU = BM / 4 * 8, XU = BN / 4 * 8;
+    constexpr bool APART = GU + XU <= THREADS;                                   // few enough units for a thread to load one kind only
+    __shared__ uint16_t s_g[3 * BM * KROW], s_x[BN * KROW];
+    const int t = threadIdx.x, l = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), half = l >> 5, lo = l & 31;
+    const long long v0 = (long long)blockIdx.x * per_split, v1 = v0 + per_split < V ? v0 + per_split : V;
+    const bool do_g = t < GU, do_x = xc != nullptr && (APART ? t >= GU && t < GU + XU : t < XU);
+    const int ux = APART ? t - GU : t;
+    const int gc = blockIdx.y * BM + t % (BM / 4) * 4, gv = t / (BM / 4) * 4, xn = blockIdx.z * BN + ux % (BN / 4) * 4, xv = ux / (BN / 4) * 4;
+    v4f G[4];
+    unsigned Y[4], X[4];
+    int S[4], S3[4];
+    auto load = [&](long long v) {
+        if (do_g) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const long long r = v + gv + j, at = r * co + gc;
+                const int left = r < v1 ? co - gc : 0;
+                G[j] = load4(gy + at, left);
+                Y[j] = yc != nullptr ? load4(yc + at, left) : 0x01010101u;
+            }
+        }
+        if (do_x) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const long long r = v + xv + j, at = r * ci + xn;
+                const int left = r < v1 ? ci - xn : 0;
+                X[j] = load4(xc + at, left);
+                S[j] = left > 0 ? xs[at >> 5] : 0;
+                S3[j] = left > 0 ? xs[(at + (left < 4 ? left - 1 : 3)) >> 5] : 0;  // 4 values may reach into the next block
+            }
+        }
+    };
+    v16f acc[TM][TN];
+#pragma unroll
+    for (int m = 0; m < TM; ++m)
+#pragma unroll
+        for (int n = 0; n < TN; ++n) acc[m][n] = v16f{};
+    v4f bsum = {};
+    const int wm = wave / WN * TM * 32, wx = wave % WN * TN * 32;
+    load(v0);
+    for (long long v = v0; v < v1; v += KSTEP) {
+        __syncthreads();
+        if (do_g) {
+            v4f g[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) g[j] = masked(G[j], Y[j]);
+            bsum = bsum + ((g[0] + g[1]) + (g[2] + g[3]));
+#pragma unroll
+            for (int c = 0; c < 4; ++c) put4(s_g + (t % (BM / 4) * 4 + c) * KROW + gv, BM * KROW, v4f{g[0][c], g[1][c], g[2][c], g[3][c]});
+        }
+        if (do_x) {
+            float f[4][4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int at = (int)((v + xv + j) * ci + xn & 31);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) f[j][c] = code_value(X[j] >> (8 * c) & 255u, x_relu, at + c < 32 ? S[j] : S3[j]);
+            }
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                uint2 p;
+                p.x = pack_hi(f[0][c], f[1][c]);
+                p.y = pack_hi(f[2][c], f[3][c]);
+                *reinterpret_cast<uint2 *>(s_x + (ux % (BN / 4) * 4 + c) * KROW + xv) = p;
+            }
+        }
+        if (v + KSTEP < v1) load(v + KSTEP);
+        __syncthreads();
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            v8bf A[TM][3], B[TN];
+#pragma unroll
+            for (int n = 0; n < TN; ++n) B[n] = row_of(s_x + (wx + n * 32 + lo) * KROW + ks * 16 + 8 * half);
+#pragma unroll
+            for (int p = 0; p < 3; ++p)
+#pragma unroll
+                for (int m = 0; m < TM; ++m) A[m][p] = row_of(s_g + (p * BM + wm + m * 32 + lo) * KROW + ks * 16 + 8 * half);
+#pragma unroll
+            for (int p = 2; p >= 0; --p)
+#pragma unroll
+                for (int m = 0; m < TM; ++m)
+#pragma unroll
+                    for (int n = 0; n < TN; ++n) acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[m][p], B[n], acc[m][n], 0, 0, 0);
+        }
+    }
+    float *pw = part_w + (long long)blockIdx.x * co * ci;
+#pragma unroll
+    for (int m = 0; m < TM; ++m)
+#pragma unroll
+        for (int n = 0; n < TN; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int o = blockIdx.y * BM + wm + m * 32 + 8 * (i / 4) + 4 * half + i % 4, c = blockIdx.z * BN + wx + n * 32 + lo;
+                if (o < co && c < ci) pw[(long long)o * ci + c] = acc[m][n][i];
+            }
+    if (blockIdx.z != 0) return;
+    __syncthreads();
+    float *s_b = reinterpret_cast<float *>(s_g);                                 // [8 voxel groups][BM]
+    if (do_g) *reinterpret_cast<v4f *>(s_b + t / (BM / 4) * BM + t % (BM / 4) * 4) = bsum;
+    __syncthreads();
+    if (t < BM && blockIdx.y * BM + t < co) {
+        float b = 0.0f;
+#pragma unroll
+        for (int g = 0; g < 8; ++g) b = b + s_b[g * BM + t];
+        part_b[(long long)blockIdx.x * co + blockIdx.y * BM + t] = b;
+    }
+}
+
+// out[e] = sum over the splits of part[split][e] in a fixed order: 1024 / R elements a workgroup and R ranges of splits; elements [0, nw) are gw's, the rest
+// gbias's.  512 partial sums of 18 x 72 weights with 8 ranges: 21 us, with 32: TIME us.
+template <int R>
+__global__ __launch_bounds__(1024) void reduce_kernel(const float *__restrict__ part_w, const float *__restrict__ part_b, float *__restrict__ gw, float *__restrict__ gb, long long nw,
+                                                      int nb, int splits)
+{
+    constexpr int E = 1024 / R;
+    __shared__ float s[R][E];
+    const int lane = threadIdx.x % E, range = threadIdx.x / E;
+    const long long e = (long long)blockIdx.x * E + lane;
     const bool is_w = e < nw;
     const float *p = is_w ? part_w + e : part_b + (e - nw);
     const long long step = is_w ? nw : nb;
     float acc = 0.0f;
-    if (e < nw + nb)
-        for (int k = range; k < splits; k += 8) acc = acc + p[k * step];
-    s[range][lane] = acc;
-    __syncthreads();
-    if (range == 0 && e < nw + nb) {
-        float t = 0.0f;
-        for (int r = 0; r < 8; ++r) t = t + s[r][lane];
-        if (is_w) { if (gw != nullptr) gw[e] = t; }
-        else if (gb != nullptr) gb[e - nw] = t;
+    if (e < nw + nb) {
+        int k = range;
+        for (; k + 3 * R < splits; k += 4 * R) {
+            const float a = p[k * step], b = p[(k + R) * step], c = p[(k + 2 * R) * step], d = p[(k + 3 * R) * step];
+            acc = acc + ((a + b) + (c + d));
+        }
+        for (; k < splits; k += R) acc = acc + p[k * step];
     }
+    if (R > 1) {
+        s[range][lane] = acc;
+        __syncthreads();
+        if (range != 0) return;
+        acc = 0.0f;
+#pragma unroll
+        for (int r = 0; r < R; ++r) acc = acc + s[r][lane];
+    }
+    if (e >= nw + nb) return;
+    if (is_w) { if (gw != nullptr) gw[e] = acc; }
+    else if (gb != nullptr) gb[e - nw] = acc;
 }
 
-// ---- gx (and g) ------------------------------------------------------------------------------------------------------------------------
-// matrix tile 32 x 32 (M = voxels, N = ci, K = 16 of co); a wave's tile each
-__global__ __launch_bounds__(THREADS) void dgrad_kernel(const float *__restrict__ gy, const uint8_t *__restrict__ yc, const float *__restrict__ w, float *__restrict__ gx,
-                                                        float *__restrict__ g_out, long long V, int ci, int co)
+void reduce_run(const float *part_w, const float *part_b, float *gw, float *gb, long long nw, int nb, long long splits, hipStream_t s)
 {
-    const int l = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const long long vbase = ((long long)blockIdx.x * WAVES + wave) * 32, r = vbase + (l & 31);
-    const int n = blockIdx.y * 32 + (l & 31);
-    v16f acc = {};
-    for (int k0 = 0; k0 < co; k0 += 16) {
-        const int k = k0 + 8 * (l >> 5);
-        float g[8], b[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            g[j] = r < V && k + j < co ? gy[r * co + k + j] : 0.0f;
-            if (yc != nullptr && r < V && k + j < co) g[j] = yc[r * co + k + j] ? g[j] : 0.0f;
-            if (g_out != nullptr && blockIdx.y == 0 && r < V && k + j < co) g_out[r * co + k + j] = g[j];
-            b[j] = n < ci && k + j < co ? w[(long long)(k + j) * ci + n] : 0.0f;
-        }
-        const Split8 A = split8(g), B = split8(b);
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A.lo, B.hi, acc, 0, 0, 0);
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A.hi, B.lo, acc, 0, 0, 0);
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A.mid, B.mid, acc, 0, 0, 0);
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A.mid, B.hi, acc, 0, 0, 0);
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A.hi, B.mid, acc, 0, 0, 0);
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A.hi, B.hi, acc, 0, 0, 0);
-    }
-    if (gx == nullptr) return;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        const long long row = vbase + 8 * (i / 4) + 4 * (l >> 5) + i % 4;
-        if (row < V && n < ci) gx[row * ci + n] = acc[i];
-    }
+    const long long n = nw + nb;
+    if (splits >= 64) reduce_kernel<32><<<dim3((unsigned)((n + 31) / 32)), 1024, 0, s>>>(part_w, part_b, gw, gb, nw, nb, (int)splits);
+    else if (splits >= 8) reduce_kernel<8><<<dim3((unsigned)((n + 127) / 128)), 1024, 0, s>>>(part_w, part_b, gw, gb, nw, nb, (int)splits);
+    else reduce_kernel<1><<<dim3((unsigned)((n + 1023) / 1024)), 1024, 0, s>>>(part_w, part_b, gw, gb, nw, nb, (int)splits);
 }
 
 // floats of one wave's LDS tiles: 32 voxels of gradients (and a row's overhang; gx's rows take the same place later), 32 of bf16 inputs (and theirs)
@@ -390,15 +593,40 @@ __global__ __launch_bounds__(THREADS, MT * NT <= 3 ? 2 : 1) void fused_kernel(co
     for (int t = threadIdx.x; t < co; t += THREADS) part_b[(long long)blockIdx.x * co + t] = sumb[t];
 }
 
-// voxels a workgroup of wgrad_kernel sums: enough workgroups for the card, not so many that the partial sums outweigh the inputs
-inline long long wgrad_split(long long V, int ci, int co)
+// the tiles of wgrad_kernel (both axes 64 or 128) and the voxels one workgroup sums: about two workgroups a CU, at least 128 voxels each
+struct WgradPlan { int bm, bn; long long tiles, per, splits; };
+inline WgradPlan wgrad_plan(long long V, int ci, int co)
 {
-    const long long tiles = (long long)((co + 31) / 32) * ((ci + 31) / 32);
-    long long splits = 1 + 2048 / tiles;
-    const long long most = (V + 255) / 256;
+    WgradPlan p;
+    p.bm = co > 64 ? 128 : 64;
+    p.bn = ci > 64 ? 128 : 64;
+    p.tiles = (long long)((co + p.bm - 1) / p.bm) * ((ci + p.bn - 1) / p.bn);
+    long long splits = (512 + p.tiles - 1) / p.tiles;
+    const long long most = (V + 127) / 128;
     if (splits > most) splits = most;
-    const long long per = (V + splits - 1) / splits;
-    return (per + 15) / 16 * 16;
+    p.per = ((V + splits - 1) / splits + KSTEP - 1) / KSTEP * KSTEP;
+    p.splits = (V + p.per - 1) / p.per;
+    return p;
+}
+
+struct Args { const float *gy; const uint8_t *yc; const float *w; const uint8_t *xc, *xs; float *gx, *g, *part_w, *part_b; long long V; int ci, co, x_relu; };
+
+template <int WM, int TM, int WN, int TN>
+void wgrad_launch(const WgradPlan &p, const Args &a, bool want_w, hipStream_t s)
+{
+    const dim3 grid((unsigned)p.splits, (unsigned)((a.co + p.bm - 1) / p.bm), want_w ? (unsigned)((a.ci + p.bn - 1) / p.bn) : 1u);
+    wgrad_kernel<WM, TM, WN, TN><<<grid, THREADS, 0, s>>>(a.gy, a.yc, a.xc, a.xs, a.part_w, a.part_b, a.V, a.ci, a.co, a.x_relu, p.per);
+}
+
+template <int WM, int TM, int WN, int TN>
+int dgrad_launch(const Args &a, hipStream_t s)
+{
+    constexpr int BM = WM * TM * 32, BN = WN * TN * 32;
+    const int ci_tiles = a.gx ? (a.ci + BM - 1) / BM : 1;
+    const long long ranges = ((a.V + BN - 1) / BN + 7) / 8 * 8;
+    if (ranges * ci_tiles >= (1LL << 24)) return MDT_ERR_UNSUPPORTED;             // 2^32 threads are the most of a launch
+    dgrad_kernel<WM, TM, WN, TN><<<dim3((unsigned)(ranges * ci_tiles)), THREADS, 0, s>>>(a.gy, a.yc, a.w, a.gx, a.g, a.V, a.ci, a.co, ci_tiles);
+    return MDT_OK;
 }
 
 struct FusedPlan { int mt, nt, lds, blocks; };
@@ -420,10 +648,8 @@ inline FusedPlan fused_plan(long long V, int ci, int co)
     return p;
 }
 
-struct FusedArgs { const float *gy; const uint8_t *yc; const float *w; const uint8_t *xc, *xs; float *gx, *g, *part_w, *part_b; long long V; int ci, co, x_relu; };
-
 template <int MT, int NT>
-int fused_launch(const FusedPlan &p, const FusedArgs &a, hipStream_t s)
+int fused_launch(const FusedPlan &p, const Args &a, hipStream_t s)
 {
     const auto kernel = a.g != nullptr ? fused_kernel<MT, NT, true> : fused_kernel<MT, NT, false>;
     if (hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, p.lds) != hipSuccess) return MDT_ERR_LAUNCH_FAILED;
@@ -431,7 +657,7 @@ int fused_launch(const FusedPlan &p, const FusedArgs &a, hipStream_t s)
     return MDT_OK;
 }
 
-int fused_run(const FusedPlan &p, const FusedArgs &a, hipStream_t s)
+int fused_run(const FusedPlan &p, const Args &a, hipStream_t s)
 {
     switch (p.mt * 10 + p.nt) {
         case 11: return fused_launch<1, 1>(p, a, s);
@@ -462,8 +688,7 @@ extern "C" {
 size_t mdt_conv1x1_act8_backward_workspace_bytes(long long n_voxels, int c_in, int c_out)
 {
     if (n_voxels < 1 || c_in < 1 || c_out < 1 || c_in > 65536 || c_out > 65536) return 256;
-    const long long per = wgrad_split(n_voxels, c_in, c_out);
-    long long splits = (n_voxels + per - 1) / per;
+    long long splits = wgrad_plan(n_voxels, c_in, c_out).splits;
     const FusedPlan p = fused_plan(n_voxels, c_in, c_out);
     if (p.blocks > splits) splits = p.blocks;
     return (size_t)(splits * ((long long)c_in * c_out + c_out)) * 4 + 256;
@@ -475,30 +700,35 @@ int mdt_conv1x1_act8_backward(const float *gy, const float *w, const void *x_cod
     if (n_voxels < 0 || n_voxels > (1LL << 30) || c_in < 1 || c_out < 1 || c_in > 65536 || c_out > 65536) return MDT_ERR_INVALID_ARGUMENT;
     const hipStream_t s = (hipStream_t)stream;
     const bool sums = gw != nullptr || gbias != nullptr;
-    if (n_voxels > 0 && (!gy || (gx && !w) || (gw && (!x_codes || !x_scales)))) return MDT_ERR_INVALID_ARGUMENT;
-    const long long per = n_voxels > 0 ? wgrad_split(n_voxels, c_in, c_out) : 16, splits = (n_voxels + per - 1) / per;
-    if (sums && n_voxels > 0 && (workspace == nullptr || workspace_bytes < mdt_conv1x1_act8_backward_workspace_bytes(n_voxels, c_in, c_out))) return MDT_ERR_WORKSPACE_TOO_SMALL;
-    const long long nw = (long long)c_in * c_out;
-    const FusedPlan p = n_voxels > 0 && gx && gw ? fused_plan(n_voxels, c_in, c_out) : FusedPlan{0, 0, 0, 0};
-    if (p.mt > 0) {
-        float *part_w = (float *)workspace, *part_b = part_w + p.blocks * nw;
-        const FusedArgs a = {gy, (const uint8_t *)y_codes, w, (const uint8_t *)x_codes, (const uint8_t *)x_scales, gx, g, part_w, part_b, n_voxels, c_in, c_out, x_relu};
-        const int rc = fused_run(p, a, s);
-        if (rc != MDT_OK) return rc;
-        reduce_kernel<<<dim3((unsigned)((nw + c_out + 31) / 32)), 256, 0, s>>>(part_w, part_b, gw, gbias, nw, c_out, p.blocks);
+    const long long V = n_voxels, nw = (long long)c_in * c_out;
+    if (V == 0) {                                                                // sums over no voxels
+        if (sums) reduce_run(nullptr, nullptr, gw, gbias, nw, c_out, 0, s);
         return launch_check();
     }
-    float *part_w = (float *)workspace, *part_b = part_w + splits * nw;
-    if (n_voxels > 0 && (gx || g)) {
-        const dim3 grid((unsigned)((n_voxels + 32 * WAVES - 1) / (32 * WAVES)), gx ? (unsigned)((c_in + 31) / 32) : 1u);
-        dgrad_kernel<<<grid, THREADS, 0, s>>>(gy, (const uint8_t *)y_codes, w, gx, g, n_voxels, c_in, c_out);
+    if (!gy || (gx && !w) || (gw && (!x_codes || !x_scales)) || ((uintptr_t)x_codes & 3) || ((uintptr_t)y_codes & 3)) return MDT_ERR_INVALID_ARGUMENT;
+    if (sums && (workspace == nullptr || workspace_bytes < mdt_conv1x1_act8_backward_workspace_bytes(V, c_in, c_out))) return MDT_ERR_WORKSPACE_TOO_SMALL;
+    Args a = {gy, (const uint8_t *)y_codes, w, (const uint8_t *)x_codes, (const uint8_t *)x_scales, gx, g, (float *)workspace, nullptr, V, c_in, c_out, x_relu};
+    const FusedPlan p = gx && gw ? fused_plan(V, c_in, c_out) : FusedPlan{0, 0, 0, 0};
+    if (p.mt > 0) {
+        a.part_b = a.part_w + p.blocks * nw;
+        const int rc = fused_run(p, a, s);
+        if (rc != MDT_OK) return rc;
+        reduce_run(a.part_w, a.part_b, gw, gbias, nw, c_out, p.blocks, s);
+        return launch_check();
+    }
+    if (gx || g) {
+        const int rc = gx && c_in > 64 ? dgrad_launch<2, 2, 2, 2>(a, s) : dgrad_launch<1, 2, 4, 1>(a, s);
+        if (rc != MDT_OK) return rc;
     }
     if (sums) {
-        if (n_voxels > 0) {
-            const dim3 grid((unsigned)splits, (unsigned)((c_out + 31) / 32), gw ? (unsigned)((c_in + 31) / 32) : 1u);
-            wgrad_kernel<<<grid, THREADS, 0, s>>>(gy, (const uint8_t *)y_codes, (const uint8_t *)x_codes, (const uint8_t *)x_scales, part_w, part_b, n_voxels, c_in, c_out, x_relu, per);
-        }
-        reduce_kernel<<<dim3((unsigned)((nw + c_out + 31) / 32)), 256, 0, s>>>(part_w, part_b, gw, gbias, nw, c_out, (int)splits);
+        const WgradPlan q = wgrad_plan(V, c_in, c_out);
+        a.part_b = a.part_w + q.splits * nw;
+        if (gw == nullptr) a.xc = nullptr;
+        if (q.bm == 128 && q.bn == 128) wgrad_launch<2, 2, 2, 2>(q, a, gw != nullptr, s);
+        else if (q.bm == 128) wgrad_launch<4, 1, 1, 2>(q, a, gw != nullptr, s);
+        else if (q.bn == 128) wgrad_launch<1, 2, 4, 1>(q, a, gw != nullptr, s);
+        else wgrad_launch<2, 1, 2, 1>(q, a, gw != nullptr, s);
+        reduce_run(a.part_w, a.part_b, gw, gbias, nw, c_out, q.splits, s);
     }
     return launch_check();
 }
