@@ -45,7 +45,9 @@ __device__ __forceinline__ Split8 split8(const float (&v)[8])
 
 __device__ __forceinline__ float code_value(unsigned c, bool is_relu, int b) { return (is_relu ? (float)c : (float)(int8_t)c) * scale_of(b); }
 
-// ---- any number of channels: one product a kernel, tiles through LDS ------------------------------------------------------------------------
+struct Args { const float *gy; const uint8_t *yc; const float *w; const uint8_t *xc, *xs; float *gx, *g, *part_w, *part_b; long long V; int ci, co, x_relu; };
+
+// ---- any number of channels: one product a workgroup, tiles through LDS ------------------------------------------------------------------------
 // Both kernels cut what they load into bf16 pieces once, put the pieces into LDS with the summed axis innermost (32 entries and 8 of padding a row: the
 // 16-byte reads and writes of neighbouring rows fall into different banks) and hold the next step's loads in registers meanwhile.  4 waves, WM x WN of
 // them with TM x TN matrix tiles of 32 x 32 each.
@@ -53,23 +55,38 @@ constexpr int KSTEP = 32, KROW = KSTEP + 8;
 
 __device__ __forceinline__ v8bf row_of(const uint16_t *p) { return __builtin_bit_cast(v8bf, *reinterpret_cast<const v4u *>(p)); }
 
-// up to 4 consecutive values from p on, zeros behind `left`
-__device__ __forceinline__ v4f load4(const float *p, int left)
-{
-    if (left >= 4) return *reinterpret_cast<const Io<float>::vec *>(p);
-    v4f v = {};
-#pragma unroll
-    for (int j = 0; j < 3; ++j) if (j < left) v[j] = p[j];
-    return v;
-}
-__device__ __forceinline__ unsigned load4(const uint8_t *p, int left)
+// A run of values from base[first] on, read 4 at a time at 32-bit offsets without branches (so that the number of loads in flight stays known and a wait for
+// one does not become a wait for all): where 4 values would pass the end of the array, the last 4 are read, and fix() moves them to their places.
+struct Run {
+    long long first;        // of the base: the run's first element, or the array's fourth last
+    int delta, last;        // the run's first element and the last 4 of the array, counted from the base
+    __device__ __forceinline__ Run(long long at, long long n)
+    {
+        first = at < n - 4 ? at : n - 4;
+        delta = (int)(at - first);
+        const long long rest = n - 4 - first;
+        last = rest < (1 << 30) ? (int)rest : 1 << 30;
+    }
+    __device__ __forceinline__ unsigned at(int off) const { return (unsigned)min(off + delta, last); }
+    __device__ __forceinline__ v4f fix(v4f v, int off) const
+    {
+        const int d = off + delta - last;
+        if (d <= 0) return v;
+        if (d & 1) v = v4f{v[1], v[2], v[3], 0.0f};
+        if (d & 2) v = v4f{v[2], v[3], 0.0f, 0.0f};
+        return d < 4 ? v : v4f{};
+    }
+    __device__ __forceinline__ unsigned fix(unsigned v, int off) const
+    {
+        const int d = off + delta - last;
+        return d <= 0 ? v : d < 4 ? v >> (8 * d) : 0u;
+    }
+};
+__device__ __forceinline__ v4f get4(const float *p) { return *reinterpret_cast<const Io<float>::vec *>(p); }
+__device__ __forceinline__ unsigned get4(const uint8_t *p)
 {
     typedef unsigned una __attribute__((aligned(1)));
-    if (left >= 4) return *reinterpret_cast<const una *>(p);
-    unsigned v = 0;
-#pragma unroll
-    for (int j = 0; j < 3; ++j) if (j < left) v |= (unsigned)p[j] << (8 * j);
-    return v;
+    return *reinterpret_cast<const una *>(p);
 }
 __device__ __forceinline__ v4f masked(v4f g, unsigned m)
 {
@@ -90,37 +107,45 @@ __device__ __forceinline__ void put4(uint16_t *to, int plane, v4f v)
     }
 }
 
-// gx (and g).  M = ci, N = voxel, K = co: a lane ends up with 4 consecutive channels of one voxel.
+// gx (and g).  M = ci, N = voxel, K = co: a lane ends up with 4 consecutive channels of one voxel.  Workgroup `id` of ranges of voxels x ci tiles x k_splits
+// ranges of co, whose sums are joined later.
+struct DgradGrid { int ci_tiles, k_splits, k_per; long long groups; float *to; };
 template <int WM, int TM, int WN, int TN>
-__global__ __launch_bounds__(THREADS, 2) void dgrad_kernel(const float *__restrict__ gy, const uint8_t *__restrict__ yc, const float *__restrict__ w, float *__restrict__ gx,
-                                                           float *__restrict__ g_out, long long V, int ci, int co, int ci_tiles)
+__device__ __forceinline__ void dgrad_tile(uint16_t *smem, const Args &a, const DgradGrid &grid, unsigned id)
 {
-    constexpr int BM = WM * TM * 32, BN = WN * TN * 32, GP = BN / 32, WG = BM / 64;
-    __shared__ uint16_t s_w[3 * BM * KROW], s_g[3 * BN * KROW];
+    constexpr int BM = WM * TM * 32, BN = WN * TN * 32, GP = BN / 32, WG = BM / 64, DEPTH = TM * TN > 1 ? 1 : 2;    // DEPTH: steps loaded ahead
+    const uint8_t *__restrict__ yc = a.yc;
+    float *__restrict__ g_out = a.g;
+    const long long V = a.V;
+    const int ci = a.ci, co = a.co;
+    uint16_t *s_w = smem, *s_g = smem + 3 * BM * KROW;
     const int t = threadIdx.x, l = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), half = l >> 5, lo = l & 31;
-    // the ci tiles of one range of voxels follow each other on one XCD (workgroups go to the 8 XCDs in turn), whose L2 then holds the range's gradients
-    const int xcd = blockIdx.x % 8, turn = blockIdx.x / 8, ct = turn % ci_tiles;
-    const long long v0 = ((long long)(turn / ci_tiles) * 8 + xcd) * BN;
-    if (v0 >= V) return;
-    const int c0 = ct * BM, gr = t >> 3, gk = (t & 7) * 4, wn = t % BM, wk = t / BM * 8;
-    v4f G[GP];
-    unsigned Y[GP];
-    float W[WG][8];
-    auto load = [&](int k0) {
+    // the tiles of one range of voxels follow each other on one XCD (workgroups go to the 8 XCDs in turn), whose L2 then holds the range's gradients
+    const unsigned xcd = id % 8, turn = id / 8, tile = turn % (grid.ci_tiles * grid.k_splits);
+    const int ct = tile % grid.ci_tiles, split = tile / grid.ci_tiles, kb = split * grid.k_per, ke = min(kb + grid.k_per, co);
+    const long long v0 = ((long long)(turn / (grid.ci_tiles * grid.k_splits)) * 8 + xcd) * BN;
+    if (v0 >= V || kb >= co) return;
+    float *__restrict__ gx = grid.to + split * V * ci;
+    // gradients: 8 lanes a row of 32, row gr + 32 i; weights: a lane a column, a wave (or two) 8 rows
+    const int c0 = ct * BM, gr = t >> 3, gk = (t & 7) * 4, wn = t % BM, wk = wave / (BM / 64) * 8;
+    const Run run(v0 * co, V * co);
+    const bool ragged = v0 + BN + 4 >= V;                                        // 4 values of a row may pass the array's end (rows may be as short as 1)
+    const float *__restrict__ gy = a.gy + run.first, *__restrict__ w = a.w + min(c0 + wn, ci - 1);
+    if (yc != nullptr) yc += run.first;
+    v4f G[DEPTH][GP];
+    unsigned Y[DEPTH][GP];
+    float W[DEPTH][WG][8];
+    auto load = [&](v4f (&G)[GP], unsigned (&Y)[GP], float (&W)[WG][8], int k0) {
+        if (yc != nullptr) {
 #pragma unroll
-        for (int i = 0; i < GP; ++i) {
-            const long long v = v0 + i * 32 + gr, at = (v < V ? v : V - 1) * co + k0 + gk;
-            const int left = co - k0 - gk;
-            G[i] = load4(gy + at, left);
-            Y[i] = yc != nullptr ? load4(yc + at, left) : 0x01010101u;
+            for (int i = 0; i < GP; ++i) Y[i] = get4(yc + run.at((i * 32 + gr) * co + k0 + gk));
         }
+#pragma unroll
+        for (int i = 0; i < GP; ++i) G[i] = get4(gy + run.at((i * 32 + gr) * co + k0 + gk));
 #pragma unroll
         for (int i = 0; i < WG; ++i)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int k = k0 + wk + i * (THREADS / BM) * 8 + j, n = c0 + wn;
-                W[i][j] = k < co && n < ci ? w[(long long)k * ci + n] : 0.0f;
-            }
+            for (int j = 0; j < 8; ++j) W[i][j] = w[(long long)min(k0 + wk + i * (THREADS / BM) * 8 + j, ke - 1) * ci];
     };
     v16f acc[TM][TN];
 #pragma unroll
@@ -128,17 +153,22 @@ __global__ __launch_bounds__(THREADS, 2) void dgrad_kernel(const float *__restri
 #pragma unroll
         for (int n = 0; n < TN; ++n) acc[m][n] = v16f{};
     const int wm = wave / WN * TM * 32, wv = wave % WN * TN * 32;
-    load(0);
-    for (int k0 = 0; k0 < co; k0 += KSTEP) {
+    auto step = [&](v4f (&G)[GP], unsigned (&Y)[GP], float (&W)[WG][8], int k0) {
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < GP; ++i) {
-            const v4f g = masked(G[i], Y[i]);
+            v4f g = G[i];
+            if (ragged) g = run.fix(g, (i * 32 + gr) * co + k0 + gk);
+            if (yc != nullptr) g = masked(g, ragged ? run.fix(Y[i], (i * 32 + gr) * co + k0 + gk) : Y[i]);
+            if (k0 + KSTEP > ke) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) g[j] = k0 + gk + j < ke ? g[j] : 0.0f;
+            }
             put4(s_g + (i * 32 + gr) * KROW + gk, BN * KROW, g);
             if (g_out != nullptr && ct == 0) {
                 const long long v = v0 + i * 32 + gr;
                 float *to = g_out + v * co + k0 + gk;
-                const int left = co - k0 - gk;
+                const int left = ke - k0 - gk;
                 if (v < V) {
                     if (left >= 4) *reinterpret_cast<Io<float>::vec *>(to) = g;
                     else
@@ -149,15 +179,19 @@ __global__ __launch_bounds__(THREADS, 2) void dgrad_kernel(const float *__restri
         }
 #pragma unroll
         for (int i = 0; i < WG; ++i) {
+            if (k0 + KSTEP > ke) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) W[i][j] = k0 + wk + i * (THREADS / BM) * 8 + j < ke ? W[i][j] : 0.0f;
+            }
             const Split8 p = split8(W[i]);
             uint16_t *to = s_w + wn * KROW + wk + i * (THREADS / BM) * 8;
             *reinterpret_cast<v4u *>(to) = __builtin_bit_cast(v4u, p.hi);
             *reinterpret_cast<v4u *>(to + BM * KROW) = __builtin_bit_cast(v4u, p.mid);
             *reinterpret_cast<v4u *>(to + 2 * BM * KROW) = __builtin_bit_cast(v4u, p.lo);
         }
-        if (k0 + KSTEP < co) load(k0 + KSTEP);
+        if (k0 + DEPTH * KSTEP < ke) load(G, Y, W, k0 + DEPTH * KSTEP);
         __syncthreads();
-        if (gx == nullptr) continue;
+        if (a.gx == nullptr) return;
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
             v8bf A[TM][3], B[TN][3];
@@ -178,8 +212,14 @@ __global__ __launch_bounds__(THREADS, 2) void dgrad_kernel(const float *__restri
                     for (int n = 0; n < TN; ++n) acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[m][PA[e]], B[n][PB[e]], acc[m][n], 0, 0, 0);
             }
         }
+    };
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) if (kb + d * KSTEP < ke) load(G[d], Y[d], W[d], kb + d * KSTEP);
+    for (int k0 = kb; k0 < ke; k0 += DEPTH * KSTEP) {
+#pragma unroll
+        for (int d = 0; d < DEPTH; ++d) if (k0 + d * KSTEP < ke) step(G[d], Y[d], W[d], k0 + d * KSTEP);
     }
-    if (gx == nullptr) return;
+    if (a.gx == nullptr) return;
 #pragma unroll
     for (int n = 0; n < TN; ++n) {
         const long long v = v0 + wv + n * 32 + lo;
@@ -199,39 +239,49 @@ __global__ __launch_bounds__(THREADS, 2) void dgrad_kernel(const float *__restri
 }
 
 // gw and gbias, partial sums over ranges of voxels.  M = co, N = ci, K = voxel: a thread loads 4 channels of 4 voxels and turns them in registers.
-template <int WM, int TM, int WN, int TN>
-__global__ __launch_bounds__(THREADS, 2) void wgrad_kernel(const float *__restrict__ gy, const uint8_t *__restrict__ yc, const uint8_t *__restrict__ xc, const uint8_t *__restrict__ xs,
-                                                           float *__restrict__ part_w, float *__restrict__ part_b, long long V, int ci, int co, int x_relu, long long per_split)
+struct WgradGrid { int co_tiles, ci_tiles; long long per, splits, groups; };
+template <int WM, int TM, int WN, int TN, bool EVEN>
+__device__ __forceinline__ void wgrad_tile(uint16_t *smem, const Args &a, const WgradGrid &grid, unsigned id)
 {
     constexpr int BM = WM * TM * 32, BN = WN * TN * 32, GU = BM / 4 * 8, XU = BN / 4 * 8;
     constexpr bool APART = GU + XU <= THREADS;                                   // few enough units for a thread to load one kind only
-    __shared__ uint16_t s_g[3 * BM * KROW], s_x[BN * KROW];
+    const uint8_t *__restrict__ yc = a.yc;
+    const long long V = a.V;
+    const int ci = a.ci, co = a.co, x_relu = a.x_relu;
+    uint16_t *s_g = smem, *s_x = smem + 3 * BM * KROW;
     const int t = threadIdx.x, l = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), half = l >> 5, lo = l & 31;
-    const long long v0 = (long long)blockIdx.x * per_split, v1 = v0 + per_split < V ? v0 + per_split : V;
-    const bool do_g = t < GU, do_x = xc != nullptr && (APART ? t >= GU && t < GU + XU : t < XU);
+    const unsigned xcd = id % 8, turn = id / 8, tile = turn % (grid.co_tiles * grid.ci_tiles);
+    const long long split = (long long)(turn / (grid.co_tiles * grid.ci_tiles)) * 8 + xcd;
+    if (split >= grid.splits) return;
+    const int bx = tile % grid.ci_tiles, by = tile / grid.ci_tiles;
+    const long long v0 = split * grid.per, v1 = v0 + grid.per < V ? v0 + grid.per : V;
+    const bool do_g = t < GU, do_x = a.xc != nullptr && (APART ? t >= GU && t < GU + XU : t < XU);
     const int ux = APART ? t - GU : t;
-    const int gc = blockIdx.y * BM + t % (BM / 4) * 4, gv = t / (BM / 4) * 4, xn = blockIdx.z * BN + ux % (BN / 4) * 4, xv = ux / (BN / 4) * 4;
-    v4f G[4];
-    unsigned Y[4], X[4];
-    int S[4], S3[4];
-    auto load = [&](long long v) {
+    // neighbouring lanes take neighbouring voxels of the same channels: 8 of them fill a row of LDS
+    const int gc = t / 8 * 4, gv = t % 8 * 4, xn = ux / 8 * 4, xv = ux % 8 * 4, c0 = by * BM, n0 = bx * BN;
+    const long long last_scale = (V * ci - 1) >> 5;
+    struct Ahead { v4f G[4]; unsigned Y[4], X[4]; int S[4], S3[4]; } ahead[2];    // two steps' loads
+    // channels behind co or ci belong to the next voxels and end in rows and columns that are not stored
+    auto load = [&](Ahead &h, long long v) {
         if (do_g) {
+            const Run run(v * co, V * co);
+            if (yc != nullptr) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const long long r = v + gv + j, at = r * co + gc;
-                const int left = r < v1 ? co - gc : 0;
-                G[j] = load4(gy + at, left);
-                Y[j] = yc != nullptr ? load4(yc + at, left) : 0x01010101u;
+                for (int j = 0; j < 4; ++j) h.Y[j] = get4(yc + run.first + run.at((gv + j) * co + c0 + gc));
             }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) h.G[j] = get4(a.gy + run.first + run.at((gv + j) * co + c0 + gc));
         }
         if (do_x) {
+            const Run run(v * ci, V * ci);                                       // v is a multiple of 32: the run begins with a block
+            const uint8_t *ps = a.xs + (v * ci >> 5);
+            const int most = (int)min(last_scale - (v * ci >> 5), 1LL << 30);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const long long r = v + xv + j, at = r * ci + xn;
-                const int left = r < v1 ? ci - xn : 0;
-                X[j] = load4(xc + at, left);
-                S[j] = left > 0 ? xs[at >> 5] : 0;
-                S3[j] = left > 0 ? xs[(at + (left < 4 ? left - 1 : 3)) >> 5] : 0;  // 4 values may reach into the next block
+                const int off = (xv + j) * ci + n0 + xn;
+                h.X[j] = get4(a.xc + run.first + run.at(off));
+                h.S[j] = ps[(unsigned)min(off >> 5, most)];
+                if (!EVEN) h.S3[j] = ps[(unsigned)min((off + 3) >> 5, most)];    // 4 values may reach into the next block
             }
         }
     };
@@ -242,34 +292,46 @@ __global__ __launch_bounds__(THREADS, 2) void wgrad_kernel(const float *__restri
         for (int n = 0; n < TN; ++n) acc[m][n] = v16f{};
     v4f bsum = {};
     const int wm = wave / WN * TM * 32, wx = wave % WN * TN * 32;
-    load(v0);
-    for (long long v = v0; v < v1; v += KSTEP) {
+    auto step = [&](Ahead &h, long long v) {
+        const bool ragged = v + KSTEP + 4 >= V;
         __syncthreads();
         if (do_g) {
+            const Run run(v * co, V * co);
             v4f g[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) g[j] = masked(G[j], Y[j]);
+            for (int j = 0; j < 4; ++j) {
+                const int off = (gv + j) * co + c0 + gc;
+                g[j] = ragged ? run.fix(h.G[j], off) : h.G[j];
+                if (yc != nullptr) g[j] = masked(g[j], ragged ? run.fix(h.Y[j], off) : h.Y[j]);
+                if (v + KSTEP > v1 && v + gv + j >= v1) g[j] = v4f{};
+            }
             bsum = bsum + ((g[0] + g[1]) + (g[2] + g[3]));
 #pragma unroll
-            for (int c = 0; c < 4; ++c) put4(s_g + (t % (BM / 4) * 4 + c) * KROW + gv, BM * KROW, v4f{g[0][c], g[1][c], g[2][c], g[3][c]});
+            for (int c = 0; c < 4; ++c) put4(s_g + (gc + c) * KROW + gv, BM * KROW, v4f{g[0][c], g[1][c], g[2][c], g[3][c]});
         }
         if (do_x) {
+            const Run run(v * ci, V * ci);
             float f[4][4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const int at = (int)((v + xv + j) * ci + xn & 31);
+                const int off = (xv + j) * ci + n0 + xn;
+                const unsigned x = ragged ? run.fix(h.X[j], off) : h.X[j];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) f[j][c] = code_value(X[j] >> (8 * c) & 255u, x_relu, at + c < 32 ? S[j] : S3[j]);
+                for (int c = 0; c < 4; ++c) f[j][c] = code_value(x >> (8 * c) & 255u, x_relu, EVEN || (off & 31) + c < 32 ? h.S[j] : h.S3[j]);
+                if (v + KSTEP > v1 && v + xv + j >= v1) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) f[j][c] = 0.0f;
+                }
             }
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 uint2 p;
                 p.x = pack_hi(f[0][c], f[1][c]);
                 p.y = pack_hi(f[2][c], f[3][c]);
-                *reinterpret_cast<uint2 *>(s_x + (ux % (BN / 4) * 4 + c) * KROW + xv) = p;
+                *reinterpret_cast<uint2 *>(s_x + (xn + c) * KROW + xv) = p;
             }
         }
-        if (v + KSTEP < v1) load(v + KSTEP);
+        if (v + 2 * KSTEP < v1) load(h, v + 2 * KSTEP);
         __syncthreads();
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
@@ -287,71 +349,113 @@ __global__ __launch_bounds__(THREADS, 2) void wgrad_kernel(const float *__restri
 #pragma unroll
                     for (int n = 0; n < TN; ++n) acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[m][p], B[n], acc[m][n], 0, 0, 0);
         }
+    };
+    load(ahead[0], v0);
+    if (v0 + KSTEP < v1) load(ahead[1], v0 + KSTEP);
+    for (long long v = v0; v < v1; v += 2 * KSTEP) {
+        step(ahead[0], v);
+        if (v + KSTEP < v1) step(ahead[1], v + KSTEP);
     }
-    float *pw = part_w + (long long)blockIdx.x * co * ci;
+    float *pw = a.part_w + split * co * ci;
 #pragma unroll
     for (int m = 0; m < TM; ++m)
 #pragma unroll
         for (int n = 0; n < TN; ++n)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                const int o = blockIdx.y * BM + wm + m * 32 + 8 * (i / 4) + 4 * half + i % 4, c = blockIdx.z * BN + wx + n * 32 + lo;
+                const int o = by * BM + wm + m * 32 + 8 * (i / 4) + 4 * half + i % 4, c = bx * BN + wx + n * 32 + lo;
                 if (o < co && c < ci) pw[(long long)o * ci + c] = acc[m][n][i];
             }
-    if (blockIdx.z != 0) return;
+    if (bx != 0) return;
     __syncthreads();
     float *s_b = reinterpret_cast<float *>(s_g);                                 // [8 voxel groups][BM]
-    if (do_g) *reinterpret_cast<v4f *>(s_b + t / (BM / 4) * BM + t % (BM / 4) * 4) = bsum;
+    if (do_g) *reinterpret_cast<v4f *>(s_b + t % 8 * BM + gc) = bsum;
     __syncthreads();
-    if (t < BM && blockIdx.y * BM + t < co) {
+    if (t < BM && by * BM + t < co) {
         float b = 0.0f;
 #pragma unroll
         for (int g = 0; g < 8; ++g) b = b + s_b[g * BM + t];
-        part_b[(long long)blockIdx.x * co + blockIdx.y * BM + t] = b;
+        a.part_b[split * co + by * BM + t] = b;
     }
 }
 
-// out[e] = sum over the splits of part[split][e] in a fixed order: 1024 / R elements a workgroup and R ranges of splits; elements [0, nw) are gw's, the rest
-// gbias's.  512 partial sums of 18 x 72 weights with 8 ranges: 21 us, with 32: TIME us.
-template <int R>
-__global__ __launch_bounds__(1024) void reduce_kernel(const float *__restrict__ part_w, const float *__restrict__ part_b, float *__restrict__ gw, float *__restrict__ gb, long long nw,
-                                                      int nb, int splits)
+// arrays of less than 4 values, which the loads of 4 above cannot read: an element of gx or gw a thread, gbias and g in plain loops
+__global__ __launch_bounds__(THREADS) void tiny_kernel(Args a, float *__restrict__ gw, float *__restrict__ gb)
 {
-    constexpr int E = 1024 / R;
-    __shared__ float s[R][E];
-    const int lane = threadIdx.x % E, range = threadIdx.x / E;
-    const long long e = (long long)blockIdx.x * E + lane;
-    const bool is_w = e < nw;
-    const float *p = is_w ? part_w + e : part_b + (e - nw);
-    const long long step = is_w ? nw : nb;
+    const long long e = (long long)blockIdx.x * THREADS + threadIdx.x, nx = a.V * a.ci, nw = (long long)a.co * a.ci, ng = a.V * a.co;
+    auto g_at = [&](long long v, int o) { return a.yc == nullptr || a.yc[v * a.co + o] ? a.gy[v * a.co + o] : 0.0f; };
+    float t = 0.0f;
+    if (e < nx) {
+        if (a.gx == nullptr) return;
+        for (int o = 0; o < a.co; ++o) t = t + g_at(e / a.ci, o) * a.w[(long long)o * a.ci + e % a.ci];
+        a.gx[e] = t;
+    } else if (e < nx + nw) {
+        if (gw == nullptr) return;
+        const int o = (int)((e - nx) / a.ci), i = (int)((e - nx) % a.ci);
+        for (long long v = 0; v < a.V; ++v) t = t + g_at(v, o) * code_value(a.xc[v * a.ci + i], a.x_relu, a.xs[(v * a.ci + i) >> 5]);
+        gw[e - nx] = t;
+    } else if (e < nx + nw + a.co) {
+        if (gb == nullptr) return;
+        for (long long v = 0; v < a.V; ++v) t = t + g_at(v, (int)(e - nx - nw));
+        gb[e - nx - nw] = t;
+    } else if (e < nx + nw + a.co + ng && a.g != nullptr) {
+        const long long i = e - nx - nw - a.co;
+        a.g[i] = g_at(i / a.co, (int)(i % a.co));
+    }
+}
+
+// one launch for the two products, which do not depend on each other: the first groups sum voxels, the others channels
+template <int W0, int W1, int W2, int W3, int D0, int D1, int D2, int D3, bool EVEN>
+__global__ __launch_bounds__(THREADS, 2) void products_kernel(Args a, WgradGrid wg, DgradGrid dg)
+{
+    constexpr int LW = (W0 * W1 * 3 + W2 * W3) * 32 * KROW, LD = (D0 * D1 + D2 * D3) * 3 * 32 * KROW;
+    __shared__ __attribute__((aligned(16))) uint16_t smem[LW > LD ? LW : LD];
+    if (blockIdx.x < wg.groups) wgrad_tile<W0, W1, W2, W3, EVEN>(smem, a, wg, blockIdx.x);
+    else dgrad_tile<D0, D1, D2, D3>(smem, a, dg, blockIdx.x - (unsigned)wg.groups);
+}
+
+// out[e] = sum over the splits of part[split][e] in a fixed order, for up to three arrays at once.  A workgroup sums 1024 >> log_r elements, each in 1 << log_r
+// interleaved ranges of splits.  512 partial sums of 18 x 72 weights with 8 ranges: 21 us, with 32: 5 us.
+struct Joined { const float *part; float *out; long long n; int splits, log_r; long long groups; };
+__global__ __launch_bounds__(1024) void join_kernel(Joined j0, Joined j1, Joined j2)
+{
+    __shared__ float s[1024];
+    long long id = blockIdx.x;
+    Joined j = j0;
+    if (id >= j0.groups) { id -= j0.groups; j = j1; if (id >= j1.groups) { id -= j1.groups; j = j2; } }
+    const int per = 1024 >> j.log_r, lane = threadIdx.x & (per - 1), range = threadIdx.x >> (10 - j.log_r), R = 1 << j.log_r;
+    const long long e = id * per + lane;
     float acc = 0.0f;
-    if (e < nw + nb) {
+    if (e < j.n) {
+        const float *p = j.part + e;
         int k = range;
-        for (; k + 3 * R < splits; k += 4 * R) {
-            const float a = p[k * step], b = p[(k + R) * step], c = p[(k + 2 * R) * step], d = p[(k + 3 * R) * step];
+        for (; k + 3 * R < j.splits; k += 4 * R) {
+            const float a = p[k * j.n], b = p[(k + R) * j.n], c = p[(k + 2 * R) * j.n], d = p[(k + 3 * R) * j.n];
             acc = acc + ((a + b) + (c + d));
         }
-        for (; k < splits; k += R) acc = acc + p[k * step];
+        for (; k < j.splits; k += R) acc = acc + p[k * j.n];
     }
-    if (R > 1) {
-        s[range][lane] = acc;
-        __syncthreads();
-        if (range != 0) return;
-        acc = 0.0f;
-#pragma unroll
-        for (int r = 0; r < R; ++r) acc = acc + s[r][lane];
-    }
-    if (e >= nw + nb) return;
-    if (is_w) { if (gw != nullptr) gw[e] = acc; }
-    else if (gb != nullptr) gb[e - nw] = acc;
+    s[threadIdx.x] = acc;
+    __syncthreads();
+    if (range != 0 || e >= j.n) return;
+    acc = 0.0f;
+    for (int r = 0; r < R; ++r) acc = acc + s[r * per + lane];
+    j.out[e] = acc;
 }
 
-void reduce_run(const float *part_w, const float *part_b, float *gw, float *gb, long long nw, int nb, long long splits, hipStream_t s)
+inline Joined joined(const float *part, float *out, long long n, long long splits)
 {
-    const long long n = nw + nb;
-    if (splits >= 64) reduce_kernel<32><<<dim3((unsigned)((n + 31) / 32)), 1024, 0, s>>>(part_w, part_b, gw, gb, nw, nb, (int)splits);
-    else if (splits >= 8) reduce_kernel<8><<<dim3((unsigned)((n + 127) / 128)), 1024, 0, s>>>(part_w, part_b, gw, gb, nw, nb, (int)splits);
-    else reduce_kernel<1><<<dim3((unsigned)((n + 1023) / 1024)), 1024, 0, s>>>(part_w, part_b, gw, gb, nw, nb, (int)splits);
+    Joined j = {part, out, out ? n : 0, (int)splits, splits >= 64 ? 5 : splits >= 8 ? 3 : 0, 0};
+    j.groups = (j.n + (1024 >> j.log_r) - 1) / (1024 >> j.log_r);
+    return j;
+}
+
+int join_run(const Joined &a, const Joined &b, const Joined &c, hipStream_t s)
+{
+    const long long groups = a.groups + b.groups + c.groups;
+    if (groups >= (1LL << 22)) return MDT_ERR_UNSUPPORTED;                        // 2^32 threads are the most of a launch
+    if (groups > 0) join_kernel<<<dim3((unsigned)groups), 1024, 0, s>>>(a, b, c);
+    return MDT_OK;
 }
 
 // floats of one wave's LDS tiles: 32 voxels of gradients (and a row's overhang; gx's rows take the same place later), 32 of bf16 inputs (and theirs)
@@ -593,40 +697,47 @@ __global__ __launch_bounds__(THREADS, MT * NT <= 3 ? 2 : 1) void fused_kernel(co
     for (int t = threadIdx.x; t < co; t += THREADS) part_b[(long long)blockIdx.x * co + t] = sumb[t];
 }
 
-// the tiles of wgrad_kernel (both axes 64 or 128) and the voxels one workgroup sums: about two workgroups a CU, at least 128 voxels each
-struct WgradPlan { int bm, bn; long long tiles, per, splits; };
-inline WgradPlan wgrad_plan(long long V, int ci, int co)
+// Tiles of the two products.  gw: 64 or 128 along each axis, about two workgroups a CU, at least 128 voxels each.  gx: 128 x 128 where that gives two workgroups
+// a CU, else 64 x 64; where even those leave CUs idle, the sum over co is split (at least 4 steps each) and joined with gw's.
+struct Plan { int w_m, w_n, d_tile; WgradGrid wg; DgradGrid dg; };
+inline Plan plan_of(long long V, int ci, int co)
 {
-    WgradPlan p;
-    p.bm = co > 64 ? 128 : 64;
-    p.bn = ci > 64 ? 128 : 64;
-    p.tiles = (long long)((co + p.bm - 1) / p.bm) * ((ci + p.bn - 1) / p.bn);
-    long long splits = (512 + p.tiles - 1) / p.tiles;
-    const long long most = (V + 127) / 128;
+    Plan p;
+    p.w_m = co > 64 ? 128 : 64;
+    p.w_n = ci > 64 ? 128 : 64;
+    WgradGrid &w = p.wg;
+    w.co_tiles = (co + p.w_m - 1) / p.w_m;
+    w.ci_tiles = (ci + p.w_n - 1) / p.w_n;
+    const long long tiles = (long long)w.co_tiles * w.ci_tiles, most = (V + 127) / 128;
+    long long splits = (512 + tiles - 1) / tiles;
     if (splits > most) splits = most;
-    p.per = ((V + splits - 1) / splits + KSTEP - 1) / KSTEP * KSTEP;
-    p.splits = (V + p.per - 1) / p.per;
+    w.per = ((V + splits - 1) / splits + KSTEP - 1) / KSTEP * KSTEP;
+    w.splits = (V + w.per - 1) / w.per;
+    w.groups = (w.splits + 7) / 8 * 8 * tiles;
+    DgradGrid &d = p.dg;
+    const long long big = ((V + 127) / 128) * ((ci + 127) / 128);
+    p.d_tile = ci > 64 && big >= 512 ? 128 : 64;
+    d.ci_tiles = (ci + p.d_tile - 1) / p.d_tile;
+    const long long ranges = (V + p.d_tile - 1) / p.d_tile, now = ranges * d.ci_tiles;
+    const int steps = (co + KSTEP - 1) / KSTEP;
+    long long ks = now >= 256 ? 1 : 512 / now;
+    if (ks > steps / 4) ks = steps / 4;
+    if (ks < 1) ks = 1;
+    d.k_per = (int)((steps + ks - 1) / ks) * KSTEP;
+    d.k_splits = (co + d.k_per - 1) / d.k_per;
+    d.groups = (ranges + 7) / 8 * 8 * d.ci_tiles * d.k_splits;
+    d.to = nullptr;
     return p;
 }
 
-struct Args { const float *gy; const uint8_t *yc; const float *w; const uint8_t *xc, *xs; float *gx, *g, *part_w, *part_b; long long V; int ci, co, x_relu; };
-
-template <int WM, int TM, int WN, int TN>
-void wgrad_launch(const WgradPlan &p, const Args &a, bool want_w, hipStream_t s)
+template <int W0, int W1, int W2, int W3>
+void products_launch(const Plan &p, const Args &a, hipStream_t s)
 {
-    const dim3 grid((unsigned)p.splits, (unsigned)((a.co + p.bm - 1) / p.bm), want_w ? (unsigned)((a.ci + p.bn - 1) / p.bn) : 1u);
-    wgrad_kernel<WM, TM, WN, TN><<<grid, THREADS, 0, s>>>(a.gy, a.yc, a.xc, a.xs, a.part_w, a.part_b, a.V, a.ci, a.co, a.x_relu, p.per);
-}
-
-template <int WM, int TM, int WN, int TN>
-int dgrad_launch(const Args &a, hipStream_t s)
-{
-    constexpr int BM = WM * TM * 32, BN = WN * TN * 32;
-    const int ci_tiles = a.gx ? (a.ci + BM - 1) / BM : 1;
-    const long long ranges = ((a.V + BN - 1) / BN + 7) / 8 * 8;
-    if (ranges * ci_tiles >= (1LL << 24)) return MDT_ERR_UNSUPPORTED;             // 2^32 threads are the most of a launch
-    dgrad_kernel<WM, TM, WN, TN><<<dim3((unsigned)(ranges * ci_tiles)), THREADS, 0, s>>>(a.gy, a.yc, a.w, a.gx, a.g, a.V, a.ci, a.co, ci_tiles);
-    return MDT_OK;
+    const dim3 grid((unsigned)(p.wg.groups + p.dg.groups));
+    const bool even = a.ci % 4 == 0;                                            // 4 input codes of a voxel lie in one block
+    const auto kernel = p.d_tile == 128 ? (even ? products_kernel<W0, W1, W2, W3, 2, 2, 2, 2, true> : products_kernel<W0, W1, W2, W3, 2, 2, 2, 2, false>)
+                                        : (even ? products_kernel<W0, W1, W2, W3, 2, 1, 2, 1, true> : products_kernel<W0, W1, W2, W3, 2, 1, 2, 1, false>);
+    kernel<<<grid, THREADS, 0, s>>>(a, p.wg, p.dg);
 }
 
 struct FusedPlan { int mt, nt, lds, blocks; };
@@ -688,10 +799,10 @@ extern "C" {
 size_t mdt_conv1x1_act8_backward_workspace_bytes(long long n_voxels, int c_in, int c_out)
 {
     if (n_voxels < 1 || c_in < 1 || c_out < 1 || c_in > 65536 || c_out > 65536) return 256;
-    long long splits = wgrad_plan(n_voxels, c_in, c_out).splits;
+    const Plan q = plan_of(n_voxels, c_in, c_out);
     const FusedPlan p = fused_plan(n_voxels, c_in, c_out);
-    if (p.blocks > splits) splits = p.blocks;
-    return (size_t)(splits * ((long long)c_in * c_out + c_out)) * 4 + 256;
+    const long long one = (long long)c_in * c_out + c_out, tiled = q.wg.splits * one + (q.dg.k_splits > 1 ? q.dg.k_splits * n_voxels * c_in : 0);
+    return (size_t)(tiled > p.blocks * one ? tiled : p.blocks * one) * 4 + 256;
 }
 
 int mdt_conv1x1_act8_backward(const float *gy, const float *w, const void *x_codes, const void *x_scales, int x_relu, const void *y_codes, float *gx, float *gw, float *gbias, float *g,
@@ -701,36 +812,51 @@ int mdt_conv1x1_act8_backward(const float *gy, const float *w, const void *x_cod
     const hipStream_t s = (hipStream_t)stream;
     const bool sums = gw != nullptr || gbias != nullptr;
     const long long V = n_voxels, nw = (long long)c_in * c_out;
+    const Joined none = {nullptr, nullptr, 0, 0, 0, 0};
     if (V == 0) {                                                                // sums over no voxels
-        if (sums) reduce_run(nullptr, nullptr, gw, gbias, nw, c_out, 0, s);
-        return launch_check();
+        const int rc = join_run(joined(nullptr, gw, nw, 0), joined(nullptr, gbias, c_out, 0), none, s);
+        return rc != MDT_OK ? rc : launch_check();
     }
     if (!gy || (gx && !w) || (gw && (!x_codes || !x_scales)) || ((uintptr_t)x_codes & 3) || ((uintptr_t)y_codes & 3)) return MDT_ERR_INVALID_ARGUMENT;
-    if (sums && (workspace == nullptr || workspace_bytes < mdt_conv1x1_act8_backward_workspace_bytes(V, c_in, c_out))) return MDT_ERR_WORKSPACE_TOO_SMALL;
+    if ((sums || gx) && (workspace == nullptr || workspace_bytes < mdt_conv1x1_act8_backward_workspace_bytes(V, c_in, c_out))) return MDT_ERR_WORKSPACE_TOO_SMALL;
     Args a = {gy, (const uint8_t *)y_codes, w, (const uint8_t *)x_codes, (const uint8_t *)x_scales, gx, g, (float *)workspace, nullptr, V, c_in, c_out, x_relu};
-    const FusedPlan p = gx && gw ? fused_plan(V, c_in, c_out) : FusedPlan{0, 0, 0, 0};
-    if (p.mt > 0) {
-        a.part_b = a.part_w + p.blocks * nw;
-        const int rc = fused_run(p, a, s);
+    const FusedPlan f = gx && gw ? fused_plan(V, c_in, c_out) : FusedPlan{0, 0, 0, 0};
+    if (f.mt > 0) {
+        a.part_b = a.part_w + f.blocks * nw;
+        const int rc = fused_run(f, a, s);
         if (rc != MDT_OK) return rc;
-        reduce_run(a.part_w, a.part_b, gw, gbias, nw, c_out, p.blocks, s);
+        const int rj = join_run(joined(a.part_w, gw, nw, f.blocks), joined(a.part_b, gbias, c_out, f.blocks), none, s);
+        return rj != MDT_OK ? rj : launch_check();
+    }
+    if (V * c_in < 4 || V * c_out < 4) {
+        const long long n = V * c_in + nw + c_out + V * c_out;
+        tiny_kernel<<<dim3((unsigned)((n + THREADS - 1) / THREADS)), THREADS, 0, s>>>(a, gw, gbias);
         return launch_check();
     }
-    if (gx || g) {
-        const int rc = gx && c_in > 64 ? dgrad_launch<2, 2, 2, 2>(a, s) : dgrad_launch<1, 2, 4, 1>(a, s);
-        if (rc != MDT_OK) return rc;
+    Plan p = plan_of(V, c_in, c_out);
+    a.part_b = a.part_w + p.wg.splits * nw;
+    float *part_x = a.part_b + p.wg.splits * c_out;
+    if (gw == nullptr) {                                                         // gbias alone: one column of tiles without inputs
+        a.xc = nullptr;
+        p.wg.groups = sums ? p.wg.groups / p.wg.ci_tiles : 0;
+        p.wg.ci_tiles = 1;
     }
-    if (sums) {
-        const WgradPlan q = wgrad_plan(V, c_in, c_out);
-        a.part_b = a.part_w + q.splits * nw;
-        if (gw == nullptr) a.xc = nullptr;
-        if (q.bm == 128 && q.bn == 128) wgrad_launch<2, 2, 2, 2>(q, a, gw != nullptr, s);
-        else if (q.bm == 128) wgrad_launch<4, 1, 1, 2>(q, a, gw != nullptr, s);
-        else if (q.bn == 128) wgrad_launch<1, 2, 4, 1>(q, a, gw != nullptr, s);
-        else wgrad_launch<2, 1, 2, 1>(q, a, gw != nullptr, s);
-        reduce_run(a.part_w, a.part_b, gw, gbias, nw, c_out, q.splits, s);
+    if (gx == nullptr) {                                                         // g alone: one column of tiles, unsplit
+        p.dg.groups = g ? p.dg.groups / (p.dg.ci_tiles * p.dg.k_splits) : 0;
+        p.dg.ci_tiles = p.dg.k_splits = 1;
+        p.dg.k_per = (c_out + KSTEP - 1) / KSTEP * KSTEP;
     }
-    return launch_check();
+    p.dg.to = p.dg.k_splits > 1 ? part_x : gx;
+    if (p.wg.groups + p.dg.groups >= (1LL << 24)) return MDT_ERR_UNSUPPORTED;    // 2^32 threads are the most of a launch
+    if (p.wg.groups + p.dg.groups > 0) {
+        if (p.w_m == 128 && p.w_n == 128) products_launch<2, 2, 2, 2>(p, a, s);
+        else if (p.w_m == 128) products_launch<4, 1, 1, 2>(p, a, s);
+        else if (p.w_n == 128) products_launch<1, 2, 4, 1>(p, a, s);
+        else products_launch<2, 1, 2, 1>(p, a, s);
+    }
+    const int rj = join_run(joined(a.part_w, gw, nw, p.wg.splits), joined(a.part_b, gbias, c_out, p.wg.splits),
+                            p.dg.k_splits > 1 ? joined(part_x, gx, V * c_in, p.dg.k_splits) : none, s);
+    return rj != MDT_OK ? rj : launch_check();
 }
 
 }  // extern "C"

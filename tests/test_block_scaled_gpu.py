@@ -196,7 +196,8 @@ def test_bias_act_checkpoint8_takes_a_residual_of_another_layout(cuda):
 
 # ---- the backward pass of a 1x1 layer ----------------------------------------------------------------------------------------------
 SHAPES = [(1, 1, 1), (1, 18, 72), (5, 3, 3), (31, 18, 72), (33, 72, 18), (693, 18, 72), (700, 72, 18), (257, 37, 101), (64, 32, 32), (100, 65, 33), (4100, 36, 144), (2000, 144, 36),
-          (96, 200, 300), (513, 576, 144), (300, 301, 40), (333, 40, 301), (1620, 192, 768), (5000, 162, 5), (150, 160, 64), (290, 96, 96)]
+          (96, 200, 300), (513, 576, 144), (300, 301, 40), (333, 40, 301), (1620, 192, 768), (5000, 162, 5), (150, 160, 64), (290, 96, 96), (1, 300, 1), (3, 200, 1), (2, 1, 300), (131, 300, 1),
+          (130, 300, 2), (129, 170, 3), (131, 2, 300), (258, 1, 161), (67, 3, 400), (1, 170, 170), (1000, 165, 163)]
 
 
 def layer(V, ci, co, integers, seed, cuda):
