@@ -71,10 +71,10 @@ struct Run {
     __device__ __forceinline__ v4f fix(v4f v, int off) const
     {
         const int d = off + delta - last;
-        if (d <= 0) return v;
-        if (d & 1) v = v4f{v[1], v[2], v[3], 0.0f};
-        if (d & 2) v = v4f{v[2], v[3], 0.0f, 0.0f};
-        return d < 4 ? v : v4f{};
+        const bool one = d > 0 && (d & 1), two = d > 0 && (d & 2), none = d >= 4;
+        v = v4f{one ? v[1] : v[0], one ? v[2] : v[1], one ? v[3] : v[2], v[3]};
+        v = v4f{two ? v[2] : v[0], two ? v[3] : v[1], v[2], v[3]};
+        return v4f{none ? 0.0f : v[0], none ? 0.0f : v[1], none ? 0.0f : v[2], none ? 0.0f : v[3]};
     }
     __device__ __forceinline__ unsigned fix(unsigned v, int off) const
     {

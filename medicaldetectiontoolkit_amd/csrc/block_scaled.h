@@ -110,6 +110,26 @@ __device__ __forceinline__ T read_back(float code, int b)
     return Io<T>::from_f(v);
 }
 
+// one lane's GV values of a 4-bit block held by 32 / GV lanes -> its GV / 2 bytes of codes (the conversion rounds to nearest even) and the block's scale byte
+template <int GV>
+__device__ __forceinline__ unsigned quantize4_group(const float (&v)[GV], int &b)
+{
+    unsigned mb = 0;
+#pragma unroll
+    for (int j = 0; j < GV; ++j) mb = umax(mb, __float_as_uint(v[j]) & 0x7fffffffu);
+    mb = group_max<BLOCK / GV>(mb);
+    b = scale_byte<Q6>(mb);
+    const float s = scale_of(b == 255 ? 127 : b);
+    unsigned w = 0;
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[0], v[1], s, 0);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[2], v[3], s, 1);
+    if (GV == 8) {
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[GV - 4], v[GV - 3], s, 2);
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[GV - 2], v[GV - 1], s, 3);
+    }
+    return b == 255 ? 0u : w;
+}
+
 inline int launch_check()
 {
     const hipError_t e = hipGetLastError();

@@ -193,20 +193,8 @@ __global__ __launch_bounds__(THREADS) void mx4_quantize_kernel(const T *__restri
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const unsigned g = g0 + u * THREADS;
-        unsigned mb = 0;
-#pragma unroll
-        for (int j = 0; j < GV; ++j) mb = umax(mb, __float_as_uint(v[u][j]) & 0x7fffffffu);
-        mb = group_max<LPB>(mb);
-        const int b = scale_byte<Q6>(mb);
-        const float s = scale_of(b == 255 ? 127 : b);
-        unsigned w = 0;
-        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[u][0], v[u][1], s, 0);
-        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[u][2], v[u][3], s, 1);
-        if (GV == 8) {
-            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[u][GV - 4], v[u][GV - 3], s, 2);
-            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[u][GV - 2], v[u][GV - 1], s, 3);
-        }
-        if (b == 255) w = 0;
+        int b;
+        const unsigned w = quantize4_group<GV>(v[u], b);
         if (g < total) {
             const long long at = row0 * groups.d + g;                      // groups of all rows are consecutive: GV / 2 bytes each
             if (GV == 8) reinterpret_cast<unsigned *>(codes)[at] = w;

@@ -1,111 +1,370 @@
 // mx4_linear.hip -- act(x W^T + bias) with both operands in 4-bit block-scaled codes (gfx950).
 //
-// The matrix units take 4-bit codes and one scale byte per 32 of them as they are (K = 64 of a 32 x 32 tile an instruction), products and sums in
-// fp32.  x is rounded to codes first (mx4_quantize_kernel), W is kept in codes.
+// The matrix units take 4-bit codes and one scale byte per 32 of them as they are (16 x 16 outputs, 128 summed values an instruction), products exact and sums
+// in fp32.  W is kept in codes; x is rounded to codes on its way into the product, in one launch and without scratch memory, so x is read once and nothing
+// else of its size is moved.
+//
+// Work goes in chunks of 256 summed values = 8 blocks.  A lane (r = lane % 16, q = lane / 16) holds blocks 2q and 2q + 1 of row r: 32 consecutive bytes of
+// codes and 2 of scales, of W straight from memory into registers, of x from LDS, where the lanes that loaded x put its codes (a row of a chunk is 64 lanes of
+// 4 floats, or 32 lanes of 8 values of 16 bits, so a block's maximum is a few lane permutes).  With W as the first operand a lane ends up with 4
+// consecutive outputs of one row.
+//
+// Two shapes of the same loop:
+//   narrow   every wave sums its own chunks (w, w + 8, ...) of a 16 x 16 TN tile, without any barrier, and the 8 waves' sums are joined in LDS at the end: few
+//            outputs a row, or few rows, where only the summed axis is long
+//   wide     the 8 waves share one 16 TM x 128 TN tile's x and take 16 TN columns each: many rows and many columns, where x must not be rounded again for
+//            each range of columns
 #include "block_scaled.h"
 
 namespace {
 
 using namespace mdt_bs;
 
-constexpr int WAVES = 4;
+constexpr int WAVES = 8;
 constexpr int THREADS = 64 * WAVES;
+constexpr int CHUNK = 256, CHUNK_BLOCKS = CHUNK / BLOCK;
+constexpr int ROW_BYTES = CHUNK / 2 + 16;                   // a row of codes in LDS, padded: 16-byte reads of neighbouring rows fall into different banks
 
-// a wave's 32 x 32 tile over the block range of its split; lane l: row / column l % 32, block kb + l / 32.  A block beyond the row's end multiplies
-// zero codes.
-__global__ __launch_bounds__(THREADS) void mx4_gemm_kernel(const uint8_t *__restrict__ xc, const uint8_t *__restrict__ xs, const uint8_t *__restrict__ wc, const uint8_t *__restrict__ ws,
-                                                           float *__restrict__ part, long long M, int N, long long kb, long long kb_per)
+
+// W's rows of one tile: a uniform base and the lane's 32-bit offsets, so that an address costs one addition.  Loads take no branches (the number of loads in
+// flight stays known, and a wait for one does not become a wait for all): columns behind the last one repeat it, blocks behind a row's end repeat its
+// last one (x's codes are zero there) and get a finite scale.
+struct Frag { v4u c[2]; unsigned s; };
+template <bool ONE>                                         // ONE: rows of a single block
+struct WRows {
+    const uint8_t *codes, *scales;
+    int mine, most, kb;                                      // in blocks: the lane's row within the tile, the last row
+    __device__ __forceinline__ WRows(const uint8_t *wc, const uint8_t *ws, int n0, int n, int blocks, int r) : kb(blocks)
+    {
+        const int from = min(n0, n - 1);
+        codes = wc + (long long)from * blocks * 16;
+        scales = ws + (long long)from * blocks;
+        mine = r * blocks;
+        most = min(n - 1 - from, 1023) * blocks;             // more than a tile's rows
+    }
+    // blocks b and b + 1 of row 16 t + r
+    __device__ __forceinline__ void load(Frag &f, int t, int b) const
+    {
+        typedef uint16_t u16una __attribute__((aligned(1)));
+        const int off = min(mine + t * 16 * kb, most);
+        f.c[0] = *reinterpret_cast<const v4u *>(codes + (unsigned)(off + min(b, kb - 1)) * 16u);
+        if (!ONE) f.c[1] = *reinterpret_cast<const v4u *>(codes + (unsigned)(off + min(b + 1, kb - 1)) * 16u);
+        if (ONE) f.s = scales[(unsigned)off];
+        else f.s = *reinterpret_cast<const u16una *>(scales + (unsigned)(off + min(b, kb - 2)));
+    }
+    // the loaded scales where the chunk reaches behind the row's end
+    __device__ __forceinline__ unsigned fix(unsigned s, int b) const { return b + 1 < kb ? s : b < kb ? (ONE ? s : s >> 8) | 127u << 8 : 127u | 127u << 8; }
+};
+
+__device__ __forceinline__ v8i operand(v4u c)
 {
-    const int l = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const long long m0 = ((long long)blockIdx.x * WAVES + wave) * 32;
-    if (m0 >= M) return;
-    const long long m = m0 + (l & 31);
-    const int n = blockIdx.y * 32 + (l & 31);
-    const long long b0 = (long long)blockIdx.z * kb_per, b1 = b0 + kb_per < kb ? b0 + kb_per : kb;
-    v16f acc = {};
-    for (long long b = b0; b < b1; b += 2) {
-        const long long at = b + (l >> 5);
-        v8i A = {}, B = {};
-        int sa = 127, sb = 127;
-        if (at < b1) {
-            if (m < M) {
-                *reinterpret_cast<v4u *>(&A) = *reinterpret_cast<const v4u *>(xc + (m * kb + at) * 16);
-                sa = xs[m * kb + at];
-            }
-            if (n < N) {
-                *reinterpret_cast<v4u *>(&B) = *reinterpret_cast<const v4u *>(wc + (n * kb + at) * 16);
-                sb = ws[n * kb + at];
-            }
-        }
-        acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(A, B, acc, 4, 4, 0, sa, 0, sb);
-    }
+    v8i v = {};
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        const long long row = m0 + 8 * (i / 4) + 4 * (l >> 5) + i % 4;
-        if (row < M && n < N) part[((long long)blockIdx.z * M + row) * N + n] = acc[i];
+    for (int j = 0; j < 4; ++j) v[j] = (int)c[j];
+    return v;
+}
+
+template <int STEP>
+__device__ __forceinline__ v4f mfma4(v4u w, unsigned ws, v4u x, unsigned xs, v4f acc)
+{
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand(w), operand(x), acc, 4, 4, STEP, (int)ws, STEP, (int)xs);
+}
+
+// x's rows of one wave: LPR lanes a row of a chunk, 64 / LPR rows a load.  Loads take no branches here either: GV values that would pass the array's end are
+// read from its last GV and moved to their places, values behind a row's end are set to zero, rows behind the last one hold anything.
+template <typename T, int LOADS, bool TINY>                  // TINY: the whole array may be shorter than one load
+struct XRows {
+    static constexpr int GV = Io<T>::GV, LPR = CHUNK / GV, PER = 64 / LPR;      // 64 lanes and 1 row, or 32 lanes and 2 rows
+    typedef typename Io<T>::vec vec;
+    const T *base;
+    long long k;
+    int off, step, last, at;                                                     // the lane's first value, PER rows, the array's last GV (tiny: its length), the place in the chunk
+    bool ragged, tiny;
+    __device__ __forceinline__ XRows(const T *x, long long row0, long long rows, long long kk, int l) : k(kk)
+    {
+        const long long total = rows * kk, first = row0 * kk;
+        tiny = TINY && total < GV;
+        const long long from = tiny ? 0 : first < total - GV ? first : total - GV;
+        base = x + from;
+        at = l % LPR * GV;
+        off = (int)(first - from) + l / LPR * (int)kk + at;
+        step = PER * (int)kk;
+        const long long rest = total - GV - from;
+        last = tiny ? (int)total : rest < (1 << 28) ? (int)rest : 1 << 28;                           // more than a tile's values (48 rows of 2^22)
+        ragged = row0 + LOADS * PER + GV >= rows;
     }
+    __device__ __forceinline__ vec load(int i, int k0) const
+    {
+        if (TINY && tiny) {
+            vec v;
+#pragma unroll
+            for (int j = 0; j < GV; ++j) v[j] = off + i * step + k0 + j < last ? base[off + i * step + k0 + j] : (T)0.0f;
+            return v;
+        }
+        return *reinterpret_cast<const vec *>(reinterpret_cast<const char *>(base) + (unsigned)min(off + i * step + k0, last) * (unsigned)sizeof(T));
+    }
+    __device__ __forceinline__ void values(float (&v)[GV], const vec &t, int i, int k0) const
+    {
+#pragma unroll
+        for (int j = 0; j < GV; ++j) v[j] = Io<T>::to_f(t[j]);
+        if (ragged && !(TINY && tiny)) {
+            const int d = off + i * step + k0 - last;
+#pragma unroll
+            for (int bit = 1; bit < GV; bit *= 2) {
+                const bool move = d > 0 && (d & bit);
+#pragma unroll
+                for (int j = 0; j < GV; ++j) v[j] = move ? (j + bit < GV ? v[j + bit] : 0.0f) : v[j];
+            }
+#pragma unroll
+            for (int j = 0; j < GV; ++j) v[j] = d < GV ? v[j] : 0.0f;
+        }
+        if (k0 + CHUNK > k) {
+#pragma unroll
+            for (int j = 0; j < GV; ++j) v[j] = k0 + at + j < k ? v[j] : 0.0f;
+        }
+    }
+    // codes and scales of load i into LDS rows `row` on
+    __device__ __forceinline__ void put(uint8_t *codes, uint8_t *scales, const vec &t, int i, int k0, int row, int l) const
+    {
+        float v[GV];
+        values(v, t, i, k0);
+        int b;
+        const unsigned w = quantize4_group<GV>(v, b);
+        const int r = row + l / LPR, c = l % LPR;
+        if (GV == 8) *reinterpret_cast<unsigned *>(codes + r * ROW_BYTES + c * 4) = w;
+        else *reinterpret_cast<uint16_t *>(codes + r * ROW_BYTES + c * 2) = (uint16_t)w;
+        if (c % (BLOCK / GV) == 0) scales[r * CHUNK_BLOCKS + c / (BLOCK / GV)] = (uint8_t)b;
+    }
+};
+
+__device__ __forceinline__ void wave_fence()
+{
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
 }
 
 template <typename T>
-__global__ __launch_bounds__(256) void mx4_finish_kernel(const float *__restrict__ part, const float *__restrict__ bias, T *__restrict__ y, long long mn, int N, int splits, int relu)
+__device__ __forceinline__ T finish(float v, float add, int relu)
 {
-    const long long e = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (e >= mn) return;
-    float t = 0.0f;
-    for (int k = 0; k < splits; ++k) t = t + part[k * mn + e];
-    if (bias != nullptr) t = t + bias[e % N];
-    if (relu) t = t < 0.0f ? 0.0f : t;
-    y[e] = Io<T>::from_f(t);
+    v = v + add;
+    if (relu) v = v < 0.0f ? 0.0f : v;
+    return Io<T>::from_f(v);
 }
 
-inline long long blocks_of(long long k) { return (k + BLOCK - 1) / BLOCK; }
-
-inline long long splits_of(long long rows, long long k, int n)
+template <typename T, int TN, bool ONE>
+__global__ __launch_bounds__(THREADS, 2) void narrow_kernel(const T *__restrict__ x, const uint8_t *__restrict__ wc, const uint8_t *__restrict__ ws, const float *__restrict__ bias,
+                                                            T *__restrict__ y, long long rows, long long k, int n, int n_tiles, int relu)
 {
-    const long long tiles = (rows + 127) / 128 * ((n + 31) / 32), kb = blocks_of(k);
-    long long s = 512 / tiles;
-    if (s < 1) s = 1;
-    if (s > (kb + 7) / 8) s = (kb + 7) / 8;
-    return s;
+    constexpr int LOADS = 16 / (64 / (CHUNK / Io<T>::GV)), LDS_X = 16 * (ROW_BYTES + CHUNK_BLOCKS), LDS_SUM = 16 * TN * 16 * 4;
+    typedef XRows<T, LOADS, ONE> R;
+    __shared__ __attribute__((aligned(16))) uint8_t smem[WAVES * (LDS_X > LDS_SUM ? LDS_X : LDS_SUM)];
+    const int l = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = l >> 4, r = l & 15;
+    const long long row0 = (long long)(blockIdx.x / n_tiles) * 16;
+    const int n0 = (int)(blockIdx.x % n_tiles) * 16 * TN, kb = (int)((k + BLOCK - 1) / BLOCK), chunks = (kb + CHUNK_BLOCKS - 1) / CHUNK_BLOCKS;
+    uint8_t *codes = smem + wave * LDS_X, *scales = codes + 16 * ROW_BYTES;
+    const R xr(x, row0, rows, k, l);
+    const WRows<ONE> wr(wc, ws, n0, n, kb, r);
+    v4f acc[TN];
+#pragma unroll
+    for (int t = 0; t < TN; ++t) acc[t] = v4f{};
+    typename R::vec X[LOADS];
+    Frag W[TN];
+    auto load_x = [&](int c) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) X[i] = xr.load(i, c * CHUNK);
+    };
+    if (wave < chunks) {
+        load_x(wave);
+#pragma unroll
+        for (int t = 0; t < TN; ++t) wr.load(W[t], t, wave * CHUNK_BLOCKS + 2 * q);
+    }
+    for (int c = wave; c < chunks; c += WAVES) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) xr.put(codes, scales, X[i], i, c * CHUNK, i * R::PER, l);
+        wave_fence();
+        const v4u x0 = *reinterpret_cast<const v4u *>(codes + r * ROW_BYTES + q * 32), x1 = *reinterpret_cast<const v4u *>(codes + r * ROW_BYTES + q * 32 + 16);
+        const unsigned xs = *reinterpret_cast<const uint16_t *>(scales + r * CHUNK_BLOCKS + q * 2);
+        const int b = c * CHUNK_BLOCKS + 2 * q;
+        const bool tail = (c + 1) * CHUNK_BLOCKS > kb;
+#pragma unroll
+        for (int t = 0; t < TN; ++t) {
+            const unsigned s = tail ? wr.fix(W[t].s, b) : W[t].s;
+            acc[t] = mfma4<0>(W[t].c[0], s, x0, xs, acc[t]);
+            if (!ONE) acc[t] = mfma4<1>(W[t].c[1], s, x1, xs, acc[t]);
+        }
+#pragma unroll
+        for (int t = 0; t < TN; ++t) asm volatile("" : "+v"(acc[t]) : : "memory");        // the products stay ahead of the loads into their operands
+        if (c + WAVES < chunks) {
+            load_x(c + WAVES);
+#pragma unroll
+            for (int t = 0; t < TN; ++t) wr.load(W[t], t, b + WAVES * CHUNK_BLOCKS);
+        }
+        wave_fence();
+    }
+    __syncthreads();
+    float *sum = reinterpret_cast<float *>(smem);
+#pragma unroll
+    for (int t = 0; t < TN; ++t) *reinterpret_cast<v4f *>(sum + ((wave * 16 + r) * TN + t) * 16 + q * 4) = acc[t];
+    __syncthreads();
+    for (int e = threadIdx.x; e < 16 * TN * 16; e += THREADS) {
+        const int col = n0 + e % (TN * 16);
+        const long long row = row0 + e / (TN * 16);
+        if (row >= rows || col >= n) continue;
+        float v = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) v = v + sum[w * 16 * TN * 16 + e];
+        y[row * n + col] = finish<T>(v, bias != nullptr ? bias[col] : 0.0f, relu);
+    }
 }
 
-inline size_t up256(size_t v) { return (v + 255) & ~(size_t)255; }
+template <typename T, int TM, int TN>
+__global__ __launch_bounds__(THREADS, 2) void wide_kernel(const T *__restrict__ x, const uint8_t *__restrict__ wc, const uint8_t *__restrict__ ws, const float *__restrict__ bias,
+                                                          T *__restrict__ y, long long rows, long long k, int n, int n_tiles, int relu)
+{
+    constexpr int BM = 16 * TM, MINE = BM / WAVES, LOADS = MINE / (64 / (CHUNK / Io<T>::GV));    // rows of x a wave rounds
+    typedef XRows<T, LOADS, false> R;
+    static_assert(LOADS * R::PER == MINE, "whole loads");
+    __shared__ __attribute__((aligned(16))) uint8_t s_codes[2][BM * ROW_BYTES], s_scales[2][BM * CHUNK_BLOCKS];
+    const int l = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = l >> 4, r = l & 15;
+    const long long row0 = (long long)(blockIdx.x / n_tiles) * BM;
+    const int n0 = ((int)(blockIdx.x % n_tiles) * WAVES + wave) * 16 * TN, kb = (int)((k + BLOCK - 1) / BLOCK), chunks = (kb + CHUNK_BLOCKS - 1) / CHUNK_BLOCKS;
+    const R xr(x, row0 + wave * MINE < rows ? row0 + wave * MINE : rows - 1, rows, k, l);
+    const WRows<false> wr(wc, ws, n0, n, kb, r);
+    v4f acc[TM][TN];
+#pragma unroll
+    for (int m = 0; m < TM; ++m)
+#pragma unroll
+        for (int t = 0; t < TN; ++t) acc[m][t] = v4f{};
+    typename R::vec X[LOADS];
+    Frag W[TN];
+    auto load_x = [&](int c) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) X[i] = xr.load(i, c * CHUNK);
+    };
+    auto put_x = [&](int c) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) xr.put(s_codes[c & 1], s_scales[c & 1], X[i], i, min(c, chunks - 1) * CHUNK, wave * MINE + i * R::PER, l);
+    };
+    load_x(0);
+#pragma unroll
+    for (int t = 0; t < TN; ++t) wr.load(W[t], t, 2 * q);
+    put_x(0);
+    load_x(min(1, chunks - 1));
+    __syncthreads();
+    for (int c = 0; c < chunks; ++c) {
+        const uint8_t *codes = s_codes[c & 1], *scales = s_scales[c & 1];
+        v4u x0[TM], x1[TM];
+        unsigned xs[TM];
+#pragma unroll
+        for (int m = 0; m < TM; ++m) {
+            x0[m] = *reinterpret_cast<const v4u *>(codes + (m * 16 + r) * ROW_BYTES + q * 32);
+            x1[m] = *reinterpret_cast<const v4u *>(codes + (m * 16 + r) * ROW_BYTES + q * 32 + 16);
+            xs[m] = *reinterpret_cast<const uint16_t *>(scales + (m * 16 + r) * CHUNK_BLOCKS + q * 2);
+        }
+        const int b = c * CHUNK_BLOCKS + 2 * q;
+        const bool tail = (c + 1) * CHUNK_BLOCKS > kb;
+#pragma unroll
+        for (int t = 0; t < TN; ++t) {
+            const unsigned s = tail ? wr.fix(W[t].s, b) : W[t].s;
+#pragma unroll
+            for (int m = 0; m < TM; ++m) acc[m][t] = mfma4<0>(W[t].c[0], s, x0[m], xs[m], acc[m][t]);
+#pragma unroll
+            for (int m = 0; m < TM; ++m) acc[m][t] = mfma4<1>(W[t].c[1], s, x1[m], xs[m], acc[m][t]);
+            // the products stay here and the next chunk's loads behind them, so that the loads can take the same registers
+#pragma unroll
+            for (int m = 0; m < TM; ++m) asm volatile("" : "+v"(acc[m][t]) : : "memory");
+            wr.load(W[t], t, b + CHUNK_BLOCKS);
+        }
+        // past the last chunk the last one is loaded and rounded again, into the buffer that nobody reads: no branch around a load
+        put_x(c + 1);
+        load_x(min(c + 2, chunks - 1));
+        __syncthreads();
+    }
+    float add[TN][4];
+#pragma unroll
+    for (int t = 0; t < TN; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) add[t][j] = bias != nullptr ? bias[min(n0 + t * 16 + q * 4 + j, n - 1)] : 0.0f;
+#pragma unroll
+    for (int m = 0; m < TM; ++m) {
+        const long long row = row0 + m * 16 + r;
+        if (row >= rows) continue;
+#pragma unroll
+        for (int t = 0; t < TN; ++t) {
+            typedef T out __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+            const int col = n0 + t * 16 + q * 4;
+            out v;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = finish<T>(acc[m][t][j], add[t][j], relu);
+            T *to = y + row * n + col;
+            if (col + 4 <= n) *reinterpret_cast<out *>(to) = v;
+            else
+#pragma unroll
+                for (int j = 0; j < 3; ++j) if (col + j < n) to[j] = v[j];
+        }
+    }
+}
+
+struct Call { const void *x; const uint8_t *wc, *ws; const float *bias; void *y; long long rows, k; int n, relu; hipStream_t s; };
+
+template <typename T, int TN>
+int narrow(const Call &a)
+{
+    const int tiles = (a.n + 16 * TN - 1) / (16 * TN);
+    const long long groups = (a.rows + 15) / 16 * tiles;
+    if (groups >= (1LL << 23)) return MDT_ERR_UNSUPPORTED;                         // 2^32 threads are the most of a launch
+    const auto kernel = a.k <= BLOCK ? narrow_kernel<T, TN, true> : narrow_kernel<T, TN, false>;
+    kernel<<<dim3((unsigned)groups), THREADS, 0, a.s>>>((const T *)a.x, a.wc, a.ws, a.bias, (T *)a.y, a.rows, a.k, a.n, tiles, a.relu);
+    return launch_check();
+}
+
+template <typename T, int TM, int TN>
+int wide(const Call &a)
+{
+    const int tiles = (a.n + 128 * TN - 1) / (128 * TN);
+    const long long groups = (a.rows + 16 * TM - 1) / (16 * TM) * tiles;
+    if (groups >= (1LL << 23)) return MDT_ERR_UNSUPPORTED;
+    wide_kernel<T, TM, TN><<<dim3((unsigned)groups), THREADS, 0, a.s>>>((const T *)a.x, a.wc, a.ws, a.bias, (T *)a.y, a.rows, a.k, a.n, tiles, a.relu);
+    return launch_check();
+}
+
+template <typename T>
+int run(const Call &a)
+{
+    constexpr int TM = 3;
+    if (a.n > 144 && a.rows >= 2048 && a.k > BLOCK) {
+        const int ranges = (a.n + 767) / 768, per = (a.n + 128 * ranges - 1) / (128 * ranges);
+        switch (per) {
+            case 1: case 2: return wide<T, TM, 2>(a);
+            case 3: return wide<T, TM, 3>(a);
+            case 4: return wide<T, TM, 4>(a);
+            case 5: return wide<T, TM, 5>(a);
+            default: return wide<T, TM, 6>(a);
+        }
+    }
+    // as few ranges of columns as still give every CU a workgroup: each range rounds x again
+    const long long row_tiles = (a.rows + 15) / 16;
+    if (row_tiles * ((a.n + 143) / 144) >= 128 && a.n > 48) return narrow<T, 9>(a);
+    if (row_tiles * ((a.n + 47) / 48) >= 128 && a.n > 16) return narrow<T, 3>(a);
+    return narrow<T, 1>(a);
+}
 
 }  // namespace
 
 extern "C" {
 
-size_t mdt_mx4_linear_workspace_bytes(long long rows, long long k, int n)
+int mdt_mx4_linear(const void *x, int dtype, const void *w_codes, const void *w_scales, const float *bias, void *y, long long rows, long long k, int n, int relu, void *stream)
 {
-    if (rows < 1 || k < 1 || n < 1) return 256;
-    const long long kb = blocks_of(k);
-    return up256((size_t)(rows * kb * 16)) + up256((size_t)(rows * kb)) + (size_t)(splits_of(rows, k, n) * rows * n) * 4 + 256;
-}
-
-int mdt_mx4_linear(const void *x, int dtype, const void *w_codes, const void *w_scales, const float *bias, void *y, long long rows, long long k, int n, int relu, void *workspace,
-                   size_t workspace_bytes, void *stream)
-{
-    if (rows < 0 || k < 1 || n < 1 || n > (1 << 20) || k > (1LL << 30) || rows > (1LL << 30) || rows > (1LL << 36) / k || rows > (1LL << 31) / n || (rows > 0 && (!x || !w_codes || !w_scales || !y))) return MDT_ERR_INVALID_ARGUMENT;
+    if (rows < 0 || k < 1 || n < 1 || n > (1 << 20) || k > (1 << 22) || rows > (1LL << 30) || (rows > 0 && (!x || !w_codes || !w_scales || !y))) return MDT_ERR_INVALID_ARGUMENT;
     if (dtype != MDT_DTYPE_F32 && dtype != MDT_DTYPE_BF16 && dtype != MDT_DTYPE_F16) return MDT_ERR_INVALID_ARGUMENT;
     if (((uintptr_t)w_codes & 15) != 0) return MDT_ERR_INVALID_ARGUMENT;
     if (rows == 0) return MDT_OK;
-    if (workspace == nullptr || workspace_bytes < mdt_mx4_linear_workspace_bytes(rows, k, n)) return MDT_ERR_WORKSPACE_TOO_SMALL;
-    const hipStream_t s = (hipStream_t)stream;
-    const long long kb = blocks_of(k), splits = splits_of(rows, k, n), per = (kb + splits - 1) / splits;
-    uint8_t *xc = (uint8_t *)workspace, *xs = xc + up256((size_t)(rows * kb * 16));
-    float *part = (float *)(xs + up256((size_t)(rows * kb)));
-    const int rc = mdt_mx4_quantize(x, xc, xs, rows, k, dtype, stream);
-    if (rc != MDT_OK) return rc;
-    const dim3 grid((unsigned)((rows + 32 * WAVES - 1) / (32 * WAVES)), (unsigned)((n + 31) / 32), (unsigned)splits);
-    mx4_gemm_kernel<<<grid, THREADS, 0, s>>>(xc, xs, (const uint8_t *)w_codes, (const uint8_t *)w_scales, part, rows, n, kb, per);
-    const long long mn = rows * n;
-    const dim3 fg((unsigned)((mn + 255) / 256));
+    const Call a = {x, (const uint8_t *)w_codes, (const uint8_t *)w_scales, bias, y, rows, k, n, relu, (hipStream_t)stream};
     switch (dtype) {
-        case MDT_DTYPE_F32: mx4_finish_kernel<float><<<fg, 256, 0, s>>>(part, bias, (float *)y, mn, n, (int)splits, relu); break;
-        case MDT_DTYPE_BF16: mx4_finish_kernel<__bf16><<<fg, 256, 0, s>>>(part, bias, (__bf16 *)y, mn, n, (int)splits, relu); break;
-        default: mx4_finish_kernel<_Float16><<<fg, 256, 0, s>>>(part, bias, (_Float16 *)y, mn, n, (int)splits, relu); break;
+        case MDT_DTYPE_F32: return run<float>(a);
+        case MDT_DTYPE_BF16: return run<__bf16>(a);
+        default: return run<_Float16>(a);
     }
-    return launch_check();
 }
 
 }  // extern "C"

@@ -352,7 +352,8 @@ def test_mx4_keeps_leading_axes_and_takes_any_strides(cuda):
     assert bs.mx4_quantize(x[:0]).dequantize().shape == (0, 4, 70)
 
 
-LINEAR = [(1, 1, 1), (1, 5292, 144), (3, 33, 5), (31, 64, 32), (33, 100, 33), (130, 5292, 144), (257, 31, 7), (64, 2048, 768), (1000, 144, 144), (515, 1000, 300), (129, 9408, 65)]
+LINEAR = [(1, 1, 1), (1, 5292, 144), (3, 33, 5), (31, 64, 32), (33, 100, 33), (130, 5292, 144), (257, 31, 7), (64, 2048, 768), (1000, 144, 144), (515, 1000, 300), (129, 9408, 65), (2100, 300, 200), (2049, 33, 150),
+          (2305, 517, 801), (2048, 256, 400), (2600, 65, 513), (2200, 1, 145), (2, 3, 200), (1, 7, 2), (4000, 40, 3)]
 
 
 @pytest.mark.parametrize("relu", [False, True])
