@@ -740,8 +740,9 @@ int mdt_mx4_dequantize(const void *codes, const void *scales, void *x, long long
  * y[r][j] = act(sum_i x4[r][i] * w4[j][i] + bias[j]): x4 = x rounded to 4-bit codes in the call, w4 the codes of w [n][k] (16-byte aligned); products and
  * sums in fp32, one rounding to x's type at the end.  bias: fp32 [n] or NULL.  The box heads' products at inference.
  */
+size_t mdt_mx4_linear_workspace_bytes(long long rows, long long k, int n);       /* 0: none is needed */
 int mdt_mx4_linear(const void *x, int dtype, const void *w_codes, const void *w_scales, const float *bias /* or NULL */, void *y,
-                   long long rows, long long k, int n, int relu, void *stream);
+                   long long rows, long long k, int n, int relu, void *workspace, size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

@@ -109,7 +109,8 @@ _SIGNATURES = {
     "mdt_conv1x1_act8_backward": (c_int, [c_void_p] * 4 + [c_int] + [c_void_p] * 5 + [c_longlong, c_int, c_int, c_void_p, c_size_t, c_void_p]),
     "mdt_mx4_quantize": (c_int, [c_void_p, c_void_p, c_void_p, c_longlong, c_longlong, c_int, c_void_p]),
     "mdt_mx4_dequantize": (c_int, [c_void_p, c_void_p, c_void_p, c_longlong, c_longlong, c_int, c_void_p]),
-    "mdt_mx4_linear": (c_int, [c_void_p, c_int] + [c_void_p] * 4 + [c_longlong, c_longlong, c_int, c_int, c_void_p]),
+    "mdt_mx4_linear_workspace_bytes": (c_size_t, [c_longlong, c_longlong, c_int]),
+    "mdt_mx4_linear": (c_int, [c_void_p, c_int] + [c_void_p] * 4 + [c_longlong, c_longlong, c_int, c_int, c_void_p, c_size_t, c_void_p]),
     "mdt_roi_levels": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p]),
     "mdt_rpn_sample_supported": (c_int, [c_int, c_int, c_int]),
     "mdt_rpn_sample_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),

@@ -4,10 +4,12 @@
 // in fp32.  W is kept in codes; x is rounded to codes on its way into the product, in one launch and without scratch memory, so x is read once and nothing
 // else of its size is moved.
 //
-// Work goes in chunks of 256 summed values = 8 blocks.  A lane (r = lane % 16, q = lane / 16) holds blocks 2q and 2q + 1 of row r: 32 consecutive bytes of
-// codes and 2 of scales, of W straight from memory into registers, of x from LDS, where the lanes that loaded x put its codes (a row of a chunk is 64 lanes of
-// 4 floats, or 32 lanes of 8 values of 16 bits, so a block's maximum is a few lane permutes).  With W as the first operand a lane ends up with 4
-// consecutive outputs of one row.
+// Work goes in chunks of 256 summed values = 8 blocks.  A lane (r = lane % 16, q = lane / 16) holds blocks 2q and 2q + 1 of row r: 32 bytes of codes and 2 of
+// scales.  x's come from LDS, where the lanes that loaded x put its codes (a row of a chunk is 64 lanes of 4 floats, or 32 lanes of 8 values of 16 bits, so a
+// block's maximum is a few lane permutes).  W's come straight from memory into registers: for few rows of x from W as it is kept, where the 64 lanes of a
+// load touch 16 rows and cost 64 requests; for more rows from a copy in the lanes' order, one contiguous kilobyte a load, that a first launch makes in the
+// workspace (the 2D head, 10000 x 9408 -> 768: 151 us without the copy, TIME us with it).  With W as the first operand a lane ends up with 4 consecutive
+// outputs of one row.
 //
 // Two shapes of the same loop:
 //   narrow   every wave sums its own chunks (w, w + 8, ...) of a 16 x 16 TN tile, without any barrier, and the 8 waves' sums are joined in LDS at the end: few
@@ -23,38 +25,95 @@ using namespace mdt_bs;
 constexpr int WAVES = 8;
 constexpr int THREADS = 64 * WAVES;
 constexpr int CHUNK = 256, CHUNK_BLOCKS = CHUNK / BLOCK;
+constexpr long long COPY_ROWS = 256;                       // from so many rows on W is copied into the lanes' order
 constexpr int ROW_BYTES = CHUNK / 2 + 16;                   // a row of codes in LDS, padded: 16-byte reads of neighbouring rows fall into different banks
 
 
-// W's rows of one tile: a uniform base and the lane's 32-bit offsets, so that an address costs one addition.  Loads take no branches (the number of loads in
-// flight stays known, and a wait for one does not become a wait for all): columns behind the last one repeat it, blocks behind a row's end repeat its
-// last one (x's codes are zero there) and get a finite scale.
+// a number that the optimiser takes for a new one: it would hold every address that it computes from a lane's number in a register of its own over the loop
+__device__ __forceinline__ int fresh(int v)
+{
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
+// one lane's fragment of 16 rows of W for a chunk: blocks 2q and 2q + 1 of its row
 struct Frag { v4u c[2]; unsigned s; };
+
+// W as it is kept.  Loads take no branches (the number of loads in flight stays known, and a wait for one does not become a wait for all): rows behind the last one
+// repeat it, blocks behind a row's end repeat its last one (x's codes are zero there) and get a finite scale.
 template <bool ONE>                                         // ONE: rows of a single block
-struct WRows {
+struct WKept {
     const uint8_t *codes, *scales;
-    int mine, most, kb;                                      // in blocks: the lane's row within the tile, the last row
-    __device__ __forceinline__ WRows(const uint8_t *wc, const uint8_t *ws, int n0, int n, int blocks, int r) : kb(blocks)
+    int mine, most, kb, q;                                   // in blocks: the lane's row within the tile, the last row
+    __device__ __forceinline__ WKept(const uint8_t *wc, const uint8_t *ws, int n0, int n, int blocks, int l) : kb(blocks), q(l >> 4)
     {
         const int from = min(n0, n - 1);
         codes = wc + (long long)from * blocks * 16;
         scales = ws + (long long)from * blocks;
-        mine = r * blocks;
+        mine = l % 16 * blocks;
         most = min(n - 1 - from, 1023) * blocks;             // more than a tile's rows
     }
-    // blocks b and b + 1 of row 16 t + r
-    __device__ __forceinline__ void load(Frag &f, int t, int b) const
+    __device__ __forceinline__ void load(Frag &f, int t, int c) const
     {
         typedef uint16_t u16una __attribute__((aligned(1)));
-        const int off = min(mine + t * 16 * kb, most);
+        const int off = min(fresh(mine) + t * 16 * kb, most), b = c * CHUNK_BLOCKS + 2 * q;
         f.c[0] = *reinterpret_cast<const v4u *>(codes + (unsigned)(off + min(b, kb - 1)) * 16u);
         if (!ONE) f.c[1] = *reinterpret_cast<const v4u *>(codes + (unsigned)(off + min(b + 1, kb - 1)) * 16u);
+        if (ONE) f.c[1] = v4u{};
         if (ONE) f.s = scales[(unsigned)off];
         else f.s = *reinterpret_cast<const u16una *>(scales + (unsigned)(off + min(b, kb - 2)));
     }
-    // the loaded scales where the chunk reaches behind the row's end
-    __device__ __forceinline__ unsigned fix(unsigned s, int b) const { return b + 1 < kb ? s : b < kb ? (ONE ? s : s >> 8) | 127u << 8 : 127u | 127u << 8; }
+    __device__ __forceinline__ unsigned scale(const Frag &f, int c) const
+    {
+        const int b = c * CHUNK_BLOCKS + 2 * q;
+        if ((c + 1) * CHUNK_BLOCKS <= kb) return f.s;
+        return b + 1 < kb ? f.s : b < kb ? (ONE ? f.s : f.s >> 8) | 127u << 8 : 127u | 127u << 8;
+    }
 };
+
+// the copy in the lanes' order: codes [tiles of 16 rows][chunks][2][64 lanes][16 bytes], scales [tiles][chunks][64 lanes][2]; zero codes and finite scales behind W's
+// rows and behind a row's end
+struct WTiled {
+    const uint8_t *codes, *scales;
+    int chunks;
+    unsigned l;
+    __device__ __forceinline__ WTiled(const uint8_t *tc, const uint8_t *ts, int n0, int n, int blocks, int lane) : chunks((blocks + CHUNK_BLOCKS - 1) / CHUNK_BLOCKS), l(lane)
+    {
+        const int tiles = (n + 15) / 16;
+        first = min(n0 / 16, tiles - 1);
+        most = tiles - 1 - first;
+        codes = tc;
+        scales = ts;
+    }
+    int first, most;                                         // tiles behind the last one repeat it
+    __device__ __forceinline__ void load(Frag &f, int t, int c) const
+    {
+        const long long at = (long long)(first + min(t, most)) * chunks + c;
+        const uint8_t *pc = codes + at * 2048, *ps = scales + at * 128;
+        f.c[0] = *reinterpret_cast<const v4u *>(pc + l * 16u);
+        f.c[1] = *reinterpret_cast<const v4u *>(pc + l * 16u + 1024);
+        f.s = *reinterpret_cast<const uint16_t *>(ps + l * 2u);
+    }
+    __device__ __forceinline__ unsigned scale(const Frag &f, int) const { return f.s; }
+};
+
+// a workgroup of 64 lanes x 4: one 16-row tile of 4 chunks
+__global__ __launch_bounds__(256) void tile_weights_kernel(const uint8_t *__restrict__ wc, const uint8_t *__restrict__ ws, uint8_t *__restrict__ tc, uint8_t *__restrict__ ts, int n, int kb,
+                                                           int chunks)
+{
+    const int c = blockIdx.x * 4 + (threadIdx.x >> 6), l = threadIdx.x & 63, tile = blockIdx.y;
+    if (c >= chunks) return;
+    // read 8 lanes a row (128 consecutive bytes), write where the fragment order wants the 16 bytes
+    const long long to = (long long)tile * chunks + c;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int r = h * 8 + l / 8, p = l % 8, row = tile * 16 + r, b = c * CHUNK_BLOCKS + p;
+        const bool in = row < n && b < kb;
+        const v4u v = in ? *reinterpret_cast<const v4u *>(wc + ((long long)row * kb + b) * 16) : v4u{};
+        *reinterpret_cast<v4u *>(tc + to * 2048 + p % 2 * 1024 + (p / 2 * 16 + r) * 16) = v;
+        ts[to * 128 + (p / 2 * 16 + r) * 2 + p % 2] = in ? ws[(long long)row * kb + b] : 127;
+    }
+}
 
 __device__ __forceinline__ v8i operand(v4u c)
 {
@@ -101,14 +160,14 @@ struct XRows {
             for (int j = 0; j < GV; ++j) v[j] = off + i * step + k0 + j < last ? base[off + i * step + k0 + j] : (T)0.0f;
             return v;
         }
-        return *reinterpret_cast<const vec *>(reinterpret_cast<const char *>(base) + (unsigned)min(off + i * step + k0, last) * (unsigned)sizeof(T));
+        return *reinterpret_cast<const vec *>(reinterpret_cast<const char *>(base) + (unsigned)min(fresh(off) + i * step + k0, last) * (unsigned)sizeof(T));
     }
     __device__ __forceinline__ void values(float (&v)[GV], const vec &t, int i, int k0) const
     {
 #pragma unroll
         for (int j = 0; j < GV; ++j) v[j] = Io<T>::to_f(t[j]);
         if (ragged && !(TINY && tiny)) {
-            const int d = off + i * step + k0 - last;
+            const int d = fresh(off) + i * step + k0 - last;
 #pragma unroll
             for (int bit = 1; bit < GV; bit *= 2) {
                 const bool move = d > 0 && (d & bit);
@@ -151,54 +210,46 @@ __device__ __forceinline__ T finish(float v, float add, int relu)
     return Io<T>::from_f(v);
 }
 
-template <typename T, int TN, bool ONE>
+template <typename T, int TN, class W, bool TINY>
 __global__ __launch_bounds__(THREADS, 2) void narrow_kernel(const T *__restrict__ x, const uint8_t *__restrict__ wc, const uint8_t *__restrict__ ws, const float *__restrict__ bias,
                                                             T *__restrict__ y, long long rows, long long k, int n, int n_tiles, int relu)
 {
     constexpr int LOADS = 16 / (64 / (CHUNK / Io<T>::GV)), LDS_X = 16 * (ROW_BYTES + CHUNK_BLOCKS), LDS_SUM = 16 * TN * 16 * 4;
-    typedef XRows<T, LOADS, ONE> R;
+    typedef XRows<T, LOADS, TINY> R;
     __shared__ __attribute__((aligned(16))) uint8_t smem[WAVES * (LDS_X > LDS_SUM ? LDS_X : LDS_SUM)];
     const int l = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = l >> 4, r = l & 15;
     const long long row0 = (long long)(blockIdx.x / n_tiles) * 16;
     const int n0 = (int)(blockIdx.x % n_tiles) * 16 * TN, kb = (int)((k + BLOCK - 1) / BLOCK), chunks = (kb + CHUNK_BLOCKS - 1) / CHUNK_BLOCKS;
     uint8_t *codes = smem + wave * LDS_X, *scales = codes + 16 * ROW_BYTES;
     const R xr(x, row0, rows, k, l);
-    const WRows<ONE> wr(wc, ws, n0, n, kb, r);
+    const W wr(wc, ws, n0, n, kb, l);
     v4f acc[TN];
 #pragma unroll
     for (int t = 0; t < TN; ++t) acc[t] = v4f{};
     typename R::vec X[LOADS];
-    Frag W[TN];
-    auto load_x = [&](int c) {
+    Frag F[TN];
+    auto load = [&](int c) {
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) X[i] = xr.load(i, c * CHUNK);
-    };
-    if (wave < chunks) {
-        load_x(wave);
 #pragma unroll
-        for (int t = 0; t < TN; ++t) wr.load(W[t], t, wave * CHUNK_BLOCKS + 2 * q);
-    }
+        for (int t = 0; t < TN; ++t) wr.load(F[t], t, c);
+    };
+    if (wave < chunks) load(wave);
     for (int c = wave; c < chunks; c += WAVES) {
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) xr.put(codes, scales, X[i], i, c * CHUNK, i * R::PER, l);
         wave_fence();
         const v4u x0 = *reinterpret_cast<const v4u *>(codes + r * ROW_BYTES + q * 32), x1 = *reinterpret_cast<const v4u *>(codes + r * ROW_BYTES + q * 32 + 16);
         const unsigned xs = *reinterpret_cast<const uint16_t *>(scales + r * CHUNK_BLOCKS + q * 2);
-        const int b = c * CHUNK_BLOCKS + 2 * q;
-        const bool tail = (c + 1) * CHUNK_BLOCKS > kb;
 #pragma unroll
         for (int t = 0; t < TN; ++t) {
-            const unsigned s = tail ? wr.fix(W[t].s, b) : W[t].s;
-            acc[t] = mfma4<0>(W[t].c[0], s, x0, xs, acc[t]);
-            if (!ONE) acc[t] = mfma4<1>(W[t].c[1], s, x1, xs, acc[t]);
+            const unsigned s = wr.scale(F[t], c);
+            acc[t] = mfma4<0>(F[t].c[0], s, x0, xs, acc[t]);
+            acc[t] = mfma4<1>(F[t].c[1], s, x1, xs, acc[t]);
         }
 #pragma unroll
         for (int t = 0; t < TN; ++t) asm volatile("" : "+v"(acc[t]) : : "memory");        // the products stay ahead of the loads into their operands
-        if (c + WAVES < chunks) {
-            load_x(c + WAVES);
-#pragma unroll
-            for (int t = 0; t < TN; ++t) wr.load(W[t], t, b + WAVES * CHUNK_BLOCKS);
-        }
+        if (c + WAVES < chunks) load(c + WAVES);
         wave_fence();
     }
     __syncthreads();
@@ -221,7 +272,7 @@ template <typename T, int TM, int TN>
 __global__ __launch_bounds__(THREADS, 2) void wide_kernel(const T *__restrict__ x, const uint8_t *__restrict__ wc, const uint8_t *__restrict__ ws, const float *__restrict__ bias,
                                                           T *__restrict__ y, long long rows, long long k, int n, int n_tiles, int relu)
 {
-    constexpr int BM = 16 * TM, MINE = BM / WAVES, LOADS = MINE / (64 / (CHUNK / Io<T>::GV));    // rows of x a wave rounds
+    constexpr int BM = 16 * TM, MINE = BM / WAVES, LOADS = MINE / (64 / (CHUNK / Io<T>::GV));    // MINE: rows of x a wave rounds
     typedef XRows<T, LOADS, false> R;
     static_assert(LOADS * R::PER == MINE, "whole loads");
     __shared__ __attribute__((aligned(16))) uint8_t s_codes[2][BM * ROW_BYTES], s_scales[2][BM * CHUNK_BLOCKS];
@@ -229,17 +280,18 @@ __global__ __launch_bounds__(THREADS, 2) void wide_kernel(const T *__restrict__ 
     const long long row0 = (long long)(blockIdx.x / n_tiles) * BM;
     const int n0 = ((int)(blockIdx.x % n_tiles) * WAVES + wave) * 16 * TN, kb = (int)((k + BLOCK - 1) / BLOCK), chunks = (kb + CHUNK_BLOCKS - 1) / CHUNK_BLOCKS;
     const R xr(x, row0 + wave * MINE < rows ? row0 + wave * MINE : rows - 1, rows, k, l);
-    const WRows<false> wr(wc, ws, n0, n, kb, r);
+    const WTiled wr(wc, ws, n0, n, kb, l);
     v4f acc[TM][TN];
 #pragma unroll
     for (int m = 0; m < TM; ++m)
 #pragma unroll
         for (int t = 0; t < TN; ++t) acc[m][t] = v4f{};
     typename R::vec X[LOADS];
-    Frag W[TN];
+    Frag F[TN];
+    // past the last chunk the last one is loaded and rounded again, into a buffer that nobody reads: no branch around a load
     auto load_x = [&](int c) {
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i) X[i] = xr.load(i, c * CHUNK);
+        for (int i = 0; i < LOADS; ++i) X[i] = xr.load(i, min(c, chunks - 1) * CHUNK);
     };
     auto put_x = [&](int c) {
 #pragma unroll
@@ -247,9 +299,9 @@ __global__ __launch_bounds__(THREADS, 2) void wide_kernel(const T *__restrict__ 
     };
     load_x(0);
 #pragma unroll
-    for (int t = 0; t < TN; ++t) wr.load(W[t], t, 2 * q);
+    for (int t = 0; t < TN; ++t) wr.load(F[t], t, 0);
     put_x(0);
-    load_x(min(1, chunks - 1));
+    load_x(1);
     __syncthreads();
     for (int c = 0; c < chunks; ++c) {
         const uint8_t *codes = s_codes[c & 1], *scales = s_scales[c & 1];
@@ -261,23 +313,19 @@ __global__ __launch_bounds__(THREADS, 2) void wide_kernel(const T *__restrict__ 
             x1[m] = *reinterpret_cast<const v4u *>(codes + (m * 16 + r) * ROW_BYTES + q * 32 + 16);
             xs[m] = *reinterpret_cast<const uint16_t *>(scales + (m * 16 + r) * CHUNK_BLOCKS + q * 2);
         }
-        const int b = c * CHUNK_BLOCKS + 2 * q;
-        const bool tail = (c + 1) * CHUNK_BLOCKS > kb;
 #pragma unroll
         for (int t = 0; t < TN; ++t) {
-            const unsigned s = tail ? wr.fix(W[t].s, b) : W[t].s;
 #pragma unroll
-            for (int m = 0; m < TM; ++m) acc[m][t] = mfma4<0>(W[t].c[0], s, x0[m], xs[m], acc[m][t]);
+            for (int m = 0; m < TM; ++m) acc[m][t] = mfma4<0>(F[t].c[0], F[t].s, x0[m], xs[m], acc[m][t]);
 #pragma unroll
-            for (int m = 0; m < TM; ++m) acc[m][t] = mfma4<1>(W[t].c[1], s, x1[m], xs[m], acc[m][t]);
+            for (int m = 0; m < TM; ++m) acc[m][t] = mfma4<1>(F[t].c[1], F[t].s, x1[m], xs[m], acc[m][t]);
             // the products stay here and the next chunk's loads behind them, so that the loads can take the same registers
 #pragma unroll
             for (int m = 0; m < TM; ++m) asm volatile("" : "+v"(acc[m][t]) : : "memory");
-            wr.load(W[t], t, b + CHUNK_BLOCKS);
+            wr.load(F[t], t, min(c + 1, chunks - 1));
         }
-        // past the last chunk the last one is loaded and rounded again, into the buffer that nobody reads: no branch around a load
         put_x(c + 1);
-        load_x(min(c + 2, chunks - 1));
+        load_x(c + 2);
         __syncthreads();
     }
     float add[TN][4];
@@ -307,14 +355,13 @@ __global__ __launch_bounds__(THREADS, 2) void wide_kernel(const T *__restrict__ 
 
 struct Call { const void *x; const uint8_t *wc, *ws; const float *bias; void *y; long long rows, k; int n, relu; hipStream_t s; };
 
-template <typename T, int TN>
+template <typename T, int TN, class W, bool TINY>
 int narrow(const Call &a)
 {
     const int tiles = (a.n + 16 * TN - 1) / (16 * TN);
     const long long groups = (a.rows + 15) / 16 * tiles;
     if (groups >= (1LL << 23)) return MDT_ERR_UNSUPPORTED;                         // 2^32 threads are the most of a launch
-    const auto kernel = a.k <= BLOCK ? narrow_kernel<T, TN, true> : narrow_kernel<T, TN, false>;
-    kernel<<<dim3((unsigned)groups), THREADS, 0, a.s>>>((const T *)a.x, a.wc, a.ws, a.bias, (T *)a.y, a.rows, a.k, a.n, tiles, a.relu);
+    narrow_kernel<T, TN, W, TINY><<<dim3((unsigned)groups), THREADS, 0, a.s>>>((const T *)a.x, a.wc, a.ws, a.bias, (T *)a.y, a.rows, a.k, a.n, tiles, a.relu);
     return launch_check();
 }
 
@@ -328,42 +375,72 @@ int wide(const Call &a)
     return launch_check();
 }
 
-template <typename T>
-int run(const Call &a)
+struct Tiled { int chunks, tiles; size_t codes, bytes; };
+inline Tiled tiled_of(long long k, int n)
 {
-    constexpr int TM = 3;
-    if (a.n > 144 && a.rows >= 2048 && a.k > BLOCK) {
-        const int ranges = (a.n + 767) / 768, per = (a.n + 128 * ranges - 1) / (128 * ranges);
-        switch (per) {
-            case 1: case 2: return wide<T, TM, 2>(a);
-            case 3: return wide<T, TM, 3>(a);
-            case 4: return wide<T, TM, 4>(a);
-            case 5: return wide<T, TM, 5>(a);
-            default: return wide<T, TM, 6>(a);
+    Tiled t;
+    t.chunks = (int)((k + CHUNK - 1) / CHUNK);
+    t.tiles = (n + 15) / 16;
+    t.codes = (size_t)t.chunks * t.tiles * 2048;
+    t.bytes = t.codes + (size_t)t.chunks * t.tiles * 128;
+    return t;
+}
+inline bool copies_w(long long rows) { return rows >= COPY_ROWS; }
+
+template <typename T>
+int run(Call a, uint8_t *workspace)
+{
+    if (copies_w(a.rows)) {
+        const Tiled t = tiled_of(a.k, a.n);
+        tile_weights_kernel<<<dim3((t.chunks + 3) / 4, t.tiles), 256, 0, a.s>>>(a.wc, a.ws, workspace, workspace + t.codes, a.n, (int)((a.k + BLOCK - 1) / BLOCK), t.chunks);
+        a.wc = workspace;
+        a.ws = workspace + t.codes;
+        constexpr int TM = 3;
+        if (a.n > 144 && a.rows >= 2048) {
+            const int ranges = (a.n + 767) / 768, per = (a.n + 128 * ranges - 1) / (128 * ranges);
+            switch (per) {
+                case 1: case 2: return wide<T, TM, 2>(a);
+                case 3: return wide<T, TM, 3>(a);
+                case 4: return wide<T, TM, 4>(a);
+                case 5: return wide<T, TM, 5>(a);
+                default: return wide<T, TM, 6>(a);
+            }
         }
+        if (a.n > 48) return narrow<T, 9, WTiled, false>(a);
+        return a.n > 16 ? narrow<T, 3, WTiled, false>(a) : narrow<T, 1, WTiled, false>(a);
     }
-    // as few ranges of columns as still give every CU a workgroup: each range rounds x again
+    // as few ranges of columns as still give half of the CUs a workgroup: each range rounds x again
     const long long row_tiles = (a.rows + 15) / 16;
-    if (row_tiles * ((a.n + 143) / 144) >= 128 && a.n > 48) return narrow<T, 9>(a);
-    if (row_tiles * ((a.n + 47) / 48) >= 128 && a.n > 16) return narrow<T, 3>(a);
-    return narrow<T, 1>(a);
+    if (a.rows * a.k < Io<T>::GV) return narrow<T, 1, WKept<true>, true>(a);
+    const bool three = row_tiles * ((a.n + 47) / 48) >= 128 && a.n > 16;
+    if (a.k <= BLOCK) return three ? narrow<T, 3, WKept<true>, false>(a) : narrow<T, 1, WKept<true>, false>(a);
+    return three ? narrow<T, 3, WKept<false>, false>(a) : narrow<T, 1, WKept<false>, false>(a);
 }
 
 }  // namespace
 
 extern "C" {
 
-int mdt_mx4_linear(const void *x, int dtype, const void *w_codes, const void *w_scales, const float *bias, void *y, long long rows, long long k, int n, int relu, void *stream)
+size_t mdt_mx4_linear_workspace_bytes(long long rows, long long k, int n)
+{
+    if (rows < 1 || k < 1 || n < 1 || k > (1 << 22) || n > (1 << 20)) return 0;
+    return copies_w(rows) ? tiled_of(k, n).bytes : 0;
+}
+
+int mdt_mx4_linear(const void *x, int dtype, const void *w_codes, const void *w_scales, const float *bias, void *y, long long rows, long long k, int n, int relu, void *workspace,
+                   size_t workspace_bytes, void *stream)
 {
     if (rows < 0 || k < 1 || n < 1 || n > (1 << 20) || k > (1 << 22) || rows > (1LL << 30) || (rows > 0 && (!x || !w_codes || !w_scales || !y))) return MDT_ERR_INVALID_ARGUMENT;
     if (dtype != MDT_DTYPE_F32 && dtype != MDT_DTYPE_BF16 && dtype != MDT_DTYPE_F16) return MDT_ERR_INVALID_ARGUMENT;
-    if (((uintptr_t)w_codes & 15) != 0) return MDT_ERR_INVALID_ARGUMENT;
+    if (((uintptr_t)w_codes & 15) != 0 || ((uintptr_t)workspace & 15) != 0) return MDT_ERR_INVALID_ARGUMENT;
     if (rows == 0) return MDT_OK;
+    const size_t need = mdt_mx4_linear_workspace_bytes(rows, k, n);
+    if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return MDT_ERR_WORKSPACE_TOO_SMALL;
     const Call a = {x, (const uint8_t *)w_codes, (const uint8_t *)w_scales, bias, y, rows, k, n, relu, (hipStream_t)stream};
     switch (dtype) {
-        case MDT_DTYPE_F32: return run<float>(a);
-        case MDT_DTYPE_BF16: return run<__bf16>(a);
-        default: return run<_Float16>(a);
+        case MDT_DTYPE_F32: return run<float>(a, (uint8_t *)workspace);
+        case MDT_DTYPE_BF16: return run<__bf16>(a, (uint8_t *)workspace);
+        default: return run<_Float16>(a, (uint8_t *)workspace);
     }
 }
 

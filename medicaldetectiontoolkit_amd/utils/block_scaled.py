@@ -267,5 +267,7 @@ def mx4_linear(x, w4, bias=None, relu=False):
     y = torch.empty(x.shape[:-1] + (n,), dtype=x.dtype, device=x.device)
     if y.numel() == 0:
         return y
-    _call(x.device, "mdt_mx4_linear", x.data_ptr(), _DTYPES[x.dtype], w4.codes.data_ptr(), w4.scales.data_ptr(), _ptr(bias), y.data_ptr(), rows, k, n, int(relu))
+    need = _lib.lib().mdt_mx4_linear_workspace_bytes(rows, k, n)
+    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    _call(x.device, "mdt_mx4_linear", x.data_ptr(), _DTYPES[x.dtype], w4.codes.data_ptr(), w4.scales.data_ptr(), _ptr(bias), y.data_ptr(), rows, k, n, int(relu), _ptr(ws), need)
     return y

@@ -103,15 +103,19 @@ def test_c_entries_refuse_bad_arguments():
     assert L.mdt_conv1x1_act8_backward(None, 16, 16, 16, 1, 16, 16, 16, 16, 16, 100, 18, 72, 16, ws, None) == bad
     assert L.mdt_conv1x1_act8_backward(16, 16, None, 16, 1, 16, 16, 16, 16, 16, 100, 18, 72, 16, ws, None) == bad
     assert L.mdt_conv1x1_act8_backward(16, 16, 16, 16, 1, 16, 16, 16, 16, 16, 100, 0, 72, 16, ws, None) == bad
-    assert L.mdt_mx4_linear(None, 0, 16, 16, 16, 16, 100, 5292, 144, 1, None) == bad
-    assert L.mdt_mx4_linear(16, 0, 24, 16, 16, 16, 100, 5292, 144, 1, None) == bad
-    assert L.mdt_mx4_linear(16, 5, 16, 16, 16, 16, 100, 5292, 144, 1, None) == bad
+    ws = L.mdt_mx4_linear_workspace_bytes(4000, 5292, 144)
+    assert ws > 0 and L.mdt_mx4_linear_workspace_bytes(1, 5292, 144) == 0
+    assert L.mdt_mx4_linear(16, 0, 16, 16, 16, 16, 4000, 5292, 144, 1, 16, ws - 1, None) == small
+    assert L.mdt_mx4_linear(16, 0, 16, 16, 16, 16, 4000, 5292, 144, 1, None, ws, None) == small
+    assert L.mdt_mx4_linear(None, 0, 16, 16, 16, 16, 100, 5292, 144, 1, None, 0, None) == bad
+    assert L.mdt_mx4_linear(16, 0, 24, 16, 16, 16, 100, 5292, 144, 1, None, 0, None) == bad
+    assert L.mdt_mx4_linear(16, 5, 16, 16, 16, 16, 100, 5292, 144, 1, None, 0, None) == bad
     # nothing to do is no error and launches nothing
     assert L.mdt_act8_quantize(None, None, None, 0, 0, 0, None) == 0
     assert L.mdt_act8_restore(None, None, None, 0, 0, 0, None) == 0
     assert L.mdt_bias_act_act8_forward(None, None, None, None, None, None, 0, 4, 1, 1, None) == 0
     assert L.mdt_mx4_quantize(None, None, None, 0, 8, 0, None) == 0
-    assert L.mdt_mx4_linear(None, 0, None, None, None, None, 0, 8, 4, 0, None) == 0
+    assert L.mdt_mx4_linear(None, 0, None, None, None, None, 0, 8, 4, 0, None, 0, None) == 0
 
 
 def test_shapes_that_do_not_belong_together():
