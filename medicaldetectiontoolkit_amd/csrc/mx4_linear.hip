@@ -178,17 +178,50 @@ struct XRows {
             for (int j = 0; j < GV; ++j) v[j] = d < GV ? v[j] : 0.0f;
         }
         if (k0 + CHUNK > k) {
+            const int left = (int)k - k0 - fresh(at);
 #pragma unroll
-            for (int j = 0; j < GV; ++j) v[j] = k0 + at + j < k ? v[j] : 0.0f;
+            for (int j = 0; j < GV; ++j) v[j] = j < left ? v[j] : 0.0f;
         }
+    }
+    // quantize4_group without the detour over float: the maximum of 16-bit patterns, two at a time, and the conversion from the type itself
+    static __device__ __forceinline__ unsigned round16(const vec &t, int &b)
+    {
+        typedef uint16_t u2 __attribute__((ext_vector_type(2)));
+        typedef T t2 __attribute__((ext_vector_type(2)));
+        const v4u whole = __builtin_bit_cast(v4u, t);
+        const unsigned p[4] = {whole[0], whole[1], whole[2], whole[3]};             // (a bit_cast of a vector's element would take the first one)
+        u2 m = __builtin_bit_cast(u2, p[0] & 0x7fff7fffu);
+#pragma unroll
+        for (int j = 1; j < 4; ++j) m = __builtin_elementwise_max(m, __builtin_bit_cast(u2, p[j] & 0x7fff7fffu));
+        const unsigned top = group_max<BLOCK / GV>(umax(m[0], m[1]));
+        b = scale_byte<Q6>(sizeof(T) == 2 && std::is_same<T, __bf16>::value ? top << 16 : __float_as_uint((float)__builtin_bit_cast(_Float16, (uint16_t)top)));
+        const float s = scale_of(b == 255 ? 127 : b);
+        unsigned w = 0;
+        if constexpr (std::is_same<T, __bf16>::value) {
+            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(v2bf, p[0]), s, 0);
+            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(v2bf, p[1]), s, 1);
+            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(v2bf, p[2]), s, 2);
+            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(v2bf, p[3]), s, 3);
+        } else if constexpr (std::is_same<T, _Float16>::value) {
+            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(w, __builtin_bit_cast(v2h, p[0]), s, 0);
+            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(w, __builtin_bit_cast(v2h, p[1]), s, 1);
+            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(w, __builtin_bit_cast(v2h, p[2]), s, 2);
+            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(w, __builtin_bit_cast(v2h, p[3]), s, 3);
+        }
+        return w;                                                                // (a block of scale 255 multiplies as NaN whatever its codes)
     }
     // codes and scales of load i into LDS rows `row` on
     __device__ __forceinline__ void put(uint8_t *codes, uint8_t *scales, const vec &t, int i, int k0, int row, int l) const
     {
-        float v[GV];
-        values(v, t, i, k0);
         int b;
-        const unsigned w = quantize4_group<GV>(v, b);
+        unsigned w;
+        if (GV == 8 && !ragged && k0 + CHUNK <= k) {
+            w = round16(t, b);
+        } else {
+            float v[GV];
+            values(v, t, i, k0);
+            w = quantize4_group<GV>(v, b);
+        }
         const int r = row + l / LPR, c = l % LPR;
         if (GV == 8) *reinterpret_cast<unsigned *>(codes + r * ROW_BYTES + c * 4) = w;
         else *reinterpret_cast<uint16_t *>(codes + r * ROW_BYTES + c * 2) = (uint16_t)w;
@@ -289,19 +322,21 @@ __global__ __launch_bounds__(THREADS, 2) void wide_kernel(const T *__restrict__ 
     typename R::vec X[LOADS];
     Frag F[TN];
     // past the last chunk the last one is loaded and rounded again, into a buffer that nobody reads: no branch around a load
-    auto load_x = [&](int c) {
+    auto load_x = [&](int i, int c) { X[i] = xr.load(i, min(c, chunks - 1) * CHUNK); };
+    auto put_x = [&](int i, int c) { xr.put(s_codes[c & 1], s_scales[c & 1], X[i], i, min(c, chunks - 1) * CHUNK, wave * MINE + i * R::PER, l); };
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i) X[i] = xr.load(i, min(c, chunks - 1) * CHUNK);
-    };
-    auto put_x = [&](int c) {
+    for (int i = 0; i < LOADS; ++i) load_x(i, 0);
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i) xr.put(s_codes[c & 1], s_scales[c & 1], X[i], i, min(c, chunks - 1) * CHUNK, wave * MINE + i * R::PER, l);
-    };
-    load_x(0);
+    for (int i = 0; i < LOADS; ++i) put_x(i, 0);
+    // in the loop's own order, for which its waits are counted
 #pragma unroll
-    for (int t = 0; t < TN; ++t) wr.load(F[t], t, 0);
-    put_x(0);
-    load_x(1);
+    for (int t = 0; t < TN; ++t) {
+        wr.load(F[t], t, 0);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = t * LOADS / TN; i < (t + 1) * LOADS / TN; ++i) load_x(i, 1);
+        __builtin_amdgcn_sched_barrier(0);
+    }
     __syncthreads();
     for (int c = 0; c < chunks; ++c) {
         const uint8_t *codes = s_codes[c & 1], *scales = s_scales[c & 1];
@@ -323,9 +358,13 @@ __global__ __launch_bounds__(THREADS, 2) void wide_kernel(const T *__restrict__ 
 #pragma unroll
             for (int m = 0; m < TM; ++m) asm volatile("" : "+v"(acc[m][t]) : : "memory");
             wr.load(F[t], t, min(c + 1, chunks - 1));
+            // a share of the next chunk's rounding between the products, which run beside it
+#pragma unroll
+            for (int i = t * LOADS / TN; i < (t + 1) * LOADS / TN; ++i) {
+                put_x(i, c + 1);
+                load_x(i, c + 2);
+            }
         }
-        put_x(c + 1);
-        load_x(c + 2);
         __syncthreads();
     }
     float add[TN][4];
