@@ -483,19 +483,6 @@ __global__ __launch_bounds__(THREADS, MT * NT <= 3 ? 2 : 1) void fused_kernel(co
     v4u *wp = smem;                                                              // [NT][KS][3][64] pieces of W in fragment order
     float *gs = reinterpret_cast<float *>(smem + NT * KS * 3 * 64) + wave * fused_wave_floats(MT, NT, ci, co);
     uint16_t *xb = reinterpret_cast<uint16_t *>(gs + fused_rows_floats(MT, ci, co));
-    for (int t = threadIdx.x; t < NT * KS * 64; t += THREADS) {
-        const int ll = t & 63, n = (t / 64 / KS) * 32 + (ll & 31), k = (t / 64 % KS) * 16 + 8 * (ll >> 5);
-        float b[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) b[j] = n < ci && k + j < co ? w[(k + j) * ci + n] : 0.0f;
-        const Split8 B = split8(b);
-        v4u *to = wp + (t / 64) * 3 * 64 + ll;
-        to[0] = __builtin_bit_cast(v4u, B.hi);
-        to[64] = __builtin_bit_cast(v4u, B.mid);
-        to[128] = __builtin_bit_cast(v4u, B.lo);
-    }
-    __syncthreads();
-
     const long long chunks = (V + 31) / 32, full = V / 32, step = (long long)gridDim.x * WAVES;
     long long chunk = (long long)blockIdx.x * WAVES + wave;
     v4f G[4 * MT];
@@ -527,20 +514,41 @@ __global__ __launch_bounds__(THREADS, MT * NT <= 3 ? 2 : 1) void fused_kernel(co
 #pragma unroll
         for (int q = 0; q < 4 * MT; ++q) G[q] = *reinterpret_cast<const Io<float>::vec *>(pg + 4 * at_gy(ln, q));
     };
-    // the last chunk where it is short: value by value, straight into the tiles
+    // the last chunk where it is short: value by value, straight into the tiles (8 loads in flight)
     auto fill_short = [&](long long c) {
-        for (int e = l; e < 32 * co; e += 64) {
-            const long long at = c * 32 * co + e;
-            float t = 0.0f;
-            if (at < V * co) {
-                t = yc == nullptr || yc[at] ? gy[at] : 0.0f;
-                if (G_OUT) g_out[at] = t;
+        const long long g0 = c * 32 * co, x0 = c * 32 * ci;
+        const int ng = (int)(V * co - g0), nx = (int)(V * ci - x0);
+        for (int e0 = l; e0 < 32 * co; e0 += 64 * 8) {
+            float t[8];
+            unsigned m[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int e = min(e0 + 64 * u, ng - 1);
+                t[u] = gy[g0 + e];
+                m[u] = yc != nullptr ? yc[g0 + e] : 1u;
             }
-            gs[e] = t;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int e = e0 + 64 * u;
+                t[u] = m[u] && e < ng ? t[u] : 0.0f;
+                if (e < 32 * co) gs[e] = t[u];
+                if (G_OUT && e < ng) g_out[g0 + e] = t[u];
+            }
         }
-        for (int e = l; e < 32 * ci; e += 64) {
-            const long long at = c * 32 * ci + e;
-            xb[e] = at < V * ci ? (uint16_t)(__float_as_uint(code_value(xc[at], x_relu, xs[at >> 5])) >> 16) : (uint16_t)0;
+        for (int e0 = l; e0 < 32 * ci; e0 += 64 * 8) {
+            unsigned t[8];
+            int b[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int e = min(e0 + 64 * u, nx - 1);
+                t[u] = xc[x0 + e];
+                b[u] = xs[(x0 + e) >> 5];
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int e = e0 + 64 * u;
+                if (e < 32 * ci) xb[e] = e < nx ? (uint16_t)(__float_as_uint(code_value(t[u], x_relu, b[u])) >> 16) : (uint16_t)0;
+            }
         }
     };
     auto fence = [] {
@@ -556,6 +564,18 @@ __global__ __launch_bounds__(THREADS, MT * NT <= 3 ? 2 : 1) void fused_kernel(co
         for (int n = 0; n < NT; ++n) acc[m][n] = v16f{};
     }
     if (chunk < full) load(chunk);
+    for (int t = threadIdx.x; t < NT * KS * 64; t += THREADS) {
+        const int ll = t & 63, n = (t / 64 / KS) * 32 + (ll & 31), k = (t / 64 % KS) * 16 + 8 * (ll >> 5);
+        float b[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) b[j] = n < ci && k + j < co ? w[(k + j) * ci + n] : 0.0f;
+        const Split8 B = split8(b);
+        v4u *to = wp + (t / 64) * 3 * 64 + ll;
+        to[0] = __builtin_bit_cast(v4u, B.hi);
+        to[64] = __builtin_bit_cast(v4u, B.mid);
+        to[128] = __builtin_bit_cast(v4u, B.lo);
+    }
+    __syncthreads();
     for (; chunk < chunks; chunk += step) {
         const bool whole = chunk < full;
         if (whole) {

@@ -8,7 +8,7 @@
 // scales.  x's come from LDS, where the lanes that loaded x put its codes (a row of a chunk is 64 lanes of 4 floats, or 32 lanes of 8 values of 16 bits, so a
 // block's maximum is a few lane permutes).  W's come straight from memory into registers: for few rows of x from W as it is kept, where the 64 lanes of a
 // load touch 16 rows and cost 64 requests; for more rows from a copy in the lanes' order, one contiguous kilobyte a load, that a first launch makes in the
-// workspace (the 2D head, 10000 x 9408 -> 768: 151 us without the copy, TIME us with it).  With W as the first operand a lane ends up with 4 consecutive
+// workspace (the 2D head, 10000 x 9408 -> 768: 151 us without the copy, 5 + 87 us with it).  With W as the first operand a lane ends up with 4 consecutive
 // outputs of one row.
 //
 // Two shapes of the same loop:
@@ -25,7 +25,6 @@ using namespace mdt_bs;
 constexpr int WAVES = 8;
 constexpr int THREADS = 64 * WAVES;
 constexpr int CHUNK = 256, CHUNK_BLOCKS = CHUNK / BLOCK;
-constexpr long long COPY_ROWS = 256;                       // from so many rows on W is copied into the lanes' order
 constexpr int ROW_BYTES = CHUNK / 2 + 16;                   // a row of codes in LDS, padded: 16-byte reads of neighbouring rows fall into different banks
 
 
@@ -261,16 +260,23 @@ __global__ __launch_bounds__(THREADS, 2) void narrow_kernel(const T *__restrict_
     for (int t = 0; t < TN; ++t) acc[t] = v4f{};
     typename R::vec X[LOADS];
     Frag F[TN];
+    // loads of x that hold a row at all; the codes of the other rows are whatever LDS holds and end in outputs that are not stored
+    const int mine = (int)min(rows - row0, 16LL), some = (mine + R::PER - 1) / R::PER;
     auto load = [&](int c) {
+        if (some == LOADS) {
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i) X[i] = xr.load(i, c * CHUNK);
+            for (int i = 0; i < LOADS; ++i) X[i] = xr.load(i, c * CHUNK);
+        } else {
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i) if (i < some) X[i] = xr.load(i, c * CHUNK);
+        }
 #pragma unroll
         for (int t = 0; t < TN; ++t) wr.load(F[t], t, c);
     };
     if (wave < chunks) load(wave);
     for (int c = wave; c < chunks; c += WAVES) {
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i) xr.put(codes, scales, X[i], i, c * CHUNK, i * R::PER, l);
+        for (int i = 0; i < LOADS; ++i) if (i < some) xr.put(codes, scales, X[i], i, c * CHUNK, i * R::PER, l);
         wave_fence();
         const v4u x0 = *reinterpret_cast<const v4u *>(codes + r * ROW_BYTES + q * 32), x1 = *reinterpret_cast<const v4u *>(codes + r * ROW_BYTES + q * 32 + 16);
         const unsigned xs = *reinterpret_cast<const uint16_t *>(scales + r * CHUNK_BLOCKS + q * 2);
@@ -424,36 +430,50 @@ inline Tiled tiled_of(long long k, int n)
     t.bytes = t.codes + (size_t)t.chunks * t.tiles * 128;
     return t;
 }
-inline bool copies_w(long long rows) { return rows >= COPY_ROWS; }
+// The wide shape for many columns and many rows; for few rows only where the sum is long (1500 x 5000 -> 500, fp32: 27 us, narrow 39; 1000 x 2000 -> 300,
+// fp16: 18 us, narrow 13).  Its W is copied into the lanes' order, the narrow one's where rows and sum make up for the launch (600 x 5292 -> 144: 23 us, else
+// 29; 4000 x 144 -> 144: 18 us, else 13).
+inline bool is_wide(long long rows, long long k, int n) { return n > 144 && (rows >= 2048 || (rows >= 512 && k >= 4096)); }
+inline bool copies_w(long long rows, long long k, int n) { return is_wide(rows, k, n) || (rows >= 256 && k >= 4096); }
+
+template <typename T, int TM>
+int wide_by_columns(const Call &a, int ranges)
+{
+    switch ((a.n + 128 * ranges - 1) / (128 * ranges)) {
+        case 1: case 2: return wide<T, TM, 2>(a);
+        case 3: return wide<T, TM, 3>(a);
+        case 4: return wide<T, TM, 4>(a);
+        case 5: return wide<T, TM, 5>(a);
+        default: return wide<T, TM, 6>(a);
+    }
+}
+
+// as few ranges of columns as still give most CUs a workgroup: each range rounds x again
+template <typename T, class W>
+int narrow_by_columns(const Call &a)
+{
+    const long long row_tiles = (a.rows + 15) / 16;
+    if (a.n > 48 && row_tiles * ((a.n + 143) / 144) >= 96) return narrow<T, 9, W, false>(a);
+    if (a.n > 16 && row_tiles * ((a.n + 47) / 48) >= 96) return narrow<T, 3, W, false>(a);
+    return narrow<T, 1, W, false>(a);
+}
 
 template <typename T>
 int run(Call a, uint8_t *workspace)
 {
-    if (copies_w(a.rows)) {
+    if (copies_w(a.rows, a.k, a.n)) {
         const Tiled t = tiled_of(a.k, a.n);
         tile_weights_kernel<<<dim3((t.chunks + 3) / 4, t.tiles), 256, 0, a.s>>>(a.wc, a.ws, workspace, workspace + t.codes, a.n, (int)((a.k + BLOCK - 1) / BLOCK), t.chunks);
         a.wc = workspace;
         a.ws = workspace + t.codes;
-        constexpr int TM = 3;
-        if (a.n > 144 && a.rows >= 2048) {
-            const int ranges = (a.n + 767) / 768, per = (a.n + 128 * ranges - 1) / (128 * ranges);
-            switch (per) {
-                case 1: case 2: return wide<T, TM, 2>(a);
-                case 3: return wide<T, TM, 3>(a);
-                case 4: return wide<T, TM, 4>(a);
-                case 5: return wide<T, TM, 5>(a);
-                default: return wide<T, TM, 6>(a);
-            }
-        }
-        if (a.n > 48) return narrow<T, 9, WTiled, false>(a);
-        return a.n > 16 ? narrow<T, 3, WTiled, false>(a) : narrow<T, 1, WTiled, false>(a);
+        if (!is_wide(a.rows, a.k, a.n)) return narrow_by_columns<T, WTiled>(a);
+        const int ranges = (a.n + 767) / 768;
+        // 16 rows a workgroup while that gives a CU few of them, else 48: a turn of the short ones takes about 6 / 10 of a long one's (2500 x 9408 -> 768: 56 us, 80)
+        const long long short_turns = ((a.rows + 15) / 16 * ranges + 255) / 256, long_turns = ((a.rows + 47) / 48 * ranges + 255) / 256;
+        return 6 * short_turns < 10 * long_turns ? wide_by_columns<T, 1>(a, ranges) : wide_by_columns<T, 3>(a, ranges);
     }
-    // as few ranges of columns as still give half of the CUs a workgroup: each range rounds x again
-    const long long row_tiles = (a.rows + 15) / 16;
     if (a.rows * a.k < Io<T>::GV) return narrow<T, 1, WKept<true>, true>(a);
-    const bool three = row_tiles * ((a.n + 47) / 48) >= 128 && a.n > 16;
-    if (a.k <= BLOCK) return three ? narrow<T, 3, WKept<true>, false>(a) : narrow<T, 1, WKept<true>, false>(a);
-    return three ? narrow<T, 3, WKept<false>, false>(a) : narrow<T, 1, WKept<false>, false>(a);
+    return a.k <= BLOCK ? narrow_by_columns<T, WKept<true>>(a) : narrow_by_columns<T, WKept<false>>(a);
 }
 
 }  // namespace
@@ -463,7 +483,7 @@ extern "C" {
 size_t mdt_mx4_linear_workspace_bytes(long long rows, long long k, int n)
 {
     if (rows < 1 || k < 1 || n < 1 || k > (1 << 22) || n > (1 << 20)) return 0;
-    return copies_w(rows) ? tiled_of(k, n).bytes : 0;
+    return copies_w(rows, k, n) ? tiled_of(k, n).bytes : 0;
 }
 
 int mdt_mx4_linear(const void *x, int dtype, const void *w_codes, const void *w_scales, const float *bias, void *y, long long rows, long long k, int n, int relu, void *workspace,

@@ -42,6 +42,11 @@ def _ptr(t):
     return t.data_ptr() if t is not None else None
 
 
+def _on_gpu(device, name):
+    if device.type != "cuda":
+        raise RuntimeError("%s must live on the GPU: the MI355X HIP path is the only implementation (no CPU fallback in the product path)" % name)
+
+
 def _float_tensor(x, name):
     if x.dtype not in _DTYPES:
         raise TypeError("%s: float32, bfloat16 or float16, not %s" % (name, x.dtype))
@@ -90,10 +95,15 @@ def _dense(x):
     return x, x.dim() == 2
 
 
+def _scales_at(n):
+    """where the scales of n codes begin in a buffer that holds both"""
+    return (n + 15) // 16 * 16
+
+
 class Checkpoint8(object):
     """An activation kept in 8 bits: `codes` (uint8, one a value, storage order) and `scales` (uint8, one for 32 codes).  `channels_last`: axis 1 is the
-    innermost of the storage (for two axes it always is)."""
-    __slots__ = ("codes", "scales", "shape", "relu", "dtype", "channels_last")
+    innermost of the storage (for two axes it always is).  What the operators make holds both in one allocation, `buffer`."""
+    __slots__ = ("buffer", "_codes", "_scales", "shape", "relu", "dtype", "channels_last", "device")
 
     def __init__(self, codes, scales, shape, relu=False, dtype=torch.float32, channels_last=None):
         shape = tuple(int(s) for s in shape)
@@ -110,7 +120,31 @@ class Checkpoint8(object):
         elif (channels_last and len(shape) not in (2, 4, 5)) or (len(shape) == 2 and not channels_last):
             raise ValueError("Checkpoint8: channels_last=%s does not describe %d axes" % (channels_last, len(shape)))
         _same_device(codes.device, scales=scales)
-        self.codes, self.scales, self.shape, self.relu, self.dtype, self.channels_last = codes, scales, shape, bool(relu), dtype, bool(channels_last)
+        self._set(None, codes, scales, shape, bool(relu), dtype, bool(channels_last), codes.device)
+
+    def _set(self, buffer, codes, scales, shape, relu, dtype, channels_last, device):
+        self.buffer, self._codes, self._scales, self.shape, self.relu, self.dtype, self.channels_last, self.device = buffer, codes, scales, shape, relu, dtype, channels_last, device
+        return self
+
+    @classmethod
+    def of_buffer(cls, buffer, shape, relu, dtype, channels_last):
+        """codes and, from _scales_at(values) on, scales in one uint8 tensor"""
+        return cls.__new__(cls)._set(buffer, None, None, shape, relu, dtype, channels_last, buffer.device)
+
+    @property
+    def codes(self):
+        return self._codes if self.buffer is None else self.buffer[:math.prod(self.shape)]
+
+    @property
+    def scales(self):
+        return self._scales if self.buffer is None else self.buffer[_scales_at(math.prod(self.shape)):]
+
+    def pointers(self):
+        """(codes, scales) as addresses"""
+        if self.buffer is None:
+            return self._codes.data_ptr(), self._scales.data_ptr()
+        at = self.buffer.data_ptr()
+        return at, at + _scales_at(math.prod(self.shape))
 
     @property
     def stride(self):
@@ -118,23 +152,26 @@ class Checkpoint8(object):
 
     def restore(self):
         """the kept values, in the type, shape and storage order of the tensor they were taken from"""
-        _lib.require_cuda(self.codes, "Checkpoint8.codes")
-        x = torch.empty_strided(self.shape, self.stride, dtype=self.dtype, device=self.codes.device)
-        _call(x.device, "mdt_act8_restore", self.codes.data_ptr(), self.scales.data_ptr(), x.data_ptr(), x.numel(), _DTYPES[self.dtype], int(self.relu))
+        _on_gpu(self.device, "Checkpoint8")
+        x = torch.empty_strided(self.shape, self.stride, dtype=self.dtype, device=self.device)
+        codes, scales = self.pointers()
+        _call(self.device, "mdt_act8_restore", codes, scales, x.data_ptr(), x.numel(), _DTYPES[self.dtype], int(self.relu))
         return x
 
 
-def _new_codes(n, device):
-    return torch.empty(n, dtype=torch.uint8, device=device), torch.empty(-(-n // BLOCK), dtype=torch.uint8, device=device)
+def _new_buffer(n, device):
+    return torch.empty(_scales_at(n) + -(-n // BLOCK), dtype=torch.uint8, device=device)
 
 
 def checkpoint8(x, relu=False):
     """x's values in 8 bits.  relu=True: x is the output of a ReLU (values <= 0 read back as 0) and is kept with twice the resolution."""
     _float_tensor(x, "x")
-    x, cl = _dense(x.detach())
-    codes, scales = _new_codes(x.numel(), x.device)
-    _call(x.device, "mdt_act8_quantize", x.data_ptr(), codes.data_ptr(), scales.data_ptr(), x.numel(), _DTYPES[x.dtype], int(relu))
-    return Checkpoint8(codes, scales, x.shape, relu, x.dtype, cl)
+    x, cl = _dense(x)
+    n, device = x.numel(), x.device
+    buffer = _new_buffer(n, device)
+    at = buffer.data_ptr()
+    _call(device, "mdt_act8_quantize", x.data_ptr(), at, at + _scales_at(n), n, _DTYPES[x.dtype], int(relu))
+    return Checkpoint8.of_buffer(buffer, tuple(x.shape), bool(relu), x.dtype, cl)
 
 
 def bias_act_checkpoint8(h, bias, residual=None, relu=True, inplace=False):
@@ -157,11 +194,12 @@ def bias_act_checkpoint8(h, bias, residual=None, relu=True, inplace=False):
     if not bias.is_contiguous():
         bias = bias.contiguous()
     y = x if inplace else torch.empty_like(x)
-    codes, scales = _new_codes(x.numel(), x.device)
-    if x.numel():
-        _call(x.device, "mdt_bias_act_act8_forward", y.data_ptr(), x.data_ptr(), bias.data_ptr(), _ptr(residual), codes.data_ptr(), scales.data_ptr(), x.numel(),
-              int(x.shape[1]), inner, int(relu))
-    return y, Checkpoint8(codes, scales, x.shape, relu, x.dtype, cl)
+    n, device = x.numel(), x.device
+    buffer = _new_buffer(n, device)
+    if n:
+        at = buffer.data_ptr()
+        _call(device, "mdt_bias_act_act8_forward", y.data_ptr(), x.data_ptr(), bias.data_ptr(), _ptr(residual), at, at + _scales_at(n), n, int(x.shape[1]), inner, int(relu))
+    return y, Checkpoint8.of_buffer(buffer, tuple(x.shape), bool(relu), x.dtype, cl)
 
 
 def conv1x1_backward8(gy, w, x8, y8=None, need_g=False, need_gx=True, need_gw=True):
@@ -174,7 +212,8 @@ def conv1x1_backward8(gy, w, x8, y8=None, need_g=False, need_gx=True, need_gw=Tr
     _lib.require_cuda(gy, "gy")
     if w.dim() < 2 or math.prod(w.shape[2:]) != 1:
         raise ValueError("conv1x1_backward8: a 1x1(x1) filter, not %s" % (tuple(w.shape),))
-    co, ci = int(w.shape[0]), int(w.shape[1])
+    w_shape = tuple(w.shape)
+    co, ci = w_shape[:2]
     shape = tuple(gy.shape)
     if gy.dim() not in (2, 4, 5) or shape[1] != co or x8.shape != shape[:1] + (ci,) + shape[2:]:
         raise ValueError("conv1x1_backward8: gy %s, w %s and x8 %s do not belong together" % (shape, tuple(w.shape), x8.shape))
@@ -182,25 +221,23 @@ def conv1x1_backward8(gy, w, x8, y8=None, need_g=False, need_gx=True, need_gw=Tr
         raise ValueError("conv1x1_backward8: the kept maps have their channels innermost")
     if y8 is not None and (y8.shape != shape or not y8.relu):
         raise ValueError("conv1x1_backward8: y8 is the kept ReLU output of gy's shape")
-    _same_device(gy.device, w=w, x8=x8.codes, y8=None if y8 is None else y8.codes)
     dev = gy.device
-    gy = gy.detach()
+    _same_device(dev, w=w, x8=x8, y8=y8)
     mf = _rows_format(gy.dim())
     if not gy.is_contiguous(memory_format=mf):
         gy = gy.contiguous(memory_format=mf)
-    wm = w.detach().reshape(co, ci)
-    if not wm.is_contiguous():
-        wm = wm.contiguous()
+    if w.stride()[:2] != (ci, 1):
+        w = w.detach().reshape(co, ci).contiguous()
     V = gy.numel() // co
     gx = torch.empty_strided(x8.shape, x8.stride, dtype=torch.float32, device=dev) if need_gx else None
-    gw = torch.empty(co, ci, dtype=torch.float32, device=dev) if need_gw else None
+    gw = torch.empty(w_shape, dtype=torch.float32, device=dev) if need_gw else None
     gbias = torch.empty(co, dtype=torch.float32, device=dev)
     write_g = need_g and y8 is not None
     g = torch.empty_like(gy) if write_g else None
     ws = torch.empty(_lib.lib().mdt_conv1x1_act8_backward_workspace_bytes(V, ci, co), dtype=torch.uint8, device=dev)
-    _call(dev, "mdt_conv1x1_act8_backward", gy.data_ptr(), wm.data_ptr(), x8.codes.data_ptr(), x8.scales.data_ptr(), int(x8.relu), _ptr(y8.codes if y8 is not None else None),
+    _call(dev, "mdt_conv1x1_act8_backward", gy.data_ptr(), w.data_ptr(), *x8.pointers(), int(x8.relu), y8.pointers()[0] if y8 is not None else None,
           _ptr(gx), _ptr(gw), gbias.data_ptr(), _ptr(g), V, ci, co, ws.data_ptr(), ws.numel())
-    return gx, (gw.view(w.shape) if gw is not None else None), gbias, (g if write_g else gy if need_g else None)
+    return gx, gw, gbias, (g if write_g else gy if need_g else None)
 
 
 class Mx4(object):
