@@ -56,7 +56,7 @@ constexpr int KSTEP = 32, KROW = KSTEP + 8;
 __device__ __forceinline__ v8bf row_of(const uint16_t *p) { return __builtin_bit_cast(v8bf, *reinterpret_cast<const v4u *>(p)); }
 
 // A run of values from base[first] on, read 4 at a time at 32-bit offsets without branches (so that the number of loads in flight stays known and a wait for
-// one does not become a wait for all): where 4 values would pass the end of the array, the last 4 are read, and fix() moves them to their places.
+// one does not become a wait for all): where 4 values would pass the end of the array, the last 4 are read, and fix() moves them to their places, zeros behind.
 struct Run {
     long long first;        // of the base: the run's first element, or the array's fourth last
     int delta, last;        // the run's first element and the last 4 of the array, counted from the base
@@ -72,8 +72,8 @@ struct Run {
     {
         const int d = off + delta - last;
         const bool one = d > 0 && (d & 1), two = d > 0 && (d & 2), none = d >= 4;
-        v = v4f{one ? v[1] : v[0], one ? v[2] : v[1], one ? v[3] : v[2], v[3]};
-        v = v4f{two ? v[2] : v[0], two ? v[3] : v[1], v[2], v[3]};
+        v = v4f{one ? v[1] : v[0], one ? v[2] : v[1], one ? v[3] : v[2], one ? 0.0f : v[3]};
+        v = v4f{two ? v[2] : v[0], two ? v[3] : v[1], two ? 0.0f : v[2], two ? 0.0f : v[3]};
         return v4f{none ? 0.0f : v[0], none ? 0.0f : v[1], none ? 0.0f : v[2], none ? 0.0f : v[3]};
     }
     __device__ __forceinline__ unsigned fix(unsigned v, int off) const
@@ -483,12 +483,12 @@ __global__ __launch_bounds__(THREADS, MT * NT <= 3 ? 2 : 1) void fused_kernel(co
     v4u *wp = smem;                                                              // [NT][KS][3][64] pieces of W in fragment order
     float *gs = reinterpret_cast<float *>(smem + NT * KS * 3 * 64) + wave * fused_wave_floats(MT, NT, ci, co);
     uint16_t *xb = reinterpret_cast<uint16_t *>(gs + fused_rows_floats(MT, ci, co));
-    const long long chunks = (V + 31) / 32, full = V / 32, step = (long long)gridDim.x * WAVES;
+    const long long chunks = (V + 31) / 32, full = V / 32, step = (long long)gridDim.x * WAVES, last_scale = (V * ci - 1) >> 5;
     long long chunk = (long long)blockIdx.x * WAVES + wave;
     v4f G[4 * MT];
     unsigned Y[4 * MT], X[4 * NT];
     int S[4 * NT];
-    // lanes behind the run's end repeat its last 16 bytes (and store them to the same place again)
+    // lanes behind the chunk's end repeat its last 16 bytes (and store them to the same place again)
     auto at_gy = [&](unsigned lane, int q) { return min(q * 64 + lane, 8u * co - 1); };
     auto at_x = [&](unsigned lane, int q) { return min(q * 64 + lane, 8u * ci - 1); };
     // the lane's number, kept from the optimiser: it would hold every address that it computes from it in a register of its own over the loop
@@ -499,57 +499,23 @@ __global__ __launch_bounds__(THREADS, MT * NT <= 3 ? 2 : 1) void fused_kernel(co
     };
     auto load = [&](long long c) {
         const unsigned ln = lane();
+        const Run rg(c * 32 * co, V * co), rx(c * 32 * ci, V * ci);
+        // 16 bytes behind the chunk's end or the array's: the last ones again
+        const int g0 = 4 * ln + rg.delta, x0 = 4 * ln + rx.delta, g1 = min(32 * co - 4 + rg.delta, rg.last), x1 = min(32 * ci - 4 + rx.delta, rx.last);
+        const int s0 = ln >> 3, s1 = (int)min(last_scale - c * ci, ci - 1LL);
+        const float *pg = gy + rg.first;
+        const uint8_t *py = yc + rg.first, *px = xc + rx.first, *ps = xs + c * ci;
         if (yc != nullptr) {
-            const uint8_t *py = yc + c * 32 * co;
 #pragma unroll
-            for (int q = 0; q < 4 * MT; ++q) Y[q] = *reinterpret_cast<const unsigned *>(py + 4 * at_gy(ln, q));
+            for (int q = 0; q < 4 * MT; ++q) Y[q] = get4(py + (unsigned)min(g0 + q * 256, g1));
         }
-        const uint8_t *px = xc + c * 32 * ci, *ps = xs + c * ci;
 #pragma unroll
         for (int q = 0; q < 4 * NT; ++q) {
-            X[q] = *reinterpret_cast<const unsigned *>(px + 4 * at_x(ln, q));
-            S[q] = ps[at_x(ln, q) >> 3];
+            X[q] = get4(px + (unsigned)min(x0 + q * 256, x1));
+            S[q] = ps[(unsigned)min(s0 + q * 8, s1)];
         }
-        const float *pg = gy + c * 32 * co;
 #pragma unroll
-        for (int q = 0; q < 4 * MT; ++q) G[q] = *reinterpret_cast<const Io<float>::vec *>(pg + 4 * at_gy(ln, q));
-    };
-    // the last chunk where it is short: value by value, straight into the tiles (8 loads in flight)
-    auto fill_short = [&](long long c) {
-        const long long g0 = c * 32 * co, x0 = c * 32 * ci;
-        const int ng = (int)(V * co - g0), nx = (int)(V * ci - x0);
-        for (int e0 = l; e0 < 32 * co; e0 += 64 * 8) {
-            float t[8];
-            unsigned m[8];
-#pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                const int e = min(e0 + 64 * u, ng - 1);
-                t[u] = gy[g0 + e];
-                m[u] = yc != nullptr ? yc[g0 + e] : 1u;
-            }
-#pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                const int e = e0 + 64 * u;
-                t[u] = m[u] && e < ng ? t[u] : 0.0f;
-                if (e < 32 * co) gs[e] = t[u];
-                if (G_OUT && e < ng) g_out[g0 + e] = t[u];
-            }
-        }
-        for (int e0 = l; e0 < 32 * ci; e0 += 64 * 8) {
-            unsigned t[8];
-            int b[8];
-#pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                const int e = min(e0 + 64 * u, nx - 1);
-                t[u] = xc[x0 + e];
-                b[u] = xs[(x0 + e) >> 5];
-            }
-#pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                const int e = e0 + 64 * u;
-                if (e < 32 * ci) xb[e] = e < nx ? (uint16_t)(__float_as_uint(code_value(t[u], x_relu, b[u])) >> 16) : (uint16_t)0;
-            }
-        }
+        for (int q = 0; q < 4 * MT; ++q) G[q] = get4(pg + (unsigned)min(g0 + q * 256, g1));
     };
     auto fence = [] {
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -563,12 +529,14 @@ __global__ __launch_bounds__(THREADS, MT * NT <= 3 ? 2 : 1) void fused_kernel(co
 #pragma unroll
         for (int n = 0; n < NT; ++n) acc[m][n] = v16f{};
     }
-    if (chunk < full) load(chunk);
+    if (chunk < chunks) load(chunk);
     for (int t = threadIdx.x; t < NT * KS * 64; t += THREADS) {
         const int ll = t & 63, n = (t / 64 / KS) * 32 + (ll & 31), k = (t / 64 % KS) * 16 + 8 * (ll >> 5);
         float b[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) b[j] = n < ci && k + j < co ? w[(k + j) * ci + n] : 0.0f;
+        for (int j = 0; j < 8; ++j) b[j] = w[min(k + j, co - 1) * ci + min(n, ci - 1)];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) b[j] = n < ci && k + j < co ? b[j] : 0.0f;
         const Split8 B = split8(b);
         v4u *to = wp + (t / 64) * 3 * 64 + ll;
         to[0] = __builtin_bit_cast(v4u, B.hi);
@@ -578,30 +546,40 @@ __global__ __launch_bounds__(THREADS, MT * NT <= 3 ? 2 : 1) void fused_kernel(co
     __syncthreads();
     for (; chunk < chunks; chunk += step) {
         const bool whole = chunk < full;
-        if (whole) {
-            const unsigned ln = lane();
+        const unsigned lp = lane();
+        if (!whole) {
+            const Run rg(chunk * 32 * co, V * co), rx(chunk * 32 * ci, V * ci);
 #pragma unroll
             for (int q = 0; q < 4 * MT; ++q) {
-                if (yc != nullptr) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) G[q][j] = (Y[q] >> (8 * j) & 255u) ? G[q][j] : 0.0f;
-                }
-                *reinterpret_cast<v4f *>(gs + 4 * at_gy(ln, q)) = G[q];
+                G[q] = rg.fix(G[q], 4 * at_gy(lp, q));
+                if (yc != nullptr) Y[q] = rg.fix(Y[q], 4 * at_gy(lp, q));
             }
 #pragma unroll
             for (int q = 0; q < 4 * NT; ++q) {
-                float t[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) t[j] = code_value(X[q] >> (8 * j) & 255u, x_relu, S[q]);
-                uint2 p;
-                p.x = pack_hi(t[0], t[1]);
-                p.y = pack_hi(t[2], t[3]);
-                *reinterpret_cast<uint2 *>(xb + 4 * at_x(ln, q)) = p;
+                X[q] = rx.fix(X[q], 4 * at_x(lp, q));
             }
-        } else {
-            fill_short(chunk);
         }
-        if (chunk + step < full) load(chunk + step);
+#pragma unroll
+        for (int q = 0; q < 4 * MT; ++q) {
+            if (yc != nullptr) G[q] = masked(G[q], Y[q]);
+            *reinterpret_cast<v4f *>(gs + 4 * at_gy(lp, q)) = G[q];
+        }
+#pragma unroll
+        for (int q = 0; q < 4 * NT; ++q) {
+            float t[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) t[j] = code_value(X[q] >> (8 * j) & 255u, x_relu, S[q]);
+            if (!whole) {                                                        // a scale of NaN must not reach the voxels behind the last one
+                const int left = (int)(V - chunk * 32) * ci - 4 * (int)at_x(lp, q);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) t[j] = j < left ? t[j] : 0.0f;
+            }
+            uint2 p;
+            p.x = pack_hi(t[0], t[1]);
+            p.y = pack_hi(t[2], t[3]);
+            *reinterpret_cast<uint2 *>(xb + 4 * at_x(lp, q)) = p;
+        }
+        if (chunk + step < chunks) load(chunk + step);
         fence();
         // gw and gbias
         const unsigned lg = lane(), og = 8 * (lg >> 5) * co + (lg & 31), ox = 8 * (lg >> 5) * ci + (lg & 31);
@@ -662,11 +640,15 @@ __global__ __launch_bounds__(THREADS, MT * NT <= 3 ? 2 : 1) void fused_kernel(co
                 d[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(hi, B.hi, d[n], 0, 0, 0);
             }
         }
-        if (G_OUT && whole) {
+        if (G_OUT) {
             float *pg = g_out + chunk * 32 * co;
-            const unsigned ln = lane();
+            if (whole) {
+                const unsigned ln = lane();
 #pragma unroll
-            for (int q = 0; q < 4 * MT; ++q) *reinterpret_cast<Io<float>::vec *>(pg + 4 * at_gy(ln, q)) = *reinterpret_cast<const v4f *>(gs + 4 * at_gy(ln, q));
+                for (int q = 0; q < 4 * MT; ++q) *reinterpret_cast<Io<float>::vec *>(pg + 4 * at_gy(ln, q)) = *reinterpret_cast<const v4f *>(gs + 4 * at_gy(ln, q));
+            } else {
+                for (int e = l; e < (V - chunk * 32) * co; e += 64) pg[e] = gs[e];
+            }
         }
         fence();
 #pragma unroll
@@ -841,7 +823,7 @@ int mdt_conv1x1_act8_backward(const float *gy, const float *w, const void *x_cod
     if ((sums || gx) && (workspace == nullptr || workspace_bytes < mdt_conv1x1_act8_backward_workspace_bytes(V, c_in, c_out))) return MDT_ERR_WORKSPACE_TOO_SMALL;
     Args a = {gy, (const uint8_t *)y_codes, w, (const uint8_t *)x_codes, (const uint8_t *)x_scales, gx, g, (float *)workspace, nullptr, V, c_in, c_out, x_relu};
     const FusedPlan f = gx && gw ? fused_plan(V, c_in, c_out) : FusedPlan{0, 0, 0, 0};
-    if (f.mt > 0) {
+    if (f.mt > 0 && V * c_in >= 4 && V * c_out >= 4) {
         a.part_b = a.part_w + f.blocks * nw;
         const int rc = fused_run(f, a, s);
         if (rc != MDT_OK) return rc;

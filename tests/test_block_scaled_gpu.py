@@ -315,6 +315,20 @@ def test_conv1x1_backward8_masked_rows_hide_non_finite_gradients(cuda):
     assert not torch.isfinite(gx[0]).any() and torch.isfinite(gx[1:]).all() and not torch.isfinite(gw[0]).any() and torch.isfinite(gw[1:]).all() and not torch.isfinite(gb[0])
 
 
+@pytest.mark.parametrize("V,ci,co", [(33, 18, 72), (70, 7, 5), (300, 200, 40), (65, 40, 300), (129, 33, 170)])
+def test_conv1x1_backward8_non_finite_inputs_show_where_they_are_used(cuda, V, ci, co):
+    """a kept block with a NaN poisons the 32 values of the block and nothing else, also where it is the last and the tiles reach behind it"""
+    x, gy, w, y = layer(V, ci, co, True, 9, cuda)
+    x[V - 1, ci - 1] = float("nan")
+    x8 = bs.checkpoint8(x, relu=True)
+    xd = x8.restore().cpu().double()
+    assert torch.isnan(xd.reshape(-1)[-1]) and torch.isnan(xd).sum() <= 32
+    gx, gw, gb, _ = bs.conv1x1_backward8(gy, w, x8, None)
+    want = gy.cpu().double().t() @ xd
+    assert torch.equal(torch.isnan(gw).cpu(), torch.isnan(want)) and torch.equal(gw.cpu().double().nan_to_num(), want.nan_to_num())
+    assert torch.equal(gx.cpu().double(), gy.cpu().double() @ w.cpu().double()) and torch.isfinite(gb).all()
+
+
 # ---- 4 bits ------------------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows,k", [(1, 1), (1, 31), (3, 32), (2, 33), (1, 416), (7, 100), (5, 1000), (130, 64), (2, 5292), (4099, 7)])
