@@ -31,6 +31,8 @@ class Configs(object):
         self.sixth_pooling = False
         self.n_latent_dims = 0
         self.operate_stride1 = False
+        # training memory: the maps of the residual stages and of the pyramid kept for the backward pass in 8 bits (utils/block_scaled.py)
+        self.act8_checkpoints = False
         # optimiser / schedule (:104, 113-114, 219)
         self.num_epochs = 100
         self.num_train_batches = 200 if dim == 2 else 200

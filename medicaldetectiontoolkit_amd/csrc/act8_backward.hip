@@ -191,7 +191,6 @@ __device__ __forceinline__ void dgrad_tile(uint16_t *smem, const Args &a, const 
         }
         if (k0 + DEPTH * KSTEP < ke) load(G, Y, W, k0 + DEPTH * KSTEP);
         __syncthreads();
-        if (a.gx == nullptr) return;
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
             v8bf A[TM][3], B[TN][3];
@@ -219,7 +218,6 @@ __device__ __forceinline__ void dgrad_tile(uint16_t *smem, const Args &a, const 
 #pragma unroll
         for (int d = 0; d < DEPTH; ++d) if (k0 + d * KSTEP < ke) step(G[d], Y[d], W[d], k0 + d * KSTEP);
     }
-    if (a.gx == nullptr) return;
 #pragma unroll
     for (int n = 0; n < TN; ++n) {
         const long long v = v0 + wv + n * 32 + lo;
@@ -380,7 +378,7 @@ __device__ __forceinline__ void wgrad_tile(uint16_t *smem, const Args &a, const 
 }
 
 // arrays of less than 4 values, which the loads of 4 above cannot read: an element of gx or gw a thread, gbias and g in plain loops
-__global__ __launch_bounds__(THREADS) void tiny_kernel(Args a, float *__restrict__ gw, float *__restrict__ gb)
+__global__ __launch_bounds__(THREADS) void conv1x1_bwd_act8_tiny(Args a, float *__restrict__ gw, float *__restrict__ gb)
 {
     const long long e = (long long)blockIdx.x * THREADS + threadIdx.x, nx = a.V * a.ci, nw = (long long)a.co * a.ci, ng = a.V * a.co;
     auto g_at = [&](long long v, int o) { return a.yc == nullptr || a.yc[v * a.co + o] ? a.gy[v * a.co + o] : 0.0f; };
@@ -406,7 +404,7 @@ __global__ __launch_bounds__(THREADS) void tiny_kernel(Args a, float *__restrict
 
 // one launch for the two products, which do not depend on each other: the first groups sum voxels, the others channels
 template <int W0, int W1, int W2, int W3, int D0, int D1, int D2, int D3, bool EVEN>
-__global__ __launch_bounds__(THREADS, 2) void products_kernel(Args a, WgradGrid wg, DgradGrid dg)
+__global__ __launch_bounds__(THREADS, 2) void conv1x1_bwd_act8_products(Args a, WgradGrid wg, DgradGrid dg)
 {
     constexpr int LW = (W0 * W1 * 3 + W2 * W3) * 32 * KROW, LD = (D0 * D1 + D2 * D3) * 3 * 32 * KROW;
     __shared__ __attribute__((aligned(16))) uint16_t smem[LW > LD ? LW : LD];
@@ -417,7 +415,7 @@ __global__ __launch_bounds__(THREADS, 2) void products_kernel(Args a, WgradGrid 
 // out[e] = sum over the splits of part[split][e] in a fixed order, for up to three arrays at once.  A workgroup sums 1024 >> log_r elements, each in 1 << log_r
 // interleaved ranges of splits.  512 partial sums of 18 x 72 weights with 8 ranges: 21 us, with 32: 5 us.
 struct Joined { const float *part; float *out; long long n; int splits, log_r; long long groups; };
-__global__ __launch_bounds__(1024) void join_kernel(Joined j0, Joined j1, Joined j2)
+__global__ __launch_bounds__(1024) void conv1x1_bwd_act8_join(Joined j0, Joined j1, Joined j2)
 {
     __shared__ float s[1024];
     long long id = blockIdx.x;
@@ -454,8 +452,108 @@ int join_run(const Joined &a, const Joined &b, const Joined &c, hipStream_t s)
 {
     const long long groups = a.groups + b.groups + c.groups;
     if (groups >= (1LL << 22)) return MDT_ERR_UNSUPPORTED;                        // 2^32 threads are the most of a launch
-    if (groups > 0) join_kernel<<<dim3((unsigned)groups), 1024, 0, s>>>(a, b, c);
+    if (groups > 0) conv1x1_bwd_act8_join<<<dim3((unsigned)groups), 1024, 0, s>>>(a, b, c);
     return MDT_OK;
+}
+
+// ---- no product wanted: the mask and the sum of columns -----------------------------------------------------------------------------------------
+// g = gy . m and gbias for a layer whose products other kernels take (a window, a stride).  5 bytes read and 4 written a value.
+// A workgroup walks over its run of quads of values in steps of `active` quads, a multiple of the period after which quads begin at the same channel again: a thread's 4
+// sums belong to the same 4 channels throughout, whatever the number of channels, as long as the period fits into a workgroup.
+constexpr int SUM_ROWS = 1024;                                                   // partial sums of a channel at most
+
+template <bool MASK>
+__global__ __launch_bounds__(THREADS) void act8_mask_sum_quads(const float *__restrict__ gy, const uint8_t *__restrict__ yc, float *__restrict__ g, float *__restrict__ part, long long n,
+                                                               int C, int active, long long per)
+{
+    __shared__ __attribute__((aligned(16))) float s[4 * THREADS];
+    const int t = threadIdx.x;
+    const long long nq = n / 4, q0 = blockIdx.x * per, q1 = min(q0 + per, nq);
+    v4f sum = {};
+    if (t < active)
+        for (long long q = q0 + t; q < q1; q += 4 * active) {
+            v4f v[4];
+            unsigned m[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const long long at = 4 * min(q + u * active, nq - 1);
+                if (MASK) m[u] = get4(yc + at);
+                v[u] = get4(gy + at);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                if (q + u * active >= q1) break;
+                if (MASK) v[u] = masked(v[u], m[u]);
+                if (g != nullptr) *reinterpret_cast<Io<float>::vec *>(g + 4 * (q + u * active)) = v[u];
+                sum = sum + v[u];
+            }
+        }
+    *reinterpret_cast<v4f *>(s + 4 * t) = sum;
+    __syncthreads();
+    const int behind = blockIdx.x == gridDim.x - 1 ? (int)(n - 4 * nq) : 0;        // values behind the last quad
+    for (int c = t; c < C; c += THREADS) {
+        float b = 0.0f;
+        for (int e = c; e < 4 * active; e += C) b = b + s[e];
+        for (int k = 0; k < behind; ++k) {
+            const long long e = 4 * nq + k;
+            if (e % C != c) continue;
+            const float v = !MASK || yc[e] ? gy[e] : 0.0f;
+            if (g != nullptr) g[e] = v;
+            b = b + v;
+        }
+        if (part != nullptr) part[(long long)blockIdx.x * C + c] = b;
+    }
+}
+
+// channels whose period is longer than a workgroup: a thread a column
+template <bool MASK>
+__global__ __launch_bounds__(THREADS) void act8_mask_sum_columns(const float *__restrict__ gy, const uint8_t *__restrict__ yc, float *__restrict__ g, float *__restrict__ part, long long V,
+                                                                 int C, long long per)
+{
+    const int c = blockIdx.x * THREADS + threadIdx.x;
+    const long long v0 = blockIdx.y * per, v1 = min(v0 + per, V);
+    if (c >= C) return;
+    float sum = 0.0f;
+    for (long long r = v0; r < v1; r += 4) {
+        float v[4];
+        uint8_t m[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const long long at = min(r + u, V - 1) * C + c;
+            if (MASK) m[u] = yc[at];
+            v[u] = gy[at];
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            if (r + u >= v1) break;
+            if (MASK && !m[u]) v[u] = 0.0f;
+            if (g != nullptr) g[(r + u) * C + c] = v[u];
+            sum = sum + v[u];
+        }
+    }
+    if (part != nullptr) part[blockIdx.y * (long long)C + c] = sum;
+}
+
+struct SumPlan { int active, rows; long long per; };                              // active 0: a thread a column
+
+inline SumPlan sum_plan(long long V, int C)
+{
+    SumPlan p;
+    const int period = C % 4 == 0 ? C / 4 : C % 2 == 0 ? C / 2 : C;
+    p.active = period <= THREADS ? THREADS / period * period : 0;
+    const long long units = p.active ? (V * C + 4LL * p.active - 1) / (4LL * p.active) : V, columns = (C + THREADS - 1) / THREADS, most = p.active ? SUM_ROWS : (SUM_ROWS + columns - 1) / columns;
+    const long long rows = (units + 3) / 4 < most ? (units + 3) / 4 : most;
+    const long long each = (units + rows - 1) / rows;
+    p.per = p.active ? each * p.active : each;
+    p.rows = (int)((units + each - 1) / each);
+    return p;
+}
+
+template <bool MASK>
+void sum_run(const SumPlan &p, const Args &a, hipStream_t s)
+{
+    if (p.active) act8_mask_sum_quads<MASK><<<p.rows, THREADS, 0, s>>>(a.gy, a.yc, a.g, a.part_b, a.V * a.co, a.co, p.active, p.per);
+    else act8_mask_sum_columns<MASK><<<dim3((a.co + THREADS - 1) / THREADS, p.rows), THREADS, 0, s>>>(a.gy, a.yc, a.g, a.part_b, a.V, a.co, p.per);
 }
 
 // floats of one wave's LDS tiles: 32 voxels of gradients (and a row's overhang; gx's rows take the same place later), 32 of bf16 inputs (and theirs)
@@ -472,7 +570,7 @@ __host__ __device__ constexpr int fused_wave_floats(int mt, int nt, int ci, int 
 // Entries of the tiles behind co or ci hold whatever follows in LDS: they only reach rows and columns that are not stored, except along gx's sum, where
 // they are set to zero.
 template <int MT, int NT, bool G_OUT>
-__global__ __launch_bounds__(THREADS, MT * NT <= 3 ? 2 : 1) void fused_kernel(const float *__restrict__ gy, const uint8_t *__restrict__ yc, const float *__restrict__ w,
+__global__ __launch_bounds__(THREADS, MT * NT <= 3 ? 2 : 1) void conv1x1_bwd_act8_fused(const float *__restrict__ gy, const uint8_t *__restrict__ yc, const float *__restrict__ w,
                                                                              const uint8_t *__restrict__ xc, const uint8_t *__restrict__ xs, float *__restrict__ gx,
                                                                              float *__restrict__ g_out, float *__restrict__ part_w, float *__restrict__ part_b, long long V, int ci, int co,
                                                                              int x_relu)
@@ -737,8 +835,8 @@ void products_launch(const Plan &p, const Args &a, hipStream_t s)
 {
     const dim3 grid((unsigned)(p.wg.groups + p.dg.groups));
     const bool even = a.ci % 4 == 0;                                            // 4 input codes of a voxel lie in one block
-    const auto kernel = p.d_tile == 128 ? (even ? products_kernel<W0, W1, W2, W3, 2, 2, 2, 2, true> : products_kernel<W0, W1, W2, W3, 2, 2, 2, 2, false>)
-                                        : (even ? products_kernel<W0, W1, W2, W3, 2, 1, 2, 1, true> : products_kernel<W0, W1, W2, W3, 2, 1, 2, 1, false>);
+    const auto kernel = p.d_tile == 128 ? (even ? conv1x1_bwd_act8_products<W0, W1, W2, W3, 2, 2, 2, 2, true> : conv1x1_bwd_act8_products<W0, W1, W2, W3, 2, 2, 2, 2, false>)
+                                        : (even ? conv1x1_bwd_act8_products<W0, W1, W2, W3, 2, 1, 2, 1, true> : conv1x1_bwd_act8_products<W0, W1, W2, W3, 2, 1, 2, 1, false>);
     kernel<<<grid, THREADS, 0, s>>>(a, p.wg, p.dg);
 }
 
@@ -764,7 +862,7 @@ inline FusedPlan fused_plan(long long V, int ci, int co)
 template <int MT, int NT>
 int fused_launch(const FusedPlan &p, const Args &a, hipStream_t s)
 {
-    const auto kernel = a.g != nullptr ? fused_kernel<MT, NT, true> : fused_kernel<MT, NT, false>;
+    const auto kernel = a.g != nullptr ? conv1x1_bwd_act8_fused<MT, NT, true> : conv1x1_bwd_act8_fused<MT, NT, false>;
     if (hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, p.lds) != hipSuccess) return MDT_ERR_LAUNCH_FAILED;
     kernel<<<p.blocks, THREADS, p.lds, s>>>(a.gy, a.yc, a.w, a.xc, a.xs, a.gx, a.g, a.part_w, a.part_b, a.V, a.ci, a.co, a.x_relu);
     return MDT_OK;
@@ -804,7 +902,8 @@ size_t mdt_conv1x1_act8_backward_workspace_bytes(long long n_voxels, int c_in, i
     const Plan q = plan_of(n_voxels, c_in, c_out);
     const FusedPlan p = fused_plan(n_voxels, c_in, c_out);
     const long long one = (long long)c_in * c_out + c_out, tiled = q.wg.splits * one + (q.dg.k_splits > 1 ? q.dg.k_splits * n_voxels * c_in : 0);
-    return (size_t)(tiled > p.blocks * one ? tiled : p.blocks * one) * 4 + 256;
+    const long long fused = p.blocks * one, sums = (long long)sum_plan(n_voxels, c_out).rows * c_out, more = tiled > fused ? tiled : fused;
+    return (size_t)(more > sums ? more : sums) * 4 + 256;
 }
 
 int mdt_conv1x1_act8_backward(const float *gy, const float *w, const void *x_codes, const void *x_scales, int x_relu, const void *y_codes, float *gx, float *gw, float *gbias, float *g,
@@ -832,8 +931,19 @@ int mdt_conv1x1_act8_backward(const float *gy, const float *w, const void *x_cod
     }
     if (V * c_in < 4 || V * c_out < 4) {
         const long long n = V * c_in + nw + c_out + V * c_out;
-        tiny_kernel<<<dim3((unsigned)((n + THREADS - 1) / THREADS)), THREADS, 0, s>>>(a, gw, gbias);
+        conv1x1_bwd_act8_tiny<<<dim3((unsigned)((n + THREADS - 1) / THREADS)), THREADS, 0, s>>>(a, gw, gbias);
         return launch_check();
+    }
+    if (gx == nullptr && (g != nullptr || gw == nullptr)) {
+        if (g == nullptr && gbias == nullptr) return launch_check();
+        const SumPlan sp = sum_plan(V, c_out);
+        a.part_b = gbias ? a.part_w : nullptr;
+        if (y_codes) sum_run<true>(sp, a, s);
+        else sum_run<false>(sp, a, s);
+        const int rc = join_run(joined(a.part_b, gbias, c_out, sp.rows), none, none, s);
+        if (rc != MDT_OK || gw == nullptr) return rc != MDT_OK ? rc : launch_check();
+        a.g = g = nullptr;
+        gbias = nullptr;
     }
     Plan p = plan_of(V, c_in, c_out);
     a.part_b = a.part_w + p.wg.splits * nw;
@@ -843,10 +953,9 @@ int mdt_conv1x1_act8_backward(const float *gy, const float *w, const void *x_cod
         p.wg.groups = sums ? p.wg.groups / p.wg.ci_tiles : 0;
         p.wg.ci_tiles = 1;
     }
-    if (gx == nullptr) {                                                         // g alone: one column of tiles, unsplit
-        p.dg.groups = g ? p.dg.groups / (p.dg.ci_tiles * p.dg.k_splits) : 0;
-        p.dg.ci_tiles = p.dg.k_splits = 1;
-        p.dg.k_per = (c_out + KSTEP - 1) / KSTEP * KSTEP;
+    if (gx == nullptr) {
+        p.dg.groups = 0;
+        p.dg.k_splits = 1;
     }
     p.dg.to = p.dg.k_splits > 1 ? part_x : gx;
     if (p.wg.groups + p.dg.groups >= (1LL << 24)) return MDT_ERR_UNSUPPORTED;    // 2^32 threads are the most of a launch

@@ -97,7 +97,7 @@ struct WTiled {
 };
 
 // a workgroup of 64 lanes x 4: one 16-row tile of 4 chunks
-__global__ __launch_bounds__(256) void tile_weights_kernel(const uint8_t *__restrict__ wc, const uint8_t *__restrict__ ws, uint8_t *__restrict__ tc, uint8_t *__restrict__ ts, int n, int kb,
+__global__ __launch_bounds__(256) void mx4_tile_weights(const uint8_t *__restrict__ wc, const uint8_t *__restrict__ ws, uint8_t *__restrict__ tc, uint8_t *__restrict__ ts, int n, int kb,
                                                            int chunks)
 {
     const int c = blockIdx.x * 4 + (threadIdx.x >> 6), l = threadIdx.x & 63, tile = blockIdx.y;
@@ -186,7 +186,6 @@ struct XRows {
     static __device__ __forceinline__ unsigned round16(const vec &t, int &b)
     {
         typedef uint16_t u2 __attribute__((ext_vector_type(2)));
-        typedef T t2 __attribute__((ext_vector_type(2)));
         const v4u whole = __builtin_bit_cast(v4u, t);
         const unsigned p[4] = {whole[0], whole[1], whole[2], whole[3]};             // (a bit_cast of a vector's element would take the first one)
         u2 m = __builtin_bit_cast(u2, p[0] & 0x7fff7fffu);
@@ -243,7 +242,7 @@ __device__ __forceinline__ T finish(float v, float add, int relu)
 }
 
 template <typename T, int TN, class W, bool TINY>
-__global__ __launch_bounds__(THREADS, 2) void narrow_kernel(const T *__restrict__ x, const uint8_t *__restrict__ wc, const uint8_t *__restrict__ ws, const float *__restrict__ bias,
+__global__ __launch_bounds__(THREADS, 2) void mx4_linear_narrow(const T *__restrict__ x, const uint8_t *__restrict__ wc, const uint8_t *__restrict__ ws, const float *__restrict__ bias,
                                                             T *__restrict__ y, long long rows, long long k, int n, int n_tiles, int relu)
 {
     constexpr int LOADS = 16 / (64 / (CHUNK / Io<T>::GV)), LDS_X = 16 * (ROW_BYTES + CHUNK_BLOCKS), LDS_SUM = 16 * TN * 16 * 4;
@@ -308,7 +307,7 @@ __global__ __launch_bounds__(THREADS, 2) void narrow_kernel(const T *__restrict_
 }
 
 template <typename T, int TM, int TN>
-__global__ __launch_bounds__(THREADS, 2) void wide_kernel(const T *__restrict__ x, const uint8_t *__restrict__ wc, const uint8_t *__restrict__ ws, const float *__restrict__ bias,
+__global__ __launch_bounds__(THREADS, 2) void mx4_linear_wide(const T *__restrict__ x, const uint8_t *__restrict__ wc, const uint8_t *__restrict__ ws, const float *__restrict__ bias,
                                                           T *__restrict__ y, long long rows, long long k, int n, int n_tiles, int relu)
 {
     constexpr int BM = 16 * TM, MINE = BM / WAVES, LOADS = MINE / (64 / (CHUNK / Io<T>::GV));    // MINE: rows of x a wave rounds
@@ -406,7 +405,7 @@ int narrow(const Call &a)
     const int tiles = (a.n + 16 * TN - 1) / (16 * TN);
     const long long groups = (a.rows + 15) / 16 * tiles;
     if (groups >= (1LL << 23)) return MDT_ERR_UNSUPPORTED;                         // 2^32 threads are the most of a launch
-    narrow_kernel<T, TN, W, TINY><<<dim3((unsigned)groups), THREADS, 0, a.s>>>((const T *)a.x, a.wc, a.ws, a.bias, (T *)a.y, a.rows, a.k, a.n, tiles, a.relu);
+    mx4_linear_narrow<T, TN, W, TINY><<<dim3((unsigned)groups), THREADS, 0, a.s>>>((const T *)a.x, a.wc, a.ws, a.bias, (T *)a.y, a.rows, a.k, a.n, tiles, a.relu);
     return launch_check();
 }
 
@@ -416,7 +415,7 @@ int wide(const Call &a)
     const int tiles = (a.n + 128 * TN - 1) / (128 * TN);
     const long long groups = (a.rows + 16 * TM - 1) / (16 * TM) * tiles;
     if (groups >= (1LL << 23)) return MDT_ERR_UNSUPPORTED;
-    wide_kernel<T, TM, TN><<<dim3((unsigned)groups), THREADS, 0, a.s>>>((const T *)a.x, a.wc, a.ws, a.bias, (T *)a.y, a.rows, a.k, a.n, tiles, a.relu);
+    mx4_linear_wide<T, TM, TN><<<dim3((unsigned)groups), THREADS, 0, a.s>>>((const T *)a.x, a.wc, a.ws, a.bias, (T *)a.y, a.rows, a.k, a.n, tiles, a.relu);
     return launch_check();
 }
 
@@ -463,7 +462,7 @@ int run(Call a, uint8_t *workspace)
 {
     if (copies_w(a.rows, a.k, a.n)) {
         const Tiled t = tiled_of(a.k, a.n);
-        tile_weights_kernel<<<dim3((t.chunks + 3) / 4, t.tiles), 256, 0, a.s>>>(a.wc, a.ws, workspace, workspace + t.codes, a.n, (int)((a.k + BLOCK - 1) / BLOCK), t.chunks);
+        mx4_tile_weights<<<dim3((t.chunks + 3) / 4, t.tiles), 256, 0, a.s>>>(a.wc, a.ws, workspace, workspace + t.codes, a.n, (int)((a.k + BLOCK - 1) / BLOCK), t.chunks);
         a.wc = workspace;
         a.ws = workspace + t.codes;
         if (!is_wide(a.rows, a.k, a.n)) return narrow_by_columns<T, WTiled>(a);

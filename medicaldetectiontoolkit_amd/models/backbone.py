@@ -6,7 +6,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from ..utils import fused_epilogue
+from ..utils import block_scaled, fused_epilogue
 from ..utils.fused_epilogue import ConvBias
 
 
@@ -82,6 +82,9 @@ class FPN(nn.Module):
         self.n_blocks = [3, 4, {"resnet50": 6, "resnet101": 23}[cf.res_architecture], 3]
         self.block_expansion = 4
         self.operate_stride1 = operate_stride1
+        self.act8 = bool(getattr(cf, "act8_checkpoints", False))
+        if self.act8 and (cf.norm is not None or cf.relu != "relu"):
+            raise ValueError("act8_checkpoints: layers without a norm and with ReLU, not norm=%r relu=%r" % (cf.norm, cf.relu))
         self.sixth_pooling = cf.sixth_pooling
         self.dim = conv.dim
         s1 = (2, 2, 1) if conv.dim == 3 else 2
@@ -146,7 +149,7 @@ class FPN(nn.Module):
             return out, x_lat
         return seq(x), x
 
-    def forward(self, x):
+    def _c0(self, x):
         if self.operate_stride1:
             # a ONE-channel image is "contiguous" in both layouts, so MIOpen returns C0[0]'s 18-channel output row-major even in a
             # channels-last net -- and C0[1] (18 -> 18 on the full-resolution volume, the most expensive layer of the Retina U-Net step)
@@ -157,9 +160,64 @@ class FPN(nn.Module):
             mf = torch.channels_last_3d if h.dim() == 5 else torch.channels_last
             if w1.is_contiguous(memory_format=mf) and not w1.is_contiguous() and not h.is_contiguous(memory_format=mf):
                 h = h.contiguous(memory_format=mf)
-            c0_out = self.C0[1](h)
+            return self.C0[1](h)
+        return x
+
+    @staticmethod
+    def _stage8(blocks, x, x8):
+        """Residual blocks on x with its 8-bit copy x8: (output, its copy, what the lateral of x's level must read).  Every layer's autograd node holds 8-bit copies in
+        place of the fp32 maps; strided first blocks run on a sub-sampled copy (fused_epilogue.stride_tap)."""
+        x_lat, conv8 = x, block_scaled.conv_bias_act8
+        for i, blk in enumerate(blocks):
+            strided = any(int(v) > 1 for v in blk.conv1[0].stride)
+            if strided:
+                tap, x = fused_epilogue.stride_tap(x, blk.conv1[0].stride)
+                x_lat = tap if i == 0 else x_lat
+                x8 = block_scaled.checkpoint8(x, relu=True)
+            res = x if blk.downsample is None else conv8(blk.downsample, x, x8, keep=False, subsampled=strided)[0]
+            h, h8 = conv8(blk.conv1[0], x, x8, relu=True, subsampled=strided)
+            h, h8 = conv8(blk.conv2[0], h, h8, relu=True)
+            x, x8 = conv8(blk.conv3, h, h8, residual=res, relu=True)
+        return x, x8, x_lat
+
+    def _forward8(self, x):
+        """forward with cf.act8_checkpoints: the same values; the residual stages, the laterals and the P convolutions keep 8-bit copies for the backward pass"""
+        conv8, up = block_scaled.conv_bias_act8, fused_epilogue.upsample_nearest
+        c0_out = self._c0(x)
+        c1_out = None
+        if not self.operate_stride1 and fused_epilogue.stem_pool_fused_applies(self.C1, self.C2[0], c0_out):
+            h = fused_epilogue.conv_stem_bias_relu_pool(self.C1, c0_out)
         else:
-            c0_out = x
+            c1_out = self.C1(c0_out)
+            h = self.C2[0](c1_out)
+        mf = torch.channels_last_3d if h.dim() == 5 else torch.channels_last
+        if not h.is_contiguous(memory_format=mf):
+            h = h.contiguous(memory_format=mf)
+        h8 = block_scaled.checkpoint8(h, relu=True)
+        levels = []                                     # (what the lateral reads, its copy) of C2 ...
+        for i, seq in enumerate([list(self.C2)[1:], self.C3, self.C4, self.C5] + ([self.C6] if self.sixth_pooling else [])):
+            below = (h8,)
+            h, h8, lat = self._stage8(seq, h, h8)
+            if i > 0:
+                levels.append((lat,) + below)
+        levels.append((h, h8))
+        ones = [self.P2_conv1, self.P3_conv1, self.P4_conv1, self.P5_conv1] + ([self.P6_conv1] if self.sixth_pooling else [])
+        threes = [self.P2_conv2, self.P3_conv2, self.P4_conv2, self.P5_conv2] + ([self.P6_conv2] if self.sixth_pooling else [])
+        pre, outs = None, []
+        for (c, c8), one, three in zip(reversed(levels), reversed(ones), reversed(threes)):
+            pre, pre8 = conv8(one, c, c8, residual=None if pre is None else up(pre, 2))
+            outs.append(conv8(three, pre, pre8, keep=False)[0])
+        outs = outs[::-1]
+        if self.operate_stride1:
+            p1_pre_out = _lateral(self.P1_conv1, c1_out, self.P2_upsample(pre))
+            p0_pre_out = _lateral(self.P0_conv1, c0_out, self.P1_upsample(p1_pre_out))
+            outs = [p0_pre_out if getattr(self, "defer_p0_conv2", False) else self.P0_conv2(p0_pre_out)] + outs
+        return outs
+
+    def forward(self, x):
+        if self.act8 and torch.is_grad_enabled() and not torch.is_autocast_enabled():
+            return self._forward8(x)
+        c0_out = self._c0(x)
         if not self.operate_stride1 and fused_epilogue.stem_pool_fused_applies(self.C1, self.C2[0], c0_out):
             # the stem output has ONE consumer here (the pooling in front of C2): one autograd node for stem + bias + ReLU + pooling, whose backward
             # applies the ReLU mask / bias gradient at the pooled resolution (utils/fused_epilogue._ConvStemBiasReLUPool)

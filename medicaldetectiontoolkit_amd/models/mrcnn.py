@@ -25,6 +25,7 @@ from ..cuda_functions import _roi_align_impl as _rai_mod
 from ..cuda_functions._roi_align_impl import pyramid_crop_and_resize
 from ..cuda_functions.roi_align_2D.roi_align.crop_and_resize import CropAndResizeFunction as ra2D
 from ..cuda_functions.roi_align_3D.roi_align.crop_and_resize import CropAndResizeFunction as ra3D
+from ..utils import block_scaled
 from ..utils import fused_epilogue
 from ..utils import model_utils as mutils
 from . import backbone as backbone_module
@@ -330,6 +331,7 @@ class Classifier(nn.Module):
         self.linear_class = nn.Linear(cf.end_filts * 4, cf.head_classes)
         self.linear_bbox = nn.Linear(cf.end_filts * 4, cf.head_classes * 2 * self.dim)
         self.compact_rows = norm == "batch_norm"
+        self.mx4 = None      # the two filters in 4 bits while utils/block_scaled.mx4_heads lasts
 
     def forward(self, x, rois):
         if self.compact_rows:
@@ -338,7 +340,10 @@ class Classifier(nn.Module):
 
     def _forward(self, x, rois):
         x = pyramid_roi_align(x, rois, self.pool_size, self.pyramid_levels, self.dim)
-        if HEAD_AS_LINEAR and isinstance(self.conv1, fused_epilogue.ConvBiasReLU) and isinstance(self.conv2, fused_epilogue.ConvBiasReLU) \
+        if self.mx4 is not None:
+            x = block_scaled.mx4_linear(x.flatten(1), self.mx4[0], self.conv1[0].bias, relu=True)
+            x = block_scaled.mx4_linear(x, self.mx4[1], self.conv2[0].bias, relu=True)
+        elif HEAD_AS_LINEAR and isinstance(self.conv1, fused_epilogue.ConvBiasReLU) and isinstance(self.conv2, fused_epilogue.ConvBiasReLU) \
                 and tuple(self.conv1[0].kernel_size) == tuple(x.shape[2:]) and not any(self.conv1[0].padding):
             # conv1's kernel IS the pooled extent (mrcnn.py:104) and conv2 is 1x1(x1) on a single voxel: both are matrix products
             # [n, C * ph * pw * pd] x [.., 4C] -- MIOpen's convolution kernels take 1.2 ms for conv1's backward on 48 RoIs

@@ -1,4 +1,5 @@
 """Mirror of the box-consolidation part of the reference's predictor.py, on the gfx950 WBC kernel."""
+import contextlib
 import ctypes
 
 import numpy as np
@@ -191,7 +192,17 @@ def _forward_chunk_dicts(net, batch_t, amp_dtype):
     return np.asarray(rows, dtype=np.float64).reshape(-1, 9), res
 
 
-def collect_raw_boxes(net, data, cf, amp_dtype=None, rank_ix="0", test_aug=False, with_seg=False):
+def _head_context(net, head_dtype):
+    """the context of a prediction's forward passes: head_dtype None (as the net is) or "mx4" (the box head's products in 4 bits)"""
+    if head_dtype is None:
+        return contextlib.nullcontext(net)
+    if head_dtype != "mx4":
+        raise ValueError("head_dtype is None or 'mx4', not %r" % (head_dtype,))
+    from .utils import block_scaled
+    return block_scaled.mx4_heads(net)
+
+
+def collect_raw_boxes(net, data, cf, amp_dtype=None, rank_ix="0", test_aug=False, with_seg=False, head_dtype=None):
     """Patch-tiled forward of one patient WITHOUT consolidation (predictor.py:279-455): returns
     (raw_boxes, info) where raw_boxes is the reference's per-patient box-dict list in patient coordinates, each det
     carrying 'patch_id' = "<rank_ix>_<aug>_<patch>", 'box_patch_center_factor' and 'box_n_overlaps'
@@ -200,7 +211,13 @@ def collect_raw_boxes(net, data, cf, amp_dtype=None, rank_ix="0", test_aug=False
 
     Device-resident: the volume goes up ONCE, patches (and their mirrored versions) are cut on the device, nets that offer
     `test_forward_detections` keep their detections on the device through all chunks and passes (ONE read-out per patient),
-    and patch-centre factor / overlap count / un-mirroring are computed for all boxes at once; box dicts are built at the end."""
+    and patch-centre factor / overlap count / un-mirroring are computed for all boxes at once; box dicts are built at the end.
+    head_dtype="mx4": the box head's products of a Mask R-CNN in 4 bits (utils/block_scaled.py), its filters rounded once for the patient."""
+    with _head_context(net, head_dtype):
+        return _collect_raw_boxes(net, data, cf, amp_dtype, rank_ix, test_aug, with_seg)
+
+
+def _collect_raw_boxes(net, data, cf, amp_dtype, rank_ix, test_aug, with_seg):
     from . import distributed as mdist
     from .utils.dataloader_utils import get_patch_crop_coords
     dim = cf.dim
@@ -331,11 +348,11 @@ def apply_wbc_to_patient(raw_boxes, cf, n_ens, device=None):
     return out
 
 
-def predict_patient(net, data, cf, n_ens=None, amp_dtype=None, rank_ix="0", test_aug=False, with_seg=False):
+def predict_patient(net, data, cf, n_ens=None, amp_dtype=None, rank_ix="0", test_aug=False, with_seg=False, head_dtype=None):
     """data: numpy [C, Y, X, Z] whole-patient volume -> {'boxes': [[box dicts]], ...} like predictor.predict_patient:
     collect_raw_boxes (tiling, optional mirrored passes, gather over ranks) + apply_wbc_to_patient.
-    n_ens defaults to the number of passes (expected predictions per position)."""
-    raw, info = collect_raw_boxes(net, data, cf, amp_dtype=amp_dtype, rank_ix=rank_ix, test_aug=test_aug, with_seg=with_seg)
+    n_ens defaults to the number of passes (expected predictions per position).  head_dtype: see collect_raw_boxes."""
+    raw, info = collect_raw_boxes(net, data, cf, amp_dtype=amp_dtype, rank_ix=rank_ix, test_aug=test_aug, with_seg=with_seg, head_dtype=head_dtype)
     if n_ens is None:
         n_ens = info["n_passes"]
     res = {"boxes": [apply_wbc_to_patient(raw, cf, n_ens, device=net.device_)], "n_patches": info["n_patches"],
@@ -345,7 +362,7 @@ def predict_patient(net, data, cf, n_ens=None, amp_dtype=None, rank_ix="0", test
     return res
 
 
-def predict_test_set(net, patients, cf, checkpoint_paths=None, out_dir=None, test_aug=None, amp_dtype=None):
+def predict_test_set(net, patients, cf, checkpoint_paths=None, out_dir=None, test_aug=None, amp_dtype=None, head_dtype=None):
     """predictor.py:122-216 in miniature: temporal ensembling over saved epochs (each checkpoint = one ensemble member,
     patch ids prefixed with its rank), raw predictions pickled in the reference's format
     ('raw_pred_boxes_list.pickle' = [[boxes_per_batch_element, pid], ...]), then WBC per patient with
@@ -363,7 +380,7 @@ def predict_test_set(net, patients, cf, checkpoint_paths=None, out_dir=None, tes
         if ckpt is not None:
             exp_utils.load_checkpoint(ckpt, net, map_location=net.device_)
         for data, pid in patients:
-            raw, info = collect_raw_boxes(net, data, cf, amp_dtype=amp_dtype, rank_ix=str(rank_ix), test_aug=test_aug)
+            raw, info = collect_raw_boxes(net, data, cf, amp_dtype=amp_dtype, rank_ix=str(rank_ix), test_aug=test_aug, head_dtype=head_dtype)
             n_passes = info["n_passes"]
             if pid not in raw_per_patient:
                 raw_per_patient[pid] = []

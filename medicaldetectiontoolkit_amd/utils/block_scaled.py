@@ -10,16 +10,25 @@ back as NaN.
   checkpoint8(x)                      -> Checkpoint8, .restore()      any float32 / bfloat16 / float16 tensor, 33 bytes for 32 values
   bias_act_checkpoint8(h, bias, res)  -> (y, Checkpoint8 of y)        the convolution epilogue of utils/fused_epilogue.bias_act that keeps the copy
   conv1x1_backward8(gy, w, x8, y8)    -> gradients of a 1x1(x1) layer from the kept copies of its input and its output
+  conv_bias_act8(conv, x, x8, ...)    -> (y, y8)                      a convolution layer of the autograd graph that keeps x8 and y8 in place of x and y
   mx4_quantize(x) -> Mx4, .dequantize();  mx4_linear(x, w4, bias)     act(x W^T + bias) with both operands in 4 bits (inference)
+  mx4_heads(net)                                                      a Mask R-CNN's box head on mx4_linear while the context lasts
+
+What calls them: models/backbone.FPN with cf.act8_checkpoints (train.py --act8 1), predictor.predict_patient / predict_test_set with head_dtype="mx4".
 
 Like every operator of this package they run on the GPU only and are queued on the current stream of the tensors' device; a tensor that was made on
 another stream is the caller's to synchronise, as with any torch operator.  Their scratch memory comes from torch's allocator for each call, so
 calls on several streams and captured graphs do not share any."""
+import contextlib
 import math
 
 import torch
+import torch.nn.functional as F
+from torch.autograd import Function
+from torch.autograd.function import once_differentiable
 
 from .. import _lib
+from . import fused_epilogue
 
 BLOCK = 32
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
@@ -146,6 +155,19 @@ class Checkpoint8(object):
         at = self.buffer.data_ptr()
         return at, at + _scales_at(math.prod(self.shape))
 
+    def tensors(self):
+        """what holds the copy, for Function.save_for_backward: of_tensors puts it together again"""
+        return (self._codes, self._scales) if self.buffer is None else (self.buffer,)
+
+    def meta(self):
+        return self.shape, self.relu, self.dtype, self.channels_last
+
+    @classmethod
+    def of_tensors(cls, tensors, meta):
+        if len(tensors) == 1:
+            return cls.of_buffer(tensors[0], *meta)
+        return cls.__new__(cls)._set(None, tensors[0], tensors[1], *meta, tensors[0].device)
+
     @property
     def stride(self):
         return _channels_last_stride(self.shape) if self.channels_last else _row_stride(self.shape)
@@ -240,6 +262,113 @@ def conv1x1_backward8(gy, w, x8, y8=None, need_g=False, need_gx=True, need_gw=Tr
     return gx, gw, gbias, (g if write_g else gy if need_g else None)
 
 
+def act_backward8(gy, y8):
+    """(g, gbias) of an activation from its kept output: g = gy * (y > 0), gbias = the sum of g over everything but axis 1.  gy: float32, in any storage order"""
+    if gy.dtype != torch.float32:
+        raise TypeError("act_backward8: float32 gradients")
+    _lib.require_cuda(gy, "gy")
+    if gy.dim() not in (2, 4, 5) or y8.shape != tuple(gy.shape) or not y8.relu or not y8.channels_last:
+        raise ValueError("act_backward8: y8 is the kept ReLU output of gy's shape, channels innermost")
+    dev = gy.device
+    _same_device(dev, y8=y8)
+    mf = _rows_format(gy.dim())
+    if not gy.is_contiguous(memory_format=mf):
+        gy = gy.contiguous(memory_format=mf)
+    co = int(gy.shape[1])
+    V = gy.numel() // co
+    g = torch.empty_like(gy)
+    gbias = torch.empty(co, dtype=torch.float32, device=dev)
+    ws = torch.empty(_lib.lib().mdt_conv1x1_act8_backward_workspace_bytes(V, 1, co), dtype=torch.uint8, device=dev)
+    _call(dev, "mdt_conv1x1_act8_backward", gy.data_ptr(), None, None, None, 0, y8.pointers()[0], None, None, gbias.data_ptr(), g.data_ptr(), V, 1, co, ws.data_ptr(), ws.numel())
+    return g, gbias
+
+
+class _ConvBiasAct8(Function):
+    """y = act(conv(x) + bias (+ residual)) whose backward pass finds x and y in 8 bits: a quarter of the memory that autograd would hold from the forward pass to the
+    backward pass.  The forward values are those of the fp32 layer; the ReLU's mask, the input gradient and the bias gradient are exact, the weight
+    gradient is taken with the kept x (off by at most half a step of its block)."""
+
+    @staticmethod
+    def forward(ctx, x, w, bias, residual, x8, relu, keep, padding):
+        nd = w.dim() - 2
+        mf = _rows_format(x.dim())
+        if residual is not None and not residual.is_contiguous(memory_format=mf):
+            residual = residual.contiguous(memory_format=mf)
+        one = math.prod(w.shape[2:]) == 1
+        y = y8 = None
+        if one and x.numel() >= (1 << 20) and x.data_ptr() % 16 == 0 and _lib.lib().mdt_conv1x1_forward_supported(int(w.shape[1]), int(w.shape[0])):
+            y = fused_epilogue._conv1x1_forward(x, w, bias, residual, relu)
+        elif nd == 3 and residual is None and padding == (1, 1, 1) and not x.is_contiguous():
+            y = fused_epilogue.conv3x3x3_small(x, w, bias.detach(), relu)
+        if y is None:
+            h = (F.conv3d if nd == 3 else F.conv2d)(x, w, None, 1, padding)
+            if not h.is_contiguous(memory_format=mf):
+                h = h.contiguous(memory_format=mf)
+            if relu or keep:
+                y, y8 = bias_act_checkpoint8(h, bias, residual, relu=relu, inplace=True)
+            else:
+                y = fused_epilogue.bias_act(h, bias, residual, False)
+        elif relu or keep:
+            y8 = checkpoint8(y, relu=relu)
+        kept = x8.tensors()
+        ctx.x8, ctx.n_x8, ctx.y8 = x8.meta(), len(kept), y8.meta() if relu else None
+        ctx.save_for_backward(w, *kept, *(y8.tensors() if relu else ()))
+        ctx.has_res, ctx.padding, ctx.one = residual is not None, padding, one
+        return y, y8
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy, _gy8):
+        w, kept = ctx.saved_tensors[0], ctx.saved_tensors[1:]
+        x8 = Checkpoint8.of_tensors(kept[:ctx.n_x8], ctx.x8)
+        y8 = Checkpoint8.of_tensors(kept[ctx.n_x8:], ctx.y8) if ctx.y8 is not None else None
+        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
+        if ctx.one:
+            gx, gw, gbias, g = conv1x1_backward8(gy, w, x8, y8, need_g=ctx.has_res and need_r, need_gx=need_x, need_gw=need_w)
+        else:
+            mf = _rows_format(gy.dim())
+            g, gbias = act_backward8(gy, y8) if y8 is not None else fused_epilogue._bias_act_bwd(gy, None, False, mf)
+            gx, gw = fused_epilogue._stride1_grads(x8.restore() if need_w else _like(x8), w, ctx.padding, g, need_x, need_w)
+        return gx, gw, (gbias if need_b else None), (g if ctx.has_res and need_r else None), None, None, None, None
+
+
+def _like(x8):
+    """an uninitialised tensor of the kept map's shape and storage order, where only those are asked for"""
+    return torch.empty_strided(x8.shape, x8.stride, dtype=x8.dtype, device=x8.device)
+
+
+def conv_bias_act8(conv, x, x8=None, residual=None, relu=False, keep=True, subsampled=False):
+    """(y, y8) for y = act(conv(x) + bias (+ residual)) of a size-preserving convolution module (unit stride; subsampled=True: a strided 1x1 layer whose
+    input was sub-sampled already): the autograd node keeps x8, x's 8-bit copy (None: one is made), and y's in place of x and y.  y8 is what the next
+    layer takes as its x8; keep=False: there is none (an output that no further layer of this kind reads; None where there is no activation either).
+    float32 maps on the GPU; a row-major x is copied to channels-last."""
+    for name, ok in (("a bias", conv.bias is not None), ("one group", conv.groups == 1), ("unit dilation", all(int(v) == 1 for v in conv.dilation)),
+                     ("zero padding", conv.padding_mode == "zeros" and not isinstance(conv.padding, str)),
+                     ("a size-preserving window", not isinstance(conv.padding, str) and all(2 * int(p) + 1 == int(k) for p, k in zip(conv.padding, conv.kernel_size))),
+                     ("unit stride", subsampled or all(int(v) == 1 for v in conv.stride))):
+        if not ok:
+            raise ValueError("conv_bias_act8: a convolution with %s" % name)
+    _float_tensor(x, "x")
+    if x.dtype != torch.float32 or conv.weight.dtype != torch.float32 or torch.is_autocast_enabled():
+        raise TypeError("conv_bias_act8: float32 training, not under autocast")
+    if x.dim() != conv.weight.dim() or int(x.shape[1]) != int(conv.weight.shape[1]):
+        raise ValueError("conv_bias_act8: x %s does not fit the filter %s" % (tuple(x.shape), tuple(conv.weight.shape)))
+    shape = (x.shape[0], conv.weight.shape[0]) + tuple(x.shape[2:])
+    if residual is not None and (tuple(residual.shape) != tuple(shape) or residual.dtype != torch.float32):
+        raise ValueError("conv_bias_act8: residual %s, output %s" % (tuple(residual.shape), tuple(shape)))
+    _same_device(x.device, weight=conv.weight, residual=residual, x8=x8)
+    if x.device.index != torch.cuda.current_device():
+        raise RuntimeError("conv_bias_act8: x is not on the current device (one process per GPU)")
+    mf = _rows_format(x.dim())
+    if not x.is_contiguous(memory_format=mf):
+        x = x.contiguous(memory_format=mf)
+    if x8 is None:
+        x8 = checkpoint8(x)
+    if x8.shape != tuple(x.shape) or not x8.channels_last or x8.dtype != torch.float32:
+        raise ValueError("conv_bias_act8: x8 is x's copy, channels innermost: %s for x %s" % (x8.shape, tuple(x.shape)))
+    return _ConvBiasAct8.apply(x, conv.weight, conv.bias, residual, x8, bool(relu), bool(keep), tuple(int(p) for p in conv.padding))
+
+
 class Mx4(object):
     """Rows in 4 bits: `codes` uint8 [..., ceil(k / 32) * 16] (two a byte, the even value in the low half), `scales` uint8 [..., ceil(k / 32)]; blocks run along
     the last axis of length k."""
@@ -308,3 +437,21 @@ def mx4_linear(x, w4, bias=None, relu=False):
     ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
     _call(x.device, "mdt_mx4_linear", x.data_ptr(), _DTYPES[x.dtype], w4.codes.data_ptr(), w4.scales.data_ptr(), _ptr(bias), y.data_ptr(), rows, k, n, int(relu), _ptr(ws), need)
     return y
+
+
+@contextlib.contextmanager
+def mx4_heads(net):
+    """A Mask R-CNN's box head (the two products of every region, `classifier.conv1` and `conv2`) in 4 bits while the context lasts: the filters are rounded when it is
+    entered, so load a checkpoint before, and not inside.  Inference only: a training step inside raises."""
+    head = getattr(net, "classifier", None)
+    if head is None or not hasattr(head, "mx4"):
+        raise ValueError("mx4_heads: a net with a box head (Mask R-CNN), not %s" % type(net).__name__)
+    if not (isinstance(head.conv1, fused_epilogue.ConvBiasReLU) and isinstance(head.conv2, fused_epilogue.ConvBiasReLU)
+            and tuple(head.conv1[0].kernel_size) == tuple(head.pool_size) and not any(head.conv1[0].padding)):
+        raise ValueError("mx4_heads: the box head's layers are convolution + ReLU without a norm, the first as large as the pooled region")
+    before = head.mx4
+    head.mx4 = tuple(mx4_quantize(c[0].weight.detach().flatten(1)) for c in (head.conv1, head.conv2))
+    try:
+        yield net
+    finally:
+        head.mx4 = before

@@ -149,3 +149,44 @@ def test_shapes_that_do_not_belong_together():
             bs.mx4_quantize(torch.zeros(3, 0))
     finally:
         _lib.require_cuda = real
+
+
+def test_where_the_framework_uses_them():
+    """the options' names and refusals"""
+    from medicaldetectiontoolkit_amd import predictor
+    from medicaldetectiontoolkit_amd.configs import Configs
+    from medicaldetectiontoolkit_amd.models import backbone
+    from medicaldetectiontoolkit_amd.utils.model_utils import NDConvGenerator
+    cf = Configs(dim=2, model="mrcnn", patch_size=[64, 64], batch_size=1)
+    assert cf.act8_checkpoints is False
+    for kw in (dict(norm="batch_norm"), dict(relu="leaky_relu")):
+        cf = Configs(dim=2, model="mrcnn", patch_size=[64, 64], batch_size=1, act8_checkpoints=True, **kw)
+        with pytest.raises(ValueError, match="act8_checkpoints"):
+            backbone.FPN(cf, NDConvGenerator(2))
+    with pytest.raises(ValueError, match="head_dtype"):
+        predictor.predict_patient(None, None, None, head_dtype="int8")
+    with pytest.raises(ValueError, match="box head"):
+        predictor.predict_patient(torch.nn.Linear(2, 2), None, None, head_dtype="mx4")
+    net = torch.nn.Module()
+    net.classifier = torch.nn.Module()
+    with pytest.raises(ValueError, match="box head"):
+        bs.mx4_heads(net).__enter__()
+    net.classifier.mx4 = None
+    net.classifier.conv1 = net.classifier.conv2 = torch.nn.Sequential(torch.nn.Conv2d(2, 2, 1), torch.nn.BatchNorm2d(2))
+    with pytest.raises(ValueError, match="without a norm"):
+        bs.mx4_heads(net).__enter__()
+    with pytest.raises(RuntimeError, match="GPU"):
+        bs.conv_bias_act8(torch.nn.Conv2d(8, 8, 1), torch.zeros(1, 8, 4, 4))
+    with pytest.raises(RuntimeError, match="GPU"):
+        bs.act_backward8(torch.zeros(4, 8), ck((4, 8), relu=True))
+    with pytest.raises(TypeError):
+        bs.act_backward8(torch.zeros(4, 8, dtype=torch.float64), ck((4, 8), relu=True))
+
+
+def test_scratch_sizes_of_every_size():
+    need = _lib.lib().mdt_conv1x1_act8_backward_workspace_bytes
+    for V in (1, 2, 3, 4, 5, 7, 31, 257, 4096, 1 << 20, 1 << 30):
+        for ci in (1, 2, 3, 18, 257, 2048, 65536):
+            for co in (1, 2, 3, 18, 255, 257, 514, 1028, 2048, 65536):
+                n = need(V, ci, co)
+                assert 4 * co <= n <= 4 * 2048 * (ci * co + co) + 4 * 32 * V * ci + 4096, (V, ci, co, n)

@@ -48,6 +48,7 @@ def main():
                     "semantics and state-dict format); 0: torch.optim.Adam itself")
     ap.add_argument("--adam-absent-grad", default="skip", choices=["skip", "zero_after_first"], help="a parameter without a gradient in a step: skip it "
                     "(torch >= 2, default) or update it with a zero gradient once it has had one (torch 0.4.1, the reference's pinned version)")
+    ap.add_argument("--act8", type=int, default=0, help="1: the backbone's maps kept for the backward pass in 8 bits (cf.act8_checkpoints)")
     args = ap.parse_args()
 
     world = int(os.environ.get("WORLD_SIZE", "1"))
@@ -73,7 +74,7 @@ def main():
     from medicaldetectiontoolkit_amd.utils.synthetic_data import make_batch, to_device
 
     patch = [int(v) for v in args.patch.split(",")]
-    cf = Configs(dim=args.dim, model=args.model, patch_size=patch, batch_size=args.batch, channels_last=True,
+    cf = Configs(dim=args.dim, model=args.model, patch_size=patch, batch_size=args.batch, channels_last=True, act8_checkpoints=bool(args.act8),
                  num_epochs=args.epochs, num_train_batches=args.batches)
     torch.manual_seed(0)
     net = (mrcnn if args.model == "mrcnn" else retina_unet).net(cf, device=dev)
