@@ -413,7 +413,8 @@ __global__ __launch_bounds__(THREADS, 2) void conv1x1_bwd_act8_products(Args a, 
 }
 
 // out[e] = sum over the splits of part[split][e] in a fixed order, for up to three arrays at once.  A workgroup sums 1024 >> log_r elements, each in 1 << log_r
-// interleaved ranges of splits.  512 partial sums of 18 x 72 weights with 8 ranges: 21 us, with 32: 5 us.
+// interleaved ranges of splits: the fewest that make two workgroups a CU (512 partial sums of 18 x 72 weights in 8 ranges: 21 us, in 32: 5 us; 13 partial sums of 384 x 1536 weights
+// in 8: 13.5 us, in 1: 8 us).
 struct Joined { const float *part; float *out; long long n; int splits, log_r; long long groups; };
 __global__ __launch_bounds__(1024) void conv1x1_bwd_act8_join(Joined j0, Joined j1, Joined j2)
 {
@@ -443,7 +444,8 @@ __global__ __launch_bounds__(1024) void conv1x1_bwd_act8_join(Joined j0, Joined 
 
 inline Joined joined(const float *part, float *out, long long n, long long splits)
 {
-    Joined j = {part, out, out ? n : 0, (int)splits, splits >= 64 ? 5 : splits >= 8 ? 3 : 0, 0};
+    Joined j = {part, out, out ? n : 0, (int)splits, 0, 0};
+    while (j.log_r < 5 && (j.n >> (10 - j.log_r)) < 512 && (splits >> j.log_r) > 4) ++j.log_r;
     j.groups = (j.n + (1024 >> j.log_r) - 1) / (1024 >> j.log_r);
     return j;
 }
@@ -863,7 +865,7 @@ template <int MT, int NT>
 int fused_launch(const FusedPlan &p, const Args &a, hipStream_t s)
 {
     const auto kernel = a.g != nullptr ? conv1x1_bwd_act8_fused<MT, NT, true> : conv1x1_bwd_act8_fused<MT, NT, false>;
-    if (hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, p.lds) != hipSuccess) return MDT_ERR_LAUNCH_FAILED;
+    if (p.lds > 64 * 1024 && hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, p.lds) != hipSuccess) return MDT_ERR_LAUNCH_FAILED;
     kernel<<<p.blocks, THREADS, p.lds, s>>>(a.gy, a.yc, a.w, a.xc, a.xs, a.gx, a.g, a.part_w, a.part_b, a.V, a.ci, a.co, a.x_relu);
     return MDT_OK;
 }

@@ -38,7 +38,7 @@ def _call(device, name, *args):
     """the C entry on `device`'s current stream"""
     fn = getattr(_lib.lib(), name)
     idx = device.index
-    if idx == torch.cuda.current_device():
+    if idx == torch._C._cuda_getDevice():                       # (a tensor on the GPU exists: no lazy initialisation to ask for)
         rc = fn(*args, torch._C._cuda_getCurrentRawStream(idx))
     else:
         with torch.cuda.device(idx):
@@ -59,7 +59,8 @@ def _on_gpu(device, name):
 def _float_tensor(x, name):
     if x.dtype not in _DTYPES:
         raise TypeError("%s: float32, bfloat16 or float16, not %s" % (name, x.dtype))
-    _lib.require_cuda(x, name)
+    if not x.is_cuda:
+        _lib.require_cuda(x, name)
 
 
 def _same_device(ref, **tensors):
@@ -128,7 +129,8 @@ class Checkpoint8(object):
             channels_last = len(shape) == 2
         elif (channels_last and len(shape) not in (2, 4, 5)) or (len(shape) == 2 and not channels_last):
             raise ValueError("Checkpoint8: channels_last=%s does not describe %d axes" % (channels_last, len(shape)))
-        _same_device(codes.device, scales=scales)
+        if scales.device != codes.device:
+            _same_device(codes.device, scales=scales)
         self._set(None, codes, scales, shape, bool(relu), dtype, bool(channels_last), codes.device)
 
     def _set(self, buffer, codes, scales, shape, relu, dtype, channels_last, device):
@@ -202,26 +204,28 @@ def bias_act_checkpoint8(h, bias, residual=None, relu=True, inplace=False):
     _float_tensor(h, "h")
     if h.dtype != torch.float32 or bias.dtype != torch.float32 or (residual is not None and residual.dtype != torch.float32):
         raise TypeError("bias_act_checkpoint8: float32 operands")
-    if h.dim() < 2 or tuple(bias.shape) != (h.shape[1],) or (residual is not None and residual.shape != h.shape):
-        raise ValueError("bias_act_checkpoint8: bias %s and residual %s do not fit h %s"
-                         % (tuple(bias.shape), None if residual is None else tuple(residual.shape), tuple(h.shape)))
-    _same_device(h.device, bias=bias, residual=residual)
-    _no_graph("bias_act_checkpoint8", h, bias, residual)
+    shape, device = h.shape, h.device
+    if len(shape) < 2 or bias.dim() != 1 or bias.shape[0] != shape[1] or (residual is not None and residual.shape != shape):
+        raise ValueError("bias_act_checkpoint8: bias %s and residual %s do not fit h %s" % (tuple(bias.shape), None if residual is None else tuple(residual.shape), tuple(shape)))
+    if bias.device != device or (residual is not None and residual.device != device):
+        _same_device(device, bias=bias, residual=residual)
+    if torch.is_grad_enabled():
+        _no_graph("bias_act_checkpoint8", h, bias, residual)
     x, cl = _dense(h)
     if inplace and x is not h:
         raise ValueError("bias_act_checkpoint8: inplace needs a dense row-major or channels-last h")
-    inner = 1 if cl else math.prod(x.shape[2:])
+    inner = 1 if cl else math.prod(shape[2:])
     if residual is not None and residual.stride() != x.stride():
         residual = residual.contiguous(memory_format=_rows_format(x.dim()) if cl else torch.contiguous_format)
     if not bias.is_contiguous():
         bias = bias.contiguous()
     y = x if inplace else torch.empty_like(x)
-    n, device = x.numel(), x.device
+    n = x.numel()
     buffer = _new_buffer(n, device)
     if n:
         at = buffer.data_ptr()
-        _call(device, "mdt_bias_act_act8_forward", y.data_ptr(), x.data_ptr(), bias.data_ptr(), _ptr(residual), at, at + _scales_at(n), n, int(x.shape[1]), inner, int(relu))
-    return y, Checkpoint8.of_buffer(buffer, tuple(x.shape), bool(relu), x.dtype, cl)
+        _call(device, "mdt_bias_act_act8_forward", y.data_ptr(), x.data_ptr(), bias.data_ptr(), _ptr(residual), at, at + _scales_at(n), n, shape[1], inner, int(relu))
+    return y, Checkpoint8.of_buffer(buffer, tuple(shape), bool(relu), x.dtype, cl)
 
 
 def conv1x1_backward8(gy, w, x8, y8=None, need_g=False, need_gx=True, need_gw=True):
@@ -232,9 +236,9 @@ def conv1x1_backward8(gy, w, x8, y8=None, need_g=False, need_gx=True, need_gw=Tr
     if gy.dtype != torch.float32 or w.dtype != torch.float32:
         raise TypeError("conv1x1_backward8: float32 gradients and weights")
     _lib.require_cuda(gy, "gy")
-    if w.dim() < 2 or math.prod(w.shape[2:]) != 1:
-        raise ValueError("conv1x1_backward8: a 1x1(x1) filter, not %s" % (tuple(w.shape),))
     w_shape = tuple(w.shape)
+    if len(w_shape) < 2 or math.prod(w_shape[2:]) != 1:
+        raise ValueError("conv1x1_backward8: a 1x1(x1) filter, not %s" % (w_shape,))
     co, ci = w_shape[:2]
     shape = tuple(gy.shape)
     if gy.dim() not in (2, 4, 5) or shape[1] != co or x8.shape != shape[:1] + (ci,) + shape[2:]:
@@ -244,8 +248,9 @@ def conv1x1_backward8(gy, w, x8, y8=None, need_g=False, need_gx=True, need_gw=Tr
     if y8 is not None and (y8.shape != shape or not y8.relu):
         raise ValueError("conv1x1_backward8: y8 is the kept ReLU output of gy's shape")
     dev = gy.device
-    _same_device(dev, w=w, x8=x8, y8=y8)
-    mf = _rows_format(gy.dim())
+    if w.device != dev or x8.device != dev or (y8 is not None and y8.device != dev):
+        _same_device(dev, w=w, x8=x8, y8=y8)
+    mf = _rows_format(len(shape))
     if not gy.is_contiguous(memory_format=mf):
         gy = gy.contiguous(memory_format=mf)
     if w.stride()[:2] != (ci, 1):
@@ -371,71 +376,106 @@ def conv_bias_act8(conv, x, x8=None, residual=None, relu=False, keep=True, subsa
 
 class Mx4(object):
     """Rows in 4 bits: `codes` uint8 [..., ceil(k / 32) * 16] (two a byte, the even value in the low half), `scales` uint8 [..., ceil(k / 32)]; blocks run along
-    the last axis of length k."""
-    __slots__ = ("codes", "scales", "k", "dtype")
+    the last axis of length k.  `shape`: the values' shape.  What mx4_quantize makes holds both in one allocation, `buffer`."""
+    __slots__ = ("buffer", "_codes", "_scales", "shape", "k", "dtype", "device")
 
     def __init__(self, codes, scales, k, dtype=torch.float32):
         k = int(k)
         kb = -(-k // BLOCK)
-        if k < 1 or codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or codes.dim() < 1 or codes.shape[-1] != 16 * kb \
-                or tuple(scales.shape) != tuple(codes.shape[:-1]) + (kb,):
+        rows = tuple(codes.shape[:-1])
+        if k < 1 or codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or codes.dim() < 1 or codes.shape[-1] != 16 * kb or tuple(scales.shape) != rows + (kb,):
             raise ValueError("Mx4: uint8 codes [..., %d] and scales [..., %d] for rows of %d, got %s %s and %s %s"
                              % (16 * kb, kb, k, tuple(codes.shape), codes.dtype, tuple(scales.shape), scales.dtype))
         if not codes.is_contiguous() or not scales.is_contiguous() or codes.data_ptr() % 16 != 0:
             raise ValueError("Mx4: codes and scales are contiguous, the codes 16-byte aligned")
         if dtype not in _DTYPES:
             raise TypeError("Mx4: float32, bfloat16 or float16, not %s" % dtype)
-        _same_device(codes.device, scales=scales)
-        self.codes, self.scales, self.k, self.dtype = codes, scales, k, dtype
+        if scales.device != codes.device:
+            _same_device(codes.device, scales=scales)
+        self.buffer, self._codes, self._scales, self.shape, self.k, self.dtype, self.device = None, codes, scales, rows + (k,), k, dtype, codes.device
+
+    @classmethod
+    def of_buffer(cls, buffer, shape, dtype):
+        """codes, then scales, in one uint8 tensor"""
+        m = cls.__new__(cls)
+        m.buffer, m._codes, m._scales, m.shape, m.k, m.dtype, m.device = buffer, None, None, shape, shape[-1], dtype, buffer.device
+        return m
+
+    def _bytes(self):
+        kb = -(-self.k // BLOCK)
+        return math.prod(self.shape[:-1]) * kb * 16, kb
 
     @property
-    def shape(self):
-        return tuple(self.codes.shape[:-1]) + (self.k,)
+    def codes(self):
+        if self.buffer is None:
+            return self._codes
+        n, kb = self._bytes()
+        return self.buffer[:n].view(self.shape[:-1] + (16 * kb,))
+
+    @property
+    def scales(self):
+        if self.buffer is None:
+            return self._scales
+        n, kb = self._bytes()
+        return self.buffer[n:].view(self.shape[:-1] + (kb,))
+
+    def pointers(self):
+        """(codes, scales) as addresses"""
+        if self.buffer is None:
+            return self._codes.data_ptr(), self._scales.data_ptr()
+        at = self.buffer.data_ptr()
+        return at, at + self._bytes()[0]
 
     def dequantize(self):
         """the values the codes stand for, in the type of the tensor they were taken from"""
-        _lib.require_cuda(self.codes, "Mx4.codes")
-        x = torch.empty(self.shape, dtype=self.dtype, device=self.codes.device)
-        _call(x.device, "mdt_mx4_dequantize", self.codes.data_ptr(), self.scales.data_ptr(), x.data_ptr(), x.numel() // self.k, self.k, _DTYPES[self.dtype])
+        _on_gpu(self.device, "Mx4")
+        x = torch.empty(self.shape, dtype=self.dtype, device=self.device)
+        codes, scales = self.pointers()
+        _call(self.device, "mdt_mx4_dequantize", codes, scales, x.data_ptr(), x.numel() // self.k, self.k, _DTYPES[self.dtype])
         return x
 
 
 def mx4_quantize(x):
     """x's rows (last axis) in 4 bits"""
     _float_tensor(x, "x")
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError("mx4_quantize: rows of at least one value, not %s" % (tuple(x.shape),))
-    x = x.detach()
+    shape = tuple(x.shape)
+    if not shape or shape[-1] < 1:
+        raise ValueError("mx4_quantize: rows of at least one value, not %s" % (shape,))
     if not x.is_contiguous():
-        x = x.contiguous()
-    k = int(x.shape[-1])
-    kb = -(-k // BLOCK)
-    codes = torch.empty(x.shape[:-1] + (16 * kb,), dtype=torch.uint8, device=x.device)
-    scales = torch.empty(x.shape[:-1] + (kb,), dtype=torch.uint8, device=x.device)
-    _call(x.device, "mdt_mx4_quantize", x.data_ptr(), codes.data_ptr(), scales.data_ptr(), x.numel() // k, k, _DTYPES[x.dtype])
-    return Mx4(codes, scales, k, x.dtype)
+        x = x.detach().contiguous()
+    k, device = shape[-1], x.device
+    rows = x.numel() // k
+    n = rows * -(-k // BLOCK)
+    buffer = torch.empty(17 * n, dtype=torch.uint8, device=device)
+    at = buffer.data_ptr()
+    _call(device, "mdt_mx4_quantize", x.data_ptr(), at, at + 16 * n, rows, k, _DTYPES[x.dtype])
+    return Mx4.of_buffer(buffer, shape, x.dtype)
 
 
 def mx4_linear(x, w4, bias=None, relu=False):
     """act(x W^T + bias) in x's type: x [..., K] (float32, bfloat16 or float16) is rounded to 4 bits in the call, w4 = mx4_quantize(W) for W [N, K]; products and
     sums in float32.  bias: [N], taken in float32.  For inference: no autograd graph."""
     _float_tensor(x, "x")
-    if len(w4.shape) != 2 or x.dim() < 1 or x.shape[-1] != w4.k or (bias is not None and tuple(bias.shape) != (w4.shape[0],)):
-        raise ValueError("mx4_linear: x %s, W %s and bias %s do not fit" % (tuple(x.shape), w4.shape, None if bias is None else tuple(bias.shape)))
-    _same_device(x.device, w4=w4.codes, bias=bias)
-    _no_graph("mx4_linear", x, bias)
+    shape, device = x.shape, x.device
+    if len(w4.shape) != 2 or not shape or shape[-1] != w4.k or (bias is not None and (bias.dim() != 1 or bias.shape[0] != w4.shape[0])):
+        raise ValueError("mx4_linear: x %s, W %s and bias %s do not fit" % (tuple(shape), w4.shape, None if bias is None else tuple(bias.shape)))
+    if w4.device != device or (bias is not None and bias.device != device):
+        _same_device(device, w4=w4, bias=bias)
+    if x.requires_grad or (bias is not None and bias.requires_grad):
+        _no_graph("mx4_linear", x, bias)
     n, k = w4.shape
     if not x.is_contiguous():
         x = x.contiguous()
     if bias is not None and (bias.dtype != torch.float32 or not bias.is_contiguous()):
         bias = bias.float().contiguous()
     rows = x.numel() // k
-    y = torch.empty(x.shape[:-1] + (n,), dtype=x.dtype, device=x.device)
+    y = torch.empty(shape[:-1] + (n,), dtype=x.dtype, device=device)
     if y.numel() == 0:
         return y
     need = _lib.lib().mdt_mx4_linear_workspace_bytes(rows, k, n)
-    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
-    _call(x.device, "mdt_mx4_linear", x.data_ptr(), _DTYPES[x.dtype], w4.codes.data_ptr(), w4.scales.data_ptr(), _ptr(bias), y.data_ptr(), rows, k, n, int(relu), _ptr(ws), need)
+    ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    codes, scales = w4.pointers()
+    _call(device, "mdt_mx4_linear", x.data_ptr(), _DTYPES[x.dtype], codes, scales, _ptr(bias), y.data_ptr(), rows, k, n, int(relu), _ptr(ws), need)
     return y
 
 
