@@ -562,6 +562,9 @@ void sum_run(const SumPlan &p, const Args &a, hipStream_t s)
 __host__ __device__ constexpr int fused_rows_floats(int mt, int ci, int co) { return 32 * (co > ci ? co : ci) + 32 * mt; }
 __host__ __device__ constexpr int fused_wave_floats(int mt, int nt, int ci, int co) { return (fused_rows_floats(mt, ci, co) + (32 * ci + 32 * nt) / 2 + 3) / 4 * 4; }
 
+// regions of LDS for the waves' sums at the end: 9 tiles for each of 4 waves are 147 KB
+__host__ __device__ constexpr int fused_regions(int tiles) { return tiles <= 9 ? WAVES : 2; }
+
 // ---- both products in one pass, for few channels --------------------------------------------------------------------------------------------
 // A wave takes 32 voxels at a time and needs no other wave: their 32 co gradients are one contiguous run, loaded 16 bytes a lane, masked, and put into the
 // wave's own LDS tile as they are; their 32 ci input codes are ci whole blocks.  From the tile gw takes columns (M = co, N = ci, K = voxel) and gx takes rows
@@ -775,12 +778,13 @@ __global__ __launch_bounds__(THREADS, MT * NT <= 3 ? 2 : 1) void conv1x1_bwd_act
         }
         fence();
     }
-    // the four waves' sums, in wave order
-    float *sum = reinterpret_cast<float *>(smem), *sumb = sum + 32 * 32 * MT * NT;
-#pragma unroll 1
-    for (int turn = 0; turn < WAVES; ++turn) {
+    // the four waves' sums, in wave order: a region of LDS each, or one for two waves where four would not fit (one region, written in turn, took 7 us of a call's end)
+    constexpr int REGIONS = fused_regions(MT * NT), REGION = 1024 * MT * NT + 32 * MT;
+    float *sum = reinterpret_cast<float *>(smem) + wave % REGIONS * REGION, *sumb = sum + 1024 * MT * NT;
+#pragma unroll
+    for (int turn = 0; turn < WAVES / REGIONS; ++turn) {
         __syncthreads();
-        if (wave != turn) continue;
+        if (wave / REGIONS != turn) continue;
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
             const float b2 = bsum[m] + __shfl_xor(bsum[m], 32);
@@ -795,8 +799,15 @@ __global__ __launch_bounds__(THREADS, MT * NT <= 3 ? 2 : 1) void conv1x1_bwd_act
         }
     }
     __syncthreads();
-    for (int t = threadIdx.x; t < co * ci; t += THREADS) part_w[(long long)blockIdx.x * co * ci + t] = sum[(t / ci) * 32 * NT + t % ci];
-    for (int t = threadIdx.x; t < co; t += THREADS) part_b[(long long)blockIdx.x * co + t] = sumb[t];
+    const float *all = reinterpret_cast<const float *>(smem);
+    auto total = [&](int at) {
+        float r = all[at];
+#pragma unroll
+        for (int k = 1; k < REGIONS; ++k) r = r + all[k * REGION + at];
+        return r;
+    };
+    for (int t = threadIdx.x; t < co * ci; t += THREADS) part_w[(long long)blockIdx.x * co * ci + t] = total((t / ci) * 32 * NT + t % ci);
+    for (int t = threadIdx.x; t < co; t += THREADS) part_b[(long long)blockIdx.x * co + t] = total(1024 * MT * NT + t);
 }
 
 // Tiles of the two products.  gw: 64 or 128 along each axis, about two workgroups a CU, at least 128 voxels each.  gx: 128 x 128 where that gives two workgroups
@@ -852,7 +863,7 @@ inline FusedPlan fused_plan(long long V, int ci, int co)
     if (tiles > 10) return {0, 0, 0, 0};
     const int ks = (co + 15) / 16;
     p.lds = p.nt * ks * 3 * 1024 + WAVES * fused_wave_floats(p.mt, p.nt, ci, co) * 4;
-    const int sums = (1024 * tiles + 32 * p.mt) * 4;
+    const int sums = fused_regions(tiles) * (1024 * tiles + 32 * p.mt) * 4;
     if (p.lds < sums) p.lds = sums;
     if (p.lds > 160 * 1024) return {0, 0, 0, 0};
     const int per_cu = tiles <= 3 ? 2 : 1, fit = 160 * 1024 / p.lds, at_once = 256 * (fit < per_cu ? fit : per_cu);
@@ -926,8 +937,12 @@ int mdt_conv1x1_act8_backward(const float *gy, const float *w, const void *x_cod
     const FusedPlan f = gx && gw ? fused_plan(V, c_in, c_out) : FusedPlan{0, 0, 0, 0};
     if (f.mt > 0 && V * c_in >= 4 && V * c_out >= 4) {
         a.part_b = a.part_w + f.blocks * nw;
+        if (f.blocks == 1) {                                                     // nothing to join
+            a.part_w = gw;
+            if (gbias) a.part_b = gbias;
+        }
         const int rc = fused_run(f, a, s);
-        if (rc != MDT_OK) return rc;
+        if (rc != MDT_OK || f.blocks == 1) return rc != MDT_OK ? rc : launch_check();
         const int rj = join_run(joined(a.part_w, gw, nw, f.blocks), joined(a.part_b, gbias, c_out, f.blocks), none, s);
         return rj != MDT_OK ? rj : launch_check();
     }
