@@ -51,6 +51,9 @@ struct Args { const float *gy; const uint8_t *yc; const float *w; const uint8_t 
 // Both kernels cut what they load into bf16 pieces once, put the pieces into LDS with the summed axis innermost (32 entries and 8 of padding a row: the
 // 16-byte reads and writes of neighbouring rows fall into different banks) and hold the next step's loads in registers meanwhile.  4 waves, WM x WN of
 // them with TM x TN matrix tiles of 32 x 32 each.
+// 1620 voxels 1536 -> 384: 45 us, 380 TFLOP/s of the 9 products of pieces, and 7 us for the joining.  The cutting, which every tile repeats for its rows (28 % of
+// the VALU's slots), and the waits at two workgroups a CU bound it.  Pieces cut once by a launch of their own and multiplied from L2 without LDS took 10 + 34 us
+// here and twice the time for long narrow maps.
 constexpr int KSTEP = 32, KROW = KSTEP + 8;
 
 __device__ __forceinline__ v8bf row_of(const uint16_t *p) { return __builtin_bit_cast(v8bf, *reinterpret_cast<const v4u *>(p)); }
@@ -460,10 +463,10 @@ int join_run(const Joined &a, const Joined &b, const Joined &c, hipStream_t s)
 }
 
 // ---- no product wanted: the mask and the sum of columns -----------------------------------------------------------------------------------------
-// g = gy . m and gbias for a layer whose products other kernels take (a window, a stride).  5 bytes read and 4 written a value.
+// g = gy . m and gbias for a layer whose products other kernels take (a window, a stride).  5 bytes read and 4 written a value: 1 M x 18 in 34 us, 5.0 TB/s.
 // A workgroup walks over its run of quads of values in steps of `active` quads, a multiple of the period after which quads begin at the same channel again: a thread's 4
 // sums belong to the same 4 channels throughout, whatever the number of channels, as long as the period fits into a workgroup.
-constexpr int SUM_ROWS = 1024;                                                   // partial sums of a channel at most
+constexpr int SUM_ROWS = 1024;                                                   // partial sums of a channel at most (1 M x 18: 512 34.2 us, 1024 34.1, 2048 38.5; 100000 x 257: 80, 56, 55)
 
 template <bool MASK>
 __global__ __launch_bounds__(THREADS) void act8_mask_sum_quads(const float *__restrict__ gy, const uint8_t *__restrict__ yc, float *__restrict__ g, float *__restrict__ part, long long n,
@@ -571,6 +574,10 @@ __host__ __device__ constexpr int fused_regions(int tiles) { return tiles <= 9 ?
 // wave's own LDS tile as they are; their 32 ci input codes are ci whole blocks.  From the tile gw takes columns (M = co, N = ci, K = voxel) and gx takes rows
 // (M = ci, N = voxel, K = co), both cut into bf16 pieces in registers; gw stays in registers over all of a wave's voxels.  gx's tile replaces the gradients in LDS
 // and leaves as the contiguous run that it is, like g.
+// Used while gw takes at most 10 tiles of 32 x 32 of a side of at most 160 (what registers hold): narrow layers gain (100000 voxels 32 -> 160: 48 us, tiled 70; 36 -> 144: 59,
+// 67; 144 -> 36: 56, 68), square ones are equal (64 -> 64: 53, 50; 96 -> 64: 47, 45; 64 -> 96: 45, 48).
+// 1 M voxels 18 -> 72 with g: 163 us, 4.8 TB/s of its 155 us floor; 72 -> 18: 121 us, 3.9 TB/s (floor 95): memory, and the waits of a wave's chunk where no other wave covers
+// them.  A call of few voxels is one chunk's chain of loads, LDS and products: 32 voxels 8 us.
 // Loads and stores share one in-order counter: the next chunk's loads are issued before this chunk's stores and every chunk issues the same number of
 // stores, so that the wait for the loads does not wait for the stores behind them.
 // Entries of the tiles behind co or ci hold whatever follows in LDS: they only reach rows and columns that are not stored, except along gx's sum, where
@@ -811,9 +818,10 @@ __global__ __launch_bounds__(THREADS, MT * NT <= 3 ? 2 : 1) void conv1x1_bwd_act
     for (int t = threadIdx.x; t < co; t += THREADS) part_b[(long long)blockIdx.x * co + t] = total(1024 * MT * NT + t);
 }
 
-// Tiles of the two products.  gx: 128 x 128 where that gives two workgroups a CU, else 64 x 64; where even those leave CUs idle, the sum over co is split (at least 4
-// steps each) and joined with gw's.  gw: 64 or 128 along each axis; its sum is split so that both products together fill whole rounds of the two workgroups that a CU
-// holds, at least 128 of them and at least 128 voxels each.  (1620 voxels 1536 -> 384: 13 ranges 64 us, 11 of them 50; 6480 voxels 192 -> 768: 43 ranges 68 us, 17 52.)
+// Tiles of the two products.  gx: 128 x 128 where that gives a workgroup a CU (20000 voxels 300 -> 400: 108 us, 64 x 64 124; 100000 voxels 200 -> 250: 205, 264), else
+// 64 x 64; where even those leave CUs idle, the sum over co is split (at least 4 steps each; 400 voxels 1000 -> 1000: 38 us, unsplit 50) and joined with gw's.  gw: 64 or
+// 128 along each axis; its sum is split so that both products together fill whole rounds of the two workgroups that a CU holds, at least 128 of them and at least 128
+// voxels each (1620 voxels 1536 -> 384: 13 ranges 64 us, 11 of them 50; 6480 voxels 192 -> 768: 43 ranges 68 us, 17 52).
 struct Plan { int w_m, w_n, d_tile; WgradGrid wg; DgradGrid dg; };
 inline Plan plan_of(long long V, int ci, int co)
 {
@@ -825,7 +833,7 @@ inline Plan plan_of(long long V, int ci, int co)
     w.ci_tiles = (ci + p.w_n - 1) / p.w_n;
     DgradGrid &d = p.dg;
     const long long big = ((V + 127) / 128) * ((ci + 127) / 128);
-    p.d_tile = ci > 64 && big >= 512 ? 128 : 64;
+    p.d_tile = ci > 64 && big >= 256 ? 128 : 64;
     d.ci_tiles = (ci + p.d_tile - 1) / p.d_tile;
     const long long ranges = (V + p.d_tile - 1) / p.d_tile, now = ranges * d.ci_tiles;
     const int steps = (co + KSTEP - 1) / KSTEP;
