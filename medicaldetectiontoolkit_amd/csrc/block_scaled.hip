@@ -2,8 +2,8 @@
 //
 // All of it is HBM-bound streaming: a block of 32 values is held by 8 lanes (4 fp32 values each) or 4 lanes (8 values of 16 bits each), 16 bytes a
 // lane and load, and its maximum is two quad permutes (and one half-row mirror) of the lanes' own maxima -- no LDS, no second pass over the data.  What they reach (a copy of
-// 1 GiB: 5.0 TB/s, read and written): 5.5 TB/s for the epilogue and the read-back of 75.5 M values with a residual (192 + 58 us), 5.2 for 94 M 16-bit values into 4 bits and back
-// (56 + 38 us).
+// 1 GiB: 5.0 TB/s, read and written): 5.5 TB/s for the epilogue and the read-back of 75.5 M values with a residual (192 + 58 us), 5.7 for 94 M 16-bit values into 4 bits and back
+// (48 + 38 us).
 #include "block_scaled.h"
 
 namespace {
