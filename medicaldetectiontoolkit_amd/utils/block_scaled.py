@@ -237,7 +237,7 @@ def conv1x1_backward8(gy, w, x8, y8=None, need_g=False, need_gx=True, need_gw=Tr
         raise TypeError("conv1x1_backward8: float32 gradients and weights")
     _lib.require_cuda(gy, "gy")
     w_shape = tuple(w.shape)
-    if len(w_shape) < 2 or math.prod(w_shape[2:]) != 1:
+    if len(w_shape) < 2 or math.prod(w_shape[2:]) != 1 or 0 in w_shape:
         raise ValueError("conv1x1_backward8: a 1x1(x1) filter, not %s" % (w_shape,))
     co, ci = w_shape[:2]
     shape = tuple(gy.shape)
@@ -272,7 +272,7 @@ def act_backward8(gy, y8):
     if gy.dtype != torch.float32:
         raise TypeError("act_backward8: float32 gradients")
     _lib.require_cuda(gy, "gy")
-    if gy.dim() not in (2, 4, 5) or y8.shape != tuple(gy.shape) or not y8.relu or not y8.channels_last:
+    if gy.dim() not in (2, 4, 5) or gy.shape[1] == 0 or y8.shape != tuple(gy.shape) or not y8.relu or not y8.channels_last:
         raise ValueError("act_backward8: y8 is the kept ReLU output of gy's shape, channels innermost")
     dev = gy.device
     _same_device(dev, y8=y8)
@@ -300,11 +300,12 @@ class _ConvBiasAct8(Function):
         if residual is not None and not residual.is_contiguous(memory_format=mf):
             residual = residual.contiguous(memory_format=mf)
         one = math.prod(w.shape[2:]) == 1
+        bias = bias.detach().contiguous()
         y = y8 = None
-        if one and x.numel() >= (1 << 20) and x.data_ptr() % 16 == 0 and _lib.lib().mdt_conv1x1_forward_supported(int(w.shape[1]), int(w.shape[0])):
+        if one and x.numel() >= (1 << 20) and x.data_ptr() % 16 == 0 and w.stride()[:2] == (w.shape[1], 1) and _lib.lib().mdt_conv1x1_forward_supported(int(w.shape[1]), int(w.shape[0])):
             y = fused_epilogue._conv1x1_forward(x, w, bias, residual, relu)
         elif nd == 3 and residual is None and padding == (1, 1, 1) and not x.is_contiguous():
-            y = fused_epilogue.conv3x3x3_small(x, w, bias.detach(), relu)
+            y = fused_epilogue.conv3x3x3_small(x, w, bias, relu)
         if y is None:
             h = (F.conv3d if nd == 3 else F.conv2d)(x, w, None, 1, padding)
             if not h.is_contiguous(memory_format=mf):
@@ -350,18 +351,18 @@ def conv_bias_act8(conv, x, x8=None, residual=None, relu=False, keep=True, subsa
     for name, ok in (("a bias", conv.bias is not None), ("one group", conv.groups == 1), ("unit dilation", all(int(v) == 1 for v in conv.dilation)),
                      ("zero padding", conv.padding_mode == "zeros" and not isinstance(conv.padding, str)),
                      ("a size-preserving window", not isinstance(conv.padding, str) and all(2 * int(p) + 1 == int(k) for p, k in zip(conv.padding, conv.kernel_size))),
-                     ("unit stride", subsampled or all(int(v) == 1 for v in conv.stride))):
+                     ("unit stride", all(int(v) == 1 for v in conv.stride) or (subsampled and all(int(k) == 1 for k in conv.kernel_size)))):
         if not ok:
             raise ValueError("conv_bias_act8: a convolution with %s" % name)
     _float_tensor(x, "x")
-    if x.dtype != torch.float32 or conv.weight.dtype != torch.float32 or torch.is_autocast_enabled():
+    if x.dtype != torch.float32 or conv.weight.dtype != torch.float32 or conv.bias.dtype != torch.float32 or torch.is_autocast_enabled():
         raise TypeError("conv_bias_act8: float32 training, not under autocast")
     if x.dim() != conv.weight.dim() or int(x.shape[1]) != int(conv.weight.shape[1]):
         raise ValueError("conv_bias_act8: x %s does not fit the filter %s" % (tuple(x.shape), tuple(conv.weight.shape)))
     shape = (x.shape[0], conv.weight.shape[0]) + tuple(x.shape[2:])
     if residual is not None and (tuple(residual.shape) != tuple(shape) or residual.dtype != torch.float32):
         raise ValueError("conv_bias_act8: residual %s, output %s" % (tuple(residual.shape), tuple(shape)))
-    _same_device(x.device, weight=conv.weight, residual=residual, x8=x8)
+    _same_device(x.device, weight=conv.weight, bias=conv.bias, residual=residual, x8=x8)
     if x.device.index != torch.cuda.current_device():
         raise RuntimeError("conv_bias_act8: x is not on the current device (one process per GPU)")
     mf = _rows_format(x.dim())
@@ -482,16 +483,18 @@ def mx4_linear(x, w4, bias=None, relu=False):
 @contextlib.contextmanager
 def mx4_heads(net):
     """A Mask R-CNN's box head (the two products of every region, `classifier.conv1` and `conv2`) in 4 bits while the context lasts: the filters are rounded when it is
-    entered, so load a checkpoint before, and not inside.  Inference only: a training step inside raises."""
+    entered, so load a checkpoint before, and not inside.  It holds for every call of the net while it lasts; a second one at the same time (nested, or of another thread)
+    raises.  Inference only: a training step inside raises."""
     head = getattr(net, "classifier", None)
     if head is None or not hasattr(head, "mx4"):
         raise ValueError("mx4_heads: a net with a box head (Mask R-CNN), not %s" % type(net).__name__)
     if not (isinstance(head.conv1, fused_epilogue.ConvBiasReLU) and isinstance(head.conv2, fused_epilogue.ConvBiasReLU)
             and tuple(head.conv1[0].kernel_size) == tuple(head.pool_size) and not any(head.conv1[0].padding)):
         raise ValueError("mx4_heads: the box head's layers are convolution + ReLU without a norm, the first as large as the pooled region")
-    before = head.mx4
+    if head.mx4 is not None:
+        raise RuntimeError("mx4_heads: the net's head is in 4 bits already")
     head.mx4 = tuple(mx4_quantize(c[0].weight.detach().flatten(1)) for c in (head.conv1, head.conv2))
     try:
         yield net
     finally:
-        head.mx4 = before
+        head.mx4 = None

@@ -202,6 +202,49 @@ def test_conv_bias_act8_shared_input_twice_and_second_backward(cuda):
     assert torch.equal(x.grad, 2 * first[0]) and torch.equal(conv.weight.grad, 2 * first[1])
 
 
+def test_conv_bias_act8_filters_and_biases_of_any_strides(cuda):
+    """a filter that is a transposed view, a bias that is a column: on a map large enough for this package's 1x1 kernel"""
+    conv, x0, gy, _ = int_layer(cuda, 3, 18, 18, 1, (64, 64, 32), 1, 9)
+    odd = nn.Conv3d(18, 18, 1).to(cuda)
+    odd.weight = nn.Parameter(conv.weight.detach().flatten(1).t().contiguous().t().view(18, 18, 1, 1, 1))
+    odd.bias = nn.Parameter(torch.stack([conv.bias.detach(), conv.bias.detach()], 1)[:, 0])
+    assert odd.weight.stride()[:2] == (1, 18) and odd.bias.stride() == (2,)
+    outs = []
+    for c in (conv, odd):
+        x = x0.to(cuda).contiguous(memory_format=torch.channels_last_3d).requires_grad_()
+        y, _ = bs.conv_bias_act8(c, x, None, relu=True)
+        y.backward(gy.to(cuda))
+        outs.append((y.detach(), x.grad, c.weight.grad, c.bias.grad))
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+
+
+def test_saved_copies_may_leave_the_card(cuda):
+    """what autograd holds goes through its hooks as plain tensors: kept on the host between the passes"""
+    conv, x0, gy, _ = int_layer(cuda, 2, 36, 36, 1, (6, 6), 2, 7)
+    grads = []
+    for hooks in (False, True):
+        conv.zero_grad(set_to_none=True)
+        x = x0.to(cuda).contiguous(memory_format=torch.channels_last).requires_grad_()
+        if hooks:
+            with torch.autograd.graph.save_on_cpu():
+                y, _ = bs.conv_bias_act8(conv, x, None, relu=True)
+        else:
+            y, _ = bs.conv_bias_act8(conv, x, None, relu=True)
+        y.backward(gy.to(cuda))
+        grads.append((x.grad, conv.weight.grad, conv.bias.grad))
+    assert all(torch.equal(a, b) for a, b in zip(*grads))
+
+
+def test_train_py_with_kept_copies(cuda, tmp_path):
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, os.path.join(root, "train.py"), "--patch", "64,64,32", "--batch", "2", "--batches", "2", "--epochs", "1", "--act8", "1", "--exp-dir", str(tmp_path)],
+                       capture_output=True, text=True, timeout=110, cwd=root)
+    assert r.returncode == 0, r.stdout[-2000:] + r.stderr[-2000:]
+
+
 def test_conv_bias_act8_refusals(cuda):
     x = torch.zeros(1, 8, 4, 4, device=cuda)
     ok = nn.Conv2d(8, 8, 1).to(cuda)
@@ -210,6 +253,12 @@ def test_conv_bias_act8_refusals(cuda):
                        (nn.Conv2d(8, 8, 3, padding=2, dilation=2), "dilation")):
         with pytest.raises(ValueError, match=what):
             bs.conv_bias_act8(conv.to(cuda), x)
+    with pytest.raises(ValueError, match="unit stride"):
+        bs.conv_bias_act8(nn.Conv2d(8, 8, 3, padding=1, stride=2).to(cuda), x, subsampled=True)
+    with pytest.raises(TypeError):
+        half = nn.Conv2d(8, 8, 1).to(cuda)
+        half.bias = nn.Parameter(half.bias.detach().half())
+        bs.conv_bias_act8(half, x)
     with pytest.raises(ValueError, match="does not fit"):
         bs.conv_bias_act8(ok, x[:, :4])
     with pytest.raises(ValueError, match="residual"):
@@ -223,6 +272,10 @@ def test_conv_bias_act8_refusals(cuda):
     y8 = bs.checkpoint8(x.contiguous(memory_format=torch.channels_last), relu=True)
     with pytest.raises(ValueError):
         bs.act_backward8(x[:, :4], y8)
+    with pytest.raises(ValueError, match="filter"):
+        bs.conv1x1_backward8(torch.zeros(4, 0, device=cuda), torch.zeros(0, 8, device=cuda), bs.checkpoint8(torch.zeros(4, 8, device=cuda)))
+    with pytest.raises(ValueError):
+        bs.act_backward8(torch.zeros(4, 0, device=cuda), bs.checkpoint8(torch.zeros(4, 0, device=cuda), relu=True))
     with pytest.raises(ValueError):
         bs.act_backward8(x, bs.checkpoint8(x.contiguous(memory_format=torch.channels_last)))
     with pytest.raises(TypeError):
@@ -388,8 +441,9 @@ def test_box_head_follows_the_weights_and_refuses_training(cuda):
             net.classifier.conv1[0].weight.fill_(s)
         with bs.mx4_heads(net):
             packs.append(net.classifier.mx4[0].dequantize())
-            with bs.mx4_heads(net):
-                pass
+            with pytest.raises(RuntimeError, match="already"):
+                with bs.mx4_heads(net):
+                    pass
             assert net.classifier.mx4 is not None
     assert bool((packs[0] == 1).all()) and bool((packs[1] == 2).all())
     with pytest.raises(KeyError):
