@@ -51,7 +51,7 @@ struct Args { const float *gy; const uint8_t *yc; const float *w; const uint8_t 
 // Both kernels cut what they load into bf16 pieces once, put the pieces into LDS with the summed axis innermost (32 entries and 8 of padding a row: the
 // 16-byte reads and writes of neighbouring rows fall into different banks) and hold the next step's loads in registers meanwhile.  4 waves, WM x WN of
 // them with TM x TN matrix tiles of 32 x 32 each.
-// 1620 voxels 1536 -> 384: 45 us, 380 TFLOP/s of the 9 products of pieces, and 7 us for the joining.  The cutting, which every tile repeats for its rows (28 % of
+// 1620 voxels 1536 -> 384: 42 us, 410 TFLOP/s of the 9 products of pieces, and 5 us for the joining.  The cutting, which every tile repeats for its rows (a quarter of
 // the VALU's slots), and the waits at two workgroups a CU bound it.  Pieces cut once by a launch of their own and multiplied from L2 without LDS took 10 + 34 us
 // here and twice the time for long narrow maps.
 constexpr int KSTEP = 32, KROW = KSTEP + 8;
@@ -818,11 +818,12 @@ __global__ __launch_bounds__(THREADS, MT * NT <= 3 ? 2 : 1) void conv1x1_bwd_act
     for (int t = threadIdx.x; t < co; t += THREADS) part_b[(long long)blockIdx.x * co + t] = total(1024 * MT * NT + t);
 }
 
-// Tiles of the two products.  gx: 128 x 128 where that gives a workgroup a CU (20000 voxels 300 -> 400: 108 us, 64 x 64 124; 100000 voxels 200 -> 250: 205, 264), else
-// 64 x 64; where even those leave CUs idle, the sum over co is split (at least 4 steps each; 400 voxels 1000 -> 1000: 38 us, unsplit 50) and joined with gw's.  gw: 64 or
+// Tiles of the two products.  gx: 128 channels x 128 voxels where that gives a workgroup a CU (20000 voxels 300 -> 400: 108 us, 64 x 64 124; 100000 voxels 200 -> 250: 205,
+// 264), else 128 x 64, or 64 x 64 where 128 would be padded (1620 voxels 1536 -> 384: 128 x 64 46 us, 64 x 64 52; 16384 voxels 72 -> 288: 31, 36; 6480 voxels 192 -> 768: 57,
+// 48); where even those leave CUs idle, the sum over co is split (at least 4 steps each; 400 voxels 1000 -> 1000: 30 us, unsplit 63, twice as many ranges 32) and joined with gw's.  gw: 64 or
 // 128 along each axis; its sum is split so that both products together fill whole rounds of the two workgroups that a CU holds, at least 128 of them and at least 128
 // voxels each (1620 voxels 1536 -> 384: 13 ranges 64 us, 11 of them 50; 6480 voxels 192 -> 768: 43 ranges 68 us, 17 52).
-struct Plan { int w_m, w_n, d_tile; WgradGrid wg; DgradGrid dg; };
+struct Plan { int w_m, w_n, d_m, d_n; WgradGrid wg; DgradGrid dg; };
 inline Plan plan_of(long long V, int ci, int co)
 {
     Plan p;
@@ -833,11 +834,12 @@ inline Plan plan_of(long long V, int ci, int co)
     w.ci_tiles = (ci + p.w_n - 1) / p.w_n;
     DgradGrid &d = p.dg;
     const long long big = ((V + 127) / 128) * ((ci + 127) / 128);
-    p.d_tile = ci > 64 && big >= 256 ? 128 : 64;
-    d.ci_tiles = (ci + p.d_tile - 1) / p.d_tile;
-    const long long ranges = (V + p.d_tile - 1) / p.d_tile, now = ranges * d.ci_tiles;
+    p.d_n = ci > 64 && big >= 256 ? 128 : 64;
+    p.d_m = p.d_n == 128 || (ci + 63) / 64 % 2 == 0 ? 128 : 64;
+    d.ci_tiles = (ci + p.d_m - 1) / p.d_m;
+    const long long ranges = (V + p.d_n - 1) / p.d_n, now = ranges * d.ci_tiles;
     const int steps = (co + KSTEP - 1) / KSTEP;
-    long long ks = now >= 256 ? 1 : 512 / now;
+    long long ks = (now + 255) / now;
     if (ks > steps / 4) ks = steps / 4;
     if (ks < 1) ks = 1;
     d.k_per = (int)((steps + ks - 1) / ks) * KSTEP;
@@ -860,8 +862,9 @@ void products_launch(const Plan &p, const Args &a, hipStream_t s)
 {
     const dim3 grid((unsigned)(p.wg.groups + p.dg.groups));
     const bool even = a.ci % 4 == 0;                                            // 4 input codes of a voxel lie in one block
-    const auto kernel = p.d_tile == 128 ? (even ? conv1x1_bwd_act8_products<W0, W1, W2, W3, 2, 2, 2, 2, true> : conv1x1_bwd_act8_products<W0, W1, W2, W3, 2, 2, 2, 2, false>)
-                                        : (even ? conv1x1_bwd_act8_products<W0, W1, W2, W3, 2, 1, 2, 1, true> : conv1x1_bwd_act8_products<W0, W1, W2, W3, 2, 1, 2, 1, false>);
+    const auto kernel = p.d_n == 128 ? (even ? conv1x1_bwd_act8_products<W0, W1, W2, W3, 2, 2, 2, 2, true> : conv1x1_bwd_act8_products<W0, W1, W2, W3, 2, 2, 2, 2, false>)
+                      : p.d_m == 128 ? (even ? conv1x1_bwd_act8_products<W0, W1, W2, W3, 2, 2, 2, 1, true> : conv1x1_bwd_act8_products<W0, W1, W2, W3, 2, 2, 2, 1, false>)
+                                     : (even ? conv1x1_bwd_act8_products<W0, W1, W2, W3, 2, 1, 2, 1, true> : conv1x1_bwd_act8_products<W0, W1, W2, W3, 2, 1, 2, 1, false>);
     kernel<<<grid, THREADS, 0, s>>>(a, p.wg, p.dg);
 }
 
