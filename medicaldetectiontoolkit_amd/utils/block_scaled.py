@@ -267,25 +267,26 @@ def conv1x1_backward8(gy, w, x8, y8=None, need_g=False, need_gx=True, need_gw=Tr
     return gx, gw, gbias, (g if write_g else gy if need_g else None)
 
 
-def act_backward8(gy, y8):
-    """(g, gbias) of an activation from its kept output: g = gy * (y > 0), gbias = the sum of g over everything but axis 1.  gy: float32, in any storage order"""
+def act_backward8(gy, y8=None):
+    """(g, gbias) of act(h + bias) from the kept output: g = gy * (y > 0) (y8 None, no activation: gy), gbias = the sum of g over everything but axis 1.
+    gy: float32, in any storage order; g has its channels innermost."""
     if gy.dtype != torch.float32:
         raise TypeError("act_backward8: float32 gradients")
     _lib.require_cuda(gy, "gy")
-    if gy.dim() not in (2, 4, 5) or gy.shape[1] == 0 or y8.shape != tuple(gy.shape) or not y8.relu or not y8.channels_last:
-        raise ValueError("act_backward8: y8 is the kept ReLU output of gy's shape, channels innermost")
-    dev = gy.device
+    shape, dev = tuple(gy.shape), gy.device
+    if len(shape) not in (2, 4, 5) or shape[1] == 0 or (y8 is not None and (y8.shape != shape or not y8.relu or not y8.channels_last)):
+        raise ValueError("act_backward8: gy %s has 2, 4 or 5 axes, y8 is the kept ReLU output of its shape, channels innermost" % (shape,))
     _same_device(dev, y8=y8)
-    mf = _rows_format(gy.dim())
+    mf = _rows_format(len(shape))
     if not gy.is_contiguous(memory_format=mf):
         gy = gy.contiguous(memory_format=mf)
-    co = int(gy.shape[1])
-    V = gy.numel() // co
-    g = torch.empty_like(gy)
-    gbias = torch.empty(co, dtype=torch.float32, device=dev)
-    ws = torch.empty(_lib.lib().mdt_conv1x1_act8_backward_workspace_bytes(V, 1, co), dtype=torch.uint8, device=dev)
-    _call(dev, "mdt_conv1x1_act8_backward", gy.data_ptr(), None, None, None, 0, y8.pointers()[0], None, None, gbias.data_ptr(), g.data_ptr(), V, 1, co, ws.data_ptr(), ws.numel())
-    return g, gbias
+    V = gy.numel() // shape[1]
+    g = torch.empty_like(gy) if y8 is not None else None
+    gbias = torch.empty(shape[1], dtype=torch.float32, device=dev)
+    ws = torch.empty(_lib.lib().mdt_conv1x1_act8_backward_workspace_bytes(V, 1, shape[1]), dtype=torch.uint8, device=dev)
+    _call(dev, "mdt_conv1x1_act8_backward", gy.data_ptr(), None, None, None, 0, y8.pointers()[0] if y8 is not None else None, None, None, gbias.data_ptr(), _ptr(g), V, 1, shape[1],
+          ws.data_ptr(), ws.numel())
+    return (g if y8 is not None else gy), gbias
 
 
 class _ConvBiasAct8(Function):
@@ -332,8 +333,7 @@ class _ConvBiasAct8(Function):
         if ctx.one:
             gx, gw, gbias, g = conv1x1_backward8(gy, w, x8, y8, need_g=ctx.has_res and need_r, need_gx=need_x, need_gw=need_w)
         else:
-            mf = _rows_format(gy.dim())
-            g, gbias = act_backward8(gy, y8) if y8 is not None else fused_epilogue._bias_act_bwd(gy, None, False, mf)
+            g, gbias = act_backward8(gy, y8)
             gx, gw = fused_epilogue._stride1_grads(x8.restore() if need_w else _like(x8), w, ctx.padding, g, need_x, need_w)
         return gx, gw, (gbias if need_b else None), (g if ctx.has_res and need_r else None), None, None, None, None
 

@@ -38,6 +38,8 @@ def test_act_backward8(cuda, shape):
     want = (gy * (y > 0)).double()
     assert g.is_contiguous(memory_format=mf) and torch.equal(g.cpu().double(), want)
     assert torch.equal(gb.cpu().double(), want.transpose(0, 1).reshape(shape[1], -1).sum(1))          # |sum| < 2^24: exact in any order
+    plain, sums = bs.act_backward8(gy.to(cuda))
+    assert torch.equal(plain.cpu(), gy) and torch.equal(sums.cpu().double(), gy.double().transpose(0, 1).reshape(shape[1], -1).sum(1))
     # without a mask, and the sums alone, through the products' entry
     if len(shape) == 2 and shape[0] > 0:
         V, C = shape
@@ -46,6 +48,37 @@ def test_act_backward8(cuda, shape):
         assert out[0] is None and out[1] is None and out[3] is None and torch.equal(out[2].cpu().double(), gy.double().sum(0))
         out = bs.conv1x1_backward8(gy_d, w, x8, y8, need_gx=False, need_gw=True, need_g=True)
         assert torch.equal(out[3], g) and torch.equal(out[2], gb) and not out[1].any()
+
+
+def test_layers_on_two_streams_do_not_share_scratch(cuda):
+    """forward and backward of two layers at once, each on its own stream, equal to one after the other"""
+    jobs = []
+    for seed in (1, 2):
+        one, x0, gy, _ = int_layer(cuda, 3, 18, 72, 1, (32, 32, 32), 1, seed)
+        three, _, gy3, _ = int_layer(cuda, 3, 18, 18, 3, (32, 32, 32), 1, seed + 5)
+        jobs.append((one, three, x0.to(cuda).contiguous(memory_format=torch.channels_last_3d), gy.to(cuda), gy3.to(cuda)))
+
+    def run(one, three, x0, gy, gy3):
+        one.zero_grad(set_to_none=True)
+        three.zero_grad(set_to_none=True)
+        x = x0.clone().requires_grad_()
+        y, _ = bs.conv_bias_act8(one, x, None, relu=True)
+        z, _ = bs.conv_bias_act8(three, x, None, keep=False)
+        ga, = torch.autograd.grad(y, x, gy, retain_graph=True)
+        gb, = torch.autograd.grad(y, one.bias, gy)
+        gc, = torch.autograd.grad(z, three.bias, gy3)
+        return ga, gb, gc
+    want = [run(*j) for j in jobs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for rep in range(5):
+        got = []
+        for j, s in zip(jobs, streams):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                got.append(run(*j))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for w, g in zip(want, got) for a, b in zip(w, g))
 
 
 def test_act_backward8_takes_slices_and_views(cuda):
