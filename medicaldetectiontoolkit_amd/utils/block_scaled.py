@@ -34,9 +34,14 @@ BLOCK = 32
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
+_ENTRIES = {}       # the C entries that were called before, by name
+
+
 def _call(device, name, *args):
     """the C entry on `device`'s current stream"""
-    fn = getattr(_lib.lib(), name)
+    fn = _ENTRIES.get(name)
+    if fn is None:
+        fn = _ENTRIES[name] = getattr(_lib.lib(), name)
     idx = device.index
     if idx == torch._C._cuda_getDevice():                       # (a tensor on the GPU exists: no lazy initialisation to ask for)
         rc = fn(*args, torch._C._cuda_getCurrentRawStream(idx))
@@ -74,24 +79,6 @@ def _no_graph(what, *tensors):
         raise RuntimeError("%s records no autograd graph: call it under torch.no_grad()" % what)
 
 
-def _channels_last_stride(shape):
-    """strides of a dense tensor whose axis 1 is the innermost"""
-    stride, s = [0] * len(shape), shape[1]
-    stride[1] = 1
-    for d in list(range(len(shape) - 1, 1, -1)) + [0]:
-        stride[d] = s
-        s *= shape[d]
-    return tuple(stride)
-
-
-def _row_stride(shape):
-    stride, s = [0] * len(shape), 1
-    for d in range(len(shape) - 1, -1, -1):
-        stride[d] = s
-        s *= shape[d]
-    return tuple(stride)
-
-
 def _rows_format(dim):
     return torch.channels_last_3d if dim == 5 else torch.channels_last if dim == 4 else torch.contiguous_format
 
@@ -103,6 +90,13 @@ def _dense(x):
     if not x.is_contiguous():
         x = x.contiguous()
     return x, x.dim() == 2
+
+
+def _empty(shape, channels_last, dtype, device):
+    """a dense tensor, channels innermost or row-major (with 2 axes both are the same)"""
+    if channels_last and len(shape) > 2:
+        return torch.empty(shape, dtype=dtype, device=device, memory_format=_rows_format(len(shape)))
+    return torch.empty(shape, dtype=dtype, device=device)
 
 
 def _scales_at(n):
@@ -170,32 +164,25 @@ class Checkpoint8(object):
             return cls.of_buffer(tensors[0], *meta)
         return cls.__new__(cls)._set(None, tensors[0], tensors[1], *meta, tensors[0].device)
 
-    @property
-    def stride(self):
-        return _channels_last_stride(self.shape) if self.channels_last else _row_stride(self.shape)
-
     def restore(self):
         """the kept values, in the type, shape and storage order of the tensor they were taken from"""
         _on_gpu(self.device, "Checkpoint8")
-        x = torch.empty_strided(self.shape, self.stride, dtype=self.dtype, device=self.device)
+        x = _empty(self.shape, self.channels_last, self.dtype, self.device)
         codes, scales = self.pointers()
-        _call(self.device, "mdt_act8_restore", codes, scales, x.data_ptr(), x.numel(), _DTYPES[self.dtype], int(self.relu))
+        _call(self.device, "mdt_act8_restore", codes, scales, x.data_ptr(), x.numel(), _DTYPES[self.dtype], self.relu)
         return x
-
-
-def _new_buffer(n, device):
-    return torch.empty(_scales_at(n) + -(-n // BLOCK), dtype=torch.uint8, device=device)
 
 
 def checkpoint8(x, relu=False):
     """x's values in 8 bits.  relu=True: x is the output of a ReLU (values <= 0 read back as 0) and is kept with twice the resolution."""
     _float_tensor(x, "x")
     x, cl = _dense(x)
-    n, device = x.numel(), x.device
-    buffer = _new_buffer(n, device)
+    n, device, dtype = x.numel(), x.device, x.dtype
+    codes = _scales_at(n)
+    buffer = torch.empty(codes + -(-n // BLOCK), dtype=torch.uint8, device=device)
     at = buffer.data_ptr()
-    _call(device, "mdt_act8_quantize", x.data_ptr(), at, at + _scales_at(n), n, _DTYPES[x.dtype], int(relu))
-    return Checkpoint8.of_buffer(buffer, tuple(x.shape), bool(relu), x.dtype, cl)
+    _call(device, "mdt_act8_quantize", x.data_ptr(), at, at + codes, n, _DTYPES[dtype], bool(relu))
+    return Checkpoint8.of_buffer(buffer, tuple(x.shape), bool(relu), dtype, cl)
 
 
 def bias_act_checkpoint8(h, bias, residual=None, relu=True, inplace=False):
@@ -221,10 +208,11 @@ def bias_act_checkpoint8(h, bias, residual=None, relu=True, inplace=False):
         bias = bias.contiguous()
     y = x if inplace else torch.empty_like(x)
     n = x.numel()
-    buffer = _new_buffer(n, device)
+    codes = _scales_at(n)
+    buffer = torch.empty(codes + -(-n // BLOCK), dtype=torch.uint8, device=device)
     if n:
         at = buffer.data_ptr()
-        _call(device, "mdt_bias_act_act8_forward", y.data_ptr(), x.data_ptr(), bias.data_ptr(), _ptr(residual), at, at + _scales_at(n), n, shape[1], inner, int(relu))
+        _call(device, "mdt_bias_act_act8_forward", y.data_ptr(), x.data_ptr(), bias.data_ptr(), _ptr(residual), at, at + codes, n, shape[1], inner, bool(relu))
     return y, Checkpoint8.of_buffer(buffer, tuple(shape), bool(relu), x.dtype, cl)
 
 
@@ -256,7 +244,7 @@ def conv1x1_backward8(gy, w, x8, y8=None, need_g=False, need_gx=True, need_gw=Tr
     if w.stride()[:2] != (ci, 1):
         w = w.detach().reshape(co, ci).contiguous()
     V = gy.numel() // co
-    gx = torch.empty_strided(x8.shape, x8.stride, dtype=torch.float32, device=dev) if need_gx else None
+    gx = _empty(x8.shape, True, torch.float32, dev) if need_gx else None
     gw = torch.empty(w_shape, dtype=torch.float32, device=dev) if need_gw else None
     gbias = torch.empty(co, dtype=torch.float32, device=dev)
     write_g = need_g and y8 is not None
@@ -340,7 +328,7 @@ class _ConvBiasAct8(Function):
 
 def _like(x8):
     """an uninitialised tensor of the kept map's shape and storage order, where only those are asked for"""
-    return torch.empty_strided(x8.shape, x8.stride, dtype=x8.dtype, device=x8.device)
+    return _empty(x8.shape, x8.channels_last, x8.dtype, x8.device)
 
 
 def conv_bias_act8(conv, x, x8=None, residual=None, relu=False, keep=True, subsampled=False):
