@@ -424,11 +424,15 @@ def test_graphed_training_step_with_kept_copies(cuda):
         grads = {n: p.grad.detach().clone() for n, p in net_e.named_parameters() if p.grad is not None}
         torch.manual_seed(1234)
         res_g = step(batch)
-        if k == 0:
-            assert {n: float(v) for n, v in res_g["loss_terms"].items()} == {n: float(v) for n, v in res_e["loss_terms"].items()}
+        assert {n: float(v) for n, v in res_g["loss_terms"].items()} == {n: float(v) for n, v in res_e["loss_terms"].items()}, k
         for n, p in net_g.named_parameters():
-            if n in grads:                   # later steps: a proposal or a sampled anchor may change on the last bit of the library's weight gradients
-                assert float((p.grad - grads[n]).abs().max()) <= (1e-5 if k == 0 else 0.1) * float(grads[n].abs().max()) + 1e-12, (k, n)
+            if n in grads:
+                assert float((p.grad - grads[n]).abs().max()) <= 1e-5 * float(grads[n].abs().max()) + 1e-12, (k, n)
+        # every replay starts from the eager step's weights: the library's weight gradients differ in their last bits from run to run, and two trajectories of their own
+        # part for good where a proposal or a sampled anchor changes on that (a gradient was off by 10.1 % in the third step, once)
+        with torch.no_grad():
+            for a, b in zip(net_g.parameters(), net_e.parameters()):
+                a.copy_(b)
 
 
 # ---- the box head in 4 bits ----------------------------------------------------------------------------------------------------------
