@@ -322,7 +322,8 @@ class _ConvBiasAct8(Function):
             gx, gw, gbias, g = conv1x1_backward8(gy, w, x8, y8, need_g=ctx.has_res and need_r, need_gx=need_x, need_gw=need_w)
         else:
             g, gbias = act_backward8(gy, y8)
-            gx, gw = fused_epilogue._stride1_grads(x8.restore() if need_w else _like(x8), w, ctx.padding, g, need_x, need_w)
+            # w.detach(): the filter is flipped for this call; the buffers that the fp32 layers share belong to one stream
+            gx, gw = fused_epilogue._stride1_grads(x8.restore() if need_w else _like(x8), w.detach(), ctx.padding, g, need_x, need_w)
         return gx, gw, (gbias if need_b else None), (g if ctx.has_res and need_r else None), None, None, None, None
 
 

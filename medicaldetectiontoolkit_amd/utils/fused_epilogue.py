@@ -50,6 +50,11 @@ def _workspace(nbytes, device):
     return ws
 
 
+def _scratch(nbytes, device):
+    """scratch memory of one call, from torch's allocator: calls on several streams at once and captured graphs do not share it"""
+    return torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=device)
+
+
 def _on_current_device(t):
     return t.device.index is None or t.device.index == torch.cuda.current_device()
 
@@ -306,7 +311,9 @@ def _flip_single(w, out, cl):
 def flip_transpose_filter(w, mf):
     """w [cout, cin, *k] -> [cin, cout, *k] with every spatial axis reversed, dense in memory format `mf`: served from the per-step batched
     launch (_FlipCache) for parameters, one launch of mdt_filter_flip_transpose for other fp32 GPU tensors dense in `mf`, torch ops otherwise.
-    The returned tensor of the cached path is a persistent buffer: valid until the weights change (read it within the step)."""
+    The returned tensor of the cached path is a persistent buffer: valid until the weights change (read it within the step), and on the stream that the steps
+    run on (a refresh is queued on the stream of the first request and other streams do not wait for it).  A caller whose layers may run on several
+    streams, or inside a graph that torch.cuda.graph captures, passes w.detach(): its filter is flipped for the call, into memory of its own."""
     nd = w.dim() - 2
     if w.is_cuda and w.dtype == torch.float32 and w.is_contiguous(memory_format=mf) and _on_current_device(w):
         # (never inside a hipGraph capture: the graph would bake the address of the record table, which is rebuilt -- and its old tensor freed -- as soon as
@@ -438,7 +445,7 @@ def conv_win_weight_grad(gy, x, w):
         return None
     if not gy.is_contiguous(memory_format=torch.channels_last_3d):
         gy = gy.contiguous(memory_format=torch.channels_last_3d)
-    ws = _workspace(L.mdt_conv_win_wgrad_workspace_bytes(B, Y, X, Z, Ci, Co, k), gy.device)
+    ws = _scratch(L.mdt_conv_win_wgrad_workspace_bytes(B, Y, X, Z, Ci, Co, k), gy.device)
     gw = torch.empty((Co, k, k, k, Ci), dtype=torch.float32, device=gy.device)
     rc = L.mdt_conv_win_wgrad(gy.data_ptr(), x.data_ptr(), gw.data_ptr(), B, Y, X, Z, Ci, Co, k, ws.data_ptr(), ws.numel(), _lib.raw_stream())
     if rc == _lib.MDT_ERR_UNSUPPORTED:
@@ -469,7 +476,7 @@ def conv3x3x3_small_weight_grad(gy, x, w):
     if not gy.is_contiguous(memory_format=torch.channels_last_3d):
         gy = gy.contiguous(memory_format=torch.channels_last_3d)
     wsb = L.mdt_conv3x3x3_small_wgrad_workspace_bytes(B, Y, X, cin, cout)
-    ws = _workspace(wsb, gy.device)
+    ws = _scratch(wsb, gy.device)
     gw = torch.empty((3, 3, 3, cin, cout), dtype=torch.float32, device=gy.device)
     rc = L.mdt_conv3x3x3_small_wgrad(x.data_ptr(), gy.data_ptr(), gw.data_ptr(), B, Y, X, Z, cin, cout, ws.data_ptr(), ws.numel(),
                                      _lib.raw_stream())
