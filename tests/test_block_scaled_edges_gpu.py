@@ -1,6 +1,7 @@
-"""Block-scaled operators (utils/block_scaled.py) at their edges: layers whose passes run on several streams or inside a captured graph.
+"""Block-scaled operators (utils/block_scaled.py) at their edges: layers whose passes run on several streams or inside a captured graph, every kernel of the 1x1 backward pass and
+of the 4-bit product, the ends of the number range, tensors of more than 2^31 values.
 
-Layers are compared on small integers, where all products and sums are exact in fp32: equality."""
+Compared on numbers whose products and sums are exact in fp32: equality."""
 import copy
 
 import pytest
@@ -8,8 +9,10 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from medicaldetectiontoolkit_amd import _lib
 from medicaldetectiontoolkit_amd.utils import block_scaled as bs
 from medicaldetectiontoolkit_amd.utils import fused_epilogue as fe
+from tests.test_block_scaled_gpu import BIG, DTYPES, f64, hard_values, kept4, kept8, layer, same
 from tests.test_block_scaled_models_gpu import int_layer
 
 pytestmark = pytest.mark.gpu
@@ -99,3 +102,280 @@ def test_layers_captured_and_replayed(cuda):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(outs, want)), rep
         assert all(torch.equal(a, b) for a, b in zip(step(*copy.deepcopy((window, one))), want)), rep
+
+
+# ---- the tiled and one-pass kernels of the 1x1 backward pass ---------------------------------------------------------------------------
+def backward_variant(V, ci, co, need_gx=True, need_gw=True):
+    """the kernels that mdt_conv1x1_act8_backward takes, restated: (one-pass tiles,) or (gw tile, gx tile, gx's sum split, input channels a multiple of 4)"""
+    if V * ci < 4 or V * co < 4:
+        return ("tiny",)
+    mt, nt = -(-co // 32), -(-ci // 32)
+    if need_gx and need_gw and co <= 160 and ci <= 160 and mt * nt <= 10:
+        ks, wave = -(-co // 16), (32 * max(co, ci) + 32 * mt + (32 * ci + 32 * nt) // 2 + 3) // 4 * 4
+        lds = max(nt * ks * 3072 + 4 * wave * 4, (4 if mt * nt <= 9 else 2) * (1024 * mt * nt + 32 * mt) * 4)
+        if lds <= 160 * 1024:
+            return (mt, nt)
+    gw = (128 if co > 64 else 64, 128 if ci > 64 else 64) if need_gw else None
+    gx = split = None
+    if need_gx:
+        dn = 128 if ci > 64 and -(-V // 128) * -(-ci // 128) >= 256 else 64
+        dm = 128 if dn == 128 or -(-ci // 64) % 2 == 0 else 64
+        now, steps = -(-V // dn) * -(-ci // dm), -(-co // 32)
+        gx, split = (dm, dn), max(1, min(-(-256 // now), steps // 4)) > 1
+    return gw, gx, split, ci % 4 == 0
+
+
+# one-pass: a tile a side and the others; tiled: gw 128 x 128, 128 x 64, 64 x 128, gx 64 x 64, 128 x 64, 128 x 128 (split and not), channels that are multiples of 4 or not
+VARIANTS = [(700, 18, 72), (700, 72, 18), (1100, 36, 144), (1100, 144, 36), (900, 96, 96), (901, 31, 160), (903, 160, 29), (600, 64, 64), (500, 37, 300), (500, 36, 300), (450, 200, 300), (450, 201, 300),
+            (460, 300, 40), (460, 301, 40), (17000, 100, 200), (17000, 101, 200), (20001, 37, 170), (20003, 36, 170), (16389, 200, 65), (16390, 202, 66), (11003, 300, 40), (11003, 301, 63),
+            (32771, 101, 200), (32771, 104, 200), (16500, 150, 70), (16500, 148, 70), (450, 150, 300), (450, 152, 300), (20000, 170, 33), (20000, 172, 33), (450, 330, 17), (450, 332, 17), (450, 150, 70), (450, 152, 70),
+            (601, 31, 33), (3, 1, 1)]
+
+
+def test_the_cases_reach_every_kernel_of_the_backward_pass():
+    seen = {backward_variant(*s) for s in VARIANTS}
+    for ci4 in (True, False):
+        for gw in ((128, 128), (128, 64), (64, 128)):
+            got = {(v[1], v[2]) for v in seen if len(v) == 4 and v[0] == gw and v[3] == ci4}
+            want = {((64, 64), False)} if gw == (128, 64) else {((64, 64), False), ((128, 64), False), ((128, 128), False)}
+            assert want <= got, (gw, ci4, want - got)
+        assert any(len(v) == 4 and v[2] and v[3] == ci4 and v[1] == t for v in seen for t in ((64, 64),)) and any(len(v) == 4 and v[2] and v[3] == ci4 and v[1] == (128, 64) for v in seen)
+    assert {(3, 1), (1, 3), (5, 2), (2, 5), (3, 3), (5, 1), (1, 5), (2, 2)} <= seen
+
+
+def single_products(V, ci, co, seed, cuda):
+    """(g, w, x) of which every gx and every gw is one product: row v of g holds one value, at v % co, and of x the value at (v // co) % ci, rows behind co * ci none; powers
+    of two where the other factor has all its bits"""
+    gen = torch.Generator().manual_seed(seed)
+    v = torch.arange(V)
+    at_o, at_i, one = v % co, v // co % ci, v < co * ci
+    x = torch.zeros(V, ci)
+    x[v[one], at_i[one]] = torch.exp2(torch.randint(0, 4, (int(one.sum()),), generator=gen).float())
+
+    def bits(*shape):
+        return torch.randint(2 ** 23, 2 ** 24, shape, generator=gen).float() * (torch.randint(0, 2, shape, generator=gen) * 2 - 1)
+
+    def powers(*shape):
+        return torch.exp2(torch.randint(-3, 4, shape, generator=gen).float())
+    cases = []
+    for gv, w in ((bits(V), powers(co, ci)), (powers(V), bits(co, ci))):
+        g = torch.zeros(V, co)
+        g[v, at_o] = gv
+        cases.append((g, w, torch.exp2(torch.randint(-40, 40, (V, 1), generator=gen).float())))
+    return x.to(cuda), [(g.to(cuda), w.to(cuda), s.to(cuda)) for g, w, s in cases]
+
+
+@pytest.mark.parametrize("V,ci,co", VARIANTS)
+def test_conv1x1_backward8_keeps_all_bits_of_a_product(cuda, V, ci, co):
+    """gradients and filters of 24 significant bits: the three pieces that a float is cut into are all needed, at any size of the gradient"""
+    x, cases = single_products(V, ci, co, V + ci, cuda)
+    x8 = bs.checkpoint8(x, relu=True)
+    assert torch.equal(x8.restore(), x)
+    for g, w, size in cases:
+        for scale in (1.0, size):
+            gs = g * scale
+            gx, gw, gb, _ = bs.conv1x1_backward8(gs, w, x8, None)
+            gd, wd, xd = gs.double(), w.double(), x.double()
+            assert torch.equal(gx.double(), gd @ wd) and torch.equal(gw.double(), gd.t() @ xd)
+            for kw in (dict(need_gx=False), dict(need_gw=False)):
+                part = bs.conv1x1_backward8(gs, w, x8, None, **kw)
+                assert all(a is None or torch.equal(a, b) for a, b in zip(part[:2], (gx, gw)))
+
+
+@pytest.mark.parametrize("relu", [True, False])
+@pytest.mark.parametrize("V,ci,co", VARIANTS)
+def test_conv1x1_backward8_variants_on_integers(cuda, V, ci, co, relu):
+    """every kernel, masked or not, with and without the residual's gradient, its parts alone: |sums| < 2^24, so the results are the exact ones"""
+    x, gy, w, y = layer(V, ci, co, True, V + ci, cuda)
+    gy = gy.clamp(-4, 4)                                              # 32771 voxels of 15 * 4
+    x8, y8 = bs.checkpoint8(x, relu=True), bs.checkpoint8(y, relu=True) if relu else None
+    m = gy * (y > 0) if relu else gy
+    want = (m.double() @ w.double(), m.double().t() @ x.double(), m.double().sum(0))
+    for kw in (dict(need_g=True), dict(), dict(need_gx=False), dict(need_gw=False), dict(need_gw=False, need_g=True), dict(need_gx=False, need_g=True)):
+        got = bs.conv1x1_backward8(gy, w, x8, y8, **kw)
+        assert all(a is None or torch.equal(a.double(), b) for a, b in zip(got, want))
+        assert got[3] is None or torch.equal(got[3], m)
+
+
+@pytest.mark.parametrize("V,ci,co", [s for s in VARIANTS if s[0] > 3])
+def test_conv1x1_backward8_variants_keep_fp32_accuracy(cuda, V, ci, co):
+    """every kernel on floats, the error in 2-norm: products are off by 2^-23 at most (what three pieces leave out), and an fp32 sum of values of either sign by a random walk of
+    roundings that stays below 16 of them for 2^15 values in partial sums"""
+    x, gy, w, y = layer(V, ci, co, False, V + co, cuda)
+    x8, y8 = bs.checkpoint8(x, relu=True), bs.checkpoint8(y, relu=True)
+    gx, gw, gb, _ = bs.conv1x1_backward8(gy, w, x8, y8)
+    md, xd = (gy * (y > 0)).double(), x8.restore().double()
+    for got, want in ((gw, md.t() @ xd), (gx, md @ w.double()), (gb, md.sum(0))):
+        assert float((got.double() - want).norm() / want.norm()) < 16 * 2.0 ** -24
+
+
+# ---- the 4-bit product's kernels -------------------------------------------------------------------------------------------------------
+def linear_variant(rows, k, n, size):
+    """the kernel that mdt_mx4_linear takes, restated: (shape, W's form, 16-row tiles of x, 16-column tiles)"""
+    wide = n > 144 and (rows >= 2048 or (rows >= 512 and k >= 4096))
+    copies = wide or (rows >= 256 and k >= 4096)
+    if wide:
+        ranges = -(-n // 768)
+        short, long = -(-(-(-rows // 16) * ranges) // 256), -(-(-(-rows // 48) * ranges) // 256)
+        return "wide", "copied", 1 if 6 * short < 10 * long else 3, min(6, max(2, -(-n // (128 * ranges))))
+    if not copies and rows * k < 16 // size:
+        return "narrow", "tiny", 1, 1
+    t = -(-rows // 16)
+    tn = 9 if n > 48 and t * -(-n // 144) >= 96 else 3 if n > 16 and t * -(-n // 48) >= 96 else 1
+    return "narrow", "copied" if copies else "one block" if k <= 32 else "kept", 1, tn
+
+
+LINEAR_MORE = [(261, 4099, 9), (777, 4131, 47), (1601, 4100, 47), (1601, 4100, 141), (600, 4200, 200), (1700, 4097, 300), (2051, 100, 200), (2051, 100, 300), (2051, 100, 500), (2051, 100, 600), (2051, 100, 767),
+               (4099, 70, 150), (4099, 70, 380), (4099, 70, 500), (4099, 70, 600), (4099, 70, 767), (4099, 300, 900), (1601, 31, 100), (1601, 29, 47), (40, 17, 300), (1601, 290, 100), (1603, 290, 47),
+               (50, 290, 33), (1, 3, 7)]
+
+
+def test_the_cases_reach_every_kernel_of_the_4_bit_product():
+    for size in (2, 4):
+        seen = {linear_variant(*s, size) for s in LINEAR_MORE}
+        assert {("wide", "copied", tm, tn) for tm in (1, 3) for tn in (2, 3, 4, 5, 6)} <= seen
+        assert all((linear_variant(*s, size)[1] == "copied") == (_lib.lib().mdt_mx4_linear_workspace_bytes(*s) > 0) for s in LINEAR_MORE)
+        assert {("narrow", w, 1, tn) for w in ("copied", "one block", "kept") for tn in (1, 3, 9)} | {("narrow", "tiny", 1, 1)} <= seen
+
+
+@pytest.mark.parametrize("relu", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,k,n", LINEAR_MORE)
+def test_mx4_linear_variants_on_integers(cuda, rows, k, n, dtype, relu):
+    """numbers that 4 bits hold exactly, sums below 2^24: the exact result, rounded once to the type"""
+    g = torch.Generator().manual_seed(rows + n)
+    vals = torch.tensor([0.0, 1, 2, 3, 4, 6, -1, -2, -3, -4, -6])
+    x, w = vals[torch.randint(0, 11, (rows, k), generator=g)].to(cuda), vals[torch.randint(0, 11, (n, k), generator=g)].to(cuda)
+    bias = torch.randint(-9, 9, (n,), generator=g).float().to(cuda)
+    y = bs.mx4_linear(x.to(dtype), bs.mx4_quantize(w), bias, relu=relu)
+    want = x.double() @ w.double().t() + bias.double()
+    assert y.dtype == dtype and torch.equal(y, (want.clamp(min=0) if relu else want).to(dtype))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,k,n", LINEAR_MORE)
+def test_mx4_linear_variants_on_floats(cuda, rows, k, n, dtype):
+    """exact products, k fp32 sums and the bias, then one rounding: half a step each"""
+    g = torch.Generator().manual_seed(rows + k)
+    x = (torch.randn(rows, k, generator=g) * torch.exp(torch.randn(k, generator=g))).to(dtype)
+    w, bias = torch.randn(n, k, generator=g) / k ** 0.5, torch.randn(n, generator=g)
+    y = bs.mx4_linear(x.to(cuda), bs.mx4_quantize(w.to(cuda)), bias.to(cuda))
+    xv, wv = (torch.from_numpy(kept4(f64(t), BIG[t.dtype])[0]).to(cuda) for t in (x, w))
+    want = xv @ wv.t() + bias.to(cuda).double()
+    tol = (k + 64) * 2.0 ** -24 * (xv.abs() @ wv.abs().t() + bias.to(cuda).abs().double()) + torch.finfo(dtype).eps / 2 * want.abs()
+    assert bool(((y.double() - want).abs() <= tol * (1 + 1e-6)).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,n", [(70, 512), (300, 512), (2100, 512)])
+def test_mx4_linear_rounds_x_as_mx4_quantize_does(cuda, rows, n, dtype):
+    """W = the unit matrix: a row of x comes back as its 4-bit values.  Ties, subnormals and numbers of very different size in whole chunks and ragged ones; a row with an infinity or a NaN is NaN,
+    and no other row"""
+    x = hard_values(rows * n, dtype, rows)
+    x[~torch.isfinite(x)] = 1
+    x[x.abs() > BIG[dtype] / 4] = 5                                   # (a sum of one value rounded up across the type's largest is an infinity, no saturated code)
+    x = x.view(rows, n)
+    x[5] = x[0].roll(32)
+    if dtype == torch.float16:
+        x[7, :64] = torch.arange(64) * 2.0 ** -24                     # fp16's smallest numbers
+        x[8, :64] = torch.arange(64) * 2.0 ** -20 - 2.0 ** -15
+    elif dtype == torch.bfloat16:
+        x[7, :64] = (torch.arange(64).double() * 2.0 ** -133).to(dtype)
+        x[8, :64] = (torch.arange(64).double() * 2.0 ** -126).to(dtype)
+    ties = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0]).repeat(8)
+    x[9, :64], x[10, :64], x[11, :64] = ties, -ties * 2.0 ** 3, ties.to(dtype) * (1 + torch.finfo(dtype).eps)
+    eye = bs.mx4_quantize(torch.eye(n, device=cuda))
+    xd = x.to(cuda)
+    v = torch.from_numpy(kept4(f64(x), BIG[dtype])[0]).to(dtype)
+    assert torch.equal(bs.mx4_linear(xd, eye).cpu(), v)
+    at = {3: float("inf"), 20: float("nan"), 33: -float("inf"), rows - 1: float("nan")}
+    for r, bad in at.items():
+        xd[r, 37 * r % n] = bad
+    y = bs.mx4_linear(xd, eye).cpu()
+    assert all(torch.isnan(y[r]).all() for r in at)
+    keep = torch.tensor([r not in at for r in range(rows)])
+    assert torch.equal(y[keep], v[keep])
+
+
+def test_two_streams_and_copies_of_w(cuda):
+    """products that copy W into scratch memory, another W and another size on each stream"""
+    jobs = []
+    for i, (rows, k, n) in enumerate([(300, 5292, 144), (700, 4200, 200), (2500, 600, 400), (300, 4100, 33)]):
+        x, w = torch.randn(rows, k, device=cuda), bs.mx4_quantize(torch.randn(n, k, device=cuda))
+        assert _lib.lib().mdt_mx4_linear_workspace_bytes(rows, k, n) > 0
+        jobs.append((x, w, bs.mx4_linear(x, w)))
+    torch.cuda.synchronize()
+    streams, outs = [torch.cuda.Stream() for _ in jobs], []
+    for rep in range(6):
+        for s, (x, w, want) in zip(streams, jobs):
+            with torch.cuda.stream(s):
+                outs.append((bs.mx4_linear(x, w), want))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in outs)
+
+
+# ---- tensors of more than 2^31 values --------------------------------------------------------------------------------------------------
+def around(n):
+    """ranges of indexes at the start, around 2^31 and at the end"""
+    return [slice(0, 4096), slice(2 ** 31 - 4096, min(n, 2 ** 31 + 4096)), slice(n - 4099, n)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_checkpoint8_of_more_than_2_31_values(cuda, dtype):
+    n = 2 ** 31 + 100037
+    x = torch.empty(n, dtype=dtype, device=cuda)
+    x.copy_(torch.randn(10007, device=cuda).repeat(-(-n // 10007))[:n])
+    ck = bs.checkpoint8(x, relu=True)
+    back = ck.restore()
+    for s in around(n):
+        first = s.start // 32 * 32
+        q, b, v = kept8(f64(x[first:s.stop]), True, BIG[dtype])
+        assert same(f64(back[first:s.stop]), v) and same(ck.codes[first:s.stop].cpu().numpy(), q)
+        assert same(ck.scales[first // 32:-(-s.stop // 32)].cpu().numpy()[:s.stop // 32 - first // 32], b[:s.stop // 32 - first // 32])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_mx4_of_more_than_2_31_values(cuda, dtype):
+    rows, k = 2 ** 31 // 4500 + 23, 4500
+    x = torch.empty(rows * k, dtype=dtype, device=cuda)
+    x.copy_(torch.randn(10007, device=cuda).repeat(-(-rows * k // 10007))[:rows * k])
+    x = x.view(rows, k)
+    m = bs.mx4_quantize(x)
+    back = m.dequantize()
+    picks = [0, 1, 2 ** 31 // 4500 - 1, 2 ** 31 // 4500, 2 ** 31 // 4500 + 1, rows - 1]
+    v = kept4(f64(x[picks]), BIG[dtype])[0]
+    assert same(f64(back[picks]), v)
+    del back
+    w = torch.zeros(9, k, device=cuda)
+    w[torch.arange(9), torch.arange(9) * 501] = 1
+    y = bs.mx4_linear(x, bs.mx4_quantize(w))
+    assert same(f64(y[picks]), v[:, ::501][:, :9])
+
+
+@pytest.mark.parametrize("V,ci,co", [(2 ** 31 // 72 + 1001, 72, 72), (2 ** 31 // 300 + 77, 300, 330)])
+def test_conv1x1_backward8_of_more_than_2_31_values(cuda, V, ci, co):
+    """gradients at a few voxels of a map whose offsets pass 31 bits; the sums alone, the mask and the epilogue on the same map"""
+    at = torch.tensor([0, 1, 2 ** 31 // co - 1, 2 ** 31 // co, 2 ** 31 // co + 1, 2 ** 31 // ci - 1, 2 ** 31 // ci, V - 2, V - 1])
+    at = at[at < V].unique().to(cuda)
+    x = torch.zeros(V, ci, device=cuda)
+    x[at] = torch.randint(1, 16, (len(at), ci), device=cuda).float()
+    x8 = bs.checkpoint8(x, relu=True)
+    del x
+    y8 = bs.Checkpoint8(torch.ones(V * co, dtype=torch.uint8, device=cuda), torch.full((-(-V * co // 32),), 127, dtype=torch.uint8, device=cuda), (V, co), relu=True)
+    gy = torch.zeros(V, co, device=cuda)
+    gy[at] = torch.randint(-8, 9, (len(at), co), device=cuda).float()
+    w = torch.randint(-8, 9, (co, ci), device=cuda).float()
+    gx, gw, gb, g = bs.conv1x1_backward8(gy, w, x8, y8, need_g=True)
+    gd = gy[at].double()
+    xd = x8.codes.view(V, ci)[at].double()
+    assert torch.equal(g[at], gy[at]) and int(g.count_nonzero()) == int(gy.count_nonzero())
+    want = gd @ w.double()
+    assert torch.equal(gx[at].double(), want) and int(gx.count_nonzero()) == int(want.count_nonzero())
+    scale = torch.stack([x8.scales[(a * ci + torch.arange(ci, device=cuda)) // 32].double() for a in at])
+    assert torch.equal(gw.double(), gd.t() @ (xd * torch.exp2(scale - 127))) and torch.equal(gb.double(), gd.sum(0))
+    del gx, g
+    g, gb = bs.act_backward8(gy, y8)
+    assert torch.equal(g[at], gy[at]) and torch.equal(gb.double(), gd.sum(0)) and int(g.count_nonzero()) == int(gy.count_nonzero())
+    del g
+    y, ck = bs.bias_act_checkpoint8(gy, torch.full((co,), 2.0, device=cuda), relu=True)
+    assert torch.equal(y[at], (gy[at] + 2).clamp(min=0)) and float(y[V // 2].min()) == 2.0 and int((ck.codes > 0).sum()) == int((y > 0).sum())
