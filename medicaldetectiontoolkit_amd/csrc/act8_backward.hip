@@ -6,7 +6,8 @@
 //
 // Both products run on the bf16 matrix units with fp32 accumulation and lose nothing that fp32 would keep: a float is the exact sum of three bf16
 // numbers (each the nearest to what the ones before leave), x^ IS a bf16 number, so gw takes 3 matrix instructions a tile and gx 6 (the three products
-// left out are at most 2^-24 of the whole, of either sign).
+// left out are at most 2^-24 of the whole, of either sign).  That holds from 2^-110 to the largest float; smaller ones are off by less than 2^-133, half a
+// step of the smallest bf16 numbers.
 #include "block_scaled.h"
 
 namespace {
@@ -29,6 +30,19 @@ __device__ __forceinline__ unsigned round2(float &a, float &b)
     return p;
 }
 
+// round2 for the first piece: a finite value that would round to an infinity (from 3.3962e38 on) gets the largest bf16 number (mid is up to 2^-7 of it then).  An infinity leaves one for
+// the next piece and a NaN is left over, so neither becomes finite.  One instruction a value.
+__device__ __forceinline__ unsigned first2(float &a, float &b)
+{
+    const float big = Largest<__bf16>::v;
+    float p = __builtin_amdgcn_fmed3f(a, -big, big), q = __builtin_amdgcn_fmed3f(b, -big, big);
+    const v2f t = {p, q};
+    const unsigned w = __builtin_bit_cast(unsigned, __builtin_convertvector(t, v2bf));
+    a = a - __uint_as_float(w << 16);
+    b = b - __uint_as_float(w & 0xffff0000u);
+    return w;
+}
+
 // 8 floats -> their three bf16 pieces: |mid| <= 2^-8 |x|, |lo| <= 2^-17 |x|, hi + mid + lo = x
 struct Split8 { v8bf hi, mid, lo; };
 __device__ __forceinline__ Split8 split8(const float (&v)[8])
@@ -38,7 +52,7 @@ __device__ __forceinline__ Split8 split8(const float (&v)[8])
     for (int q = 0; q < 4; ++q) {
         float a = v[2 * q], b = v[2 * q + 1];
 #pragma unroll
-        for (int k = 0; k < 3; ++k) p[k][q] = round2(a, b);
+        for (int k = 0; k < 3; ++k) p[k][q] = k == 0 ? first2(a, b) : round2(a, b);
     }
     return {__builtin_bit_cast(v8bf, p[0]), __builtin_bit_cast(v8bf, p[1]), __builtin_bit_cast(v8bf, p[2])};
 }
@@ -104,8 +118,8 @@ __device__ __forceinline__ void put4(uint16_t *to, int plane, v4f v)
 #pragma unroll
     for (int k = 0; k < 3; ++k) {
         uint2 p;
-        p.x = round2(a, b);
-        p.y = round2(c, d);
+        p.x = k == 0 ? first2(a, b) : round2(a, b);
+        p.y = k == 0 ? first2(c, d) : round2(c, d);
         *reinterpret_cast<uint2 *>(to + k * plane) = p;
     }
 }

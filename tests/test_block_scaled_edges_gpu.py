@@ -209,6 +209,46 @@ def test_conv1x1_backward8_variants_keep_fp32_accuracy(cuda, V, ci, co):
         assert float((got.double() - want).norm() / want.norm()) < 16 * 2.0 ** -24
 
 
+EXTREME = [(40, 18, 72), (40, 72, 18), (40, 37, 300), (40, 300, 40), (40, 200, 300), (33000, 101, 200), (2, 1, 1)]
+
+
+@pytest.mark.parametrize("V,ci,co", EXTREME)
+def test_conv1x1_backward8_of_the_largest_finite_values(cuda, V, ci, co):
+    """gradients and filters between the largest bf16 and the largest fp32 number: a finite product stays what it is"""
+    x, cases = single_products(V, ci, co, 7, cuda)
+    x = x.clamp(max=1)
+    x[min(V, co):] = 0
+    x8 = bs.checkpoint8(x, relu=True)
+    top = torch.finfo(torch.float32).max
+    for k, (g, w, _) in enumerate(cases):
+        g = torch.sign(g)
+        g[min(V, co):] = 0                                            # a value a column: no sum passes the largest number
+        w = torch.sign(torch.randn(co, ci, generator=torch.Generator().manual_seed(3))).to(cuda)
+        big = torch.rand(g.shape if k == 0 else w.shape, generator=torch.Generator().manual_seed(4)).to(cuda) * (top - 3.39e38) + 3.39e38
+        big.view(-1)[0] = top
+        g, w = (g * big, w * 0.5) if k == 0 else (g * 0.5, w * big)
+        gx, gw, gb, gr = bs.conv1x1_backward8(g, w, x8, None, need_g=True)
+        gd = g.double()
+        assert torch.isfinite(gd @ w.double()).all() and torch.equal(gx.double(), gd @ w.double())
+        assert torch.equal(gw.double(), gd.t() @ x.double()) and torch.equal(gb.double(), gd.sum(0)) and torch.equal(gr, g)
+
+
+@pytest.mark.parametrize("V,ci,co", [(40, 18, 72), (40, 37, 300), (450, 300, 40)])
+def test_conv1x1_backward8_of_the_smallest_values(cuda, V, ci, co):
+    """a piece below 2^-133 does not exist in bf16: gradients keep all their bits from 2^-110 on, and smaller ones are off by less than 2^-133"""
+    x, cases = single_products(V, ci, co, 11, cuda)
+    x = x.clamp(max=1)
+    x8 = bs.checkpoint8(x, relu=True)
+    g, w, _ = cases[0]
+    w = torch.sign(w)
+    for e in (-86, -133, -140, -149):                                # the last: numbers around the smallest normal one
+        gs = (g.double() * 2.0 ** e).float()
+        gx, gw, gb, _ = bs.conv1x1_backward8(gs, w, x8, None)
+        gd = gs.double()
+        tol = 0 if e >= -133 else 2.0 ** -133
+        assert bool(((gx.double() - gd @ w.double()).abs() <= tol).all()) and bool(((gw.double() - gd.t() @ x.double()).abs() <= tol).all()), e
+
+
 # ---- the 4-bit product's kernels -------------------------------------------------------------------------------------------------------
 def linear_variant(rows, k, n, size):
     """the kernel that mdt_mx4_linear takes, restated: (shape, W's form, 16-row tiles of x, 16-column tiles)"""
