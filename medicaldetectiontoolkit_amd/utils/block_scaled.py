@@ -21,6 +21,7 @@ another stream is the caller's to synchronise, as with any torch operator.  Thei
 calls on several streams and captured graphs do not share any."""
 import contextlib
 import math
+import threading
 
 import torch
 import torch.nn.functional as F
@@ -469,6 +470,9 @@ def mx4_linear(x, w4, bias=None, relu=False):
     return y
 
 
+_HEADS = threading.Lock()       # a head is looked at and taken in one step
+
+
 @contextlib.contextmanager
 def mx4_heads(net):
     """A Mask R-CNN's box head (the two products of every region, `classifier.conv1` and `conv2`) in 4 bits while the context lasts: the filters are rounded when it is
@@ -480,9 +484,10 @@ def mx4_heads(net):
     if not (isinstance(head.conv1, fused_epilogue.ConvBiasReLU) and isinstance(head.conv2, fused_epilogue.ConvBiasReLU)
             and tuple(head.conv1[0].kernel_size) == tuple(head.pool_size) and not any(head.conv1[0].padding)):
         raise ValueError("mx4_heads: the box head's layers are convolution + ReLU without a norm, the first as large as the pooled region")
-    if head.mx4 is not None:
-        raise RuntimeError("mx4_heads: the net's head is in 4 bits already")
-    head.mx4 = tuple(mx4_quantize(c[0].weight.detach().flatten(1)) for c in (head.conv1, head.conv2))
+    with _HEADS:
+        if head.mx4 is not None:
+            raise RuntimeError("mx4_heads: the net's head is in 4 bits already")
+        head.mx4 = tuple(mx4_quantize(c[0].weight.detach().flatten(1)) for c in (head.conv1, head.conv2))
     try:
         yield net
     finally:

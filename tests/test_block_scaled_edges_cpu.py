@@ -1,0 +1,68 @@
+"""What the block-scaled operators (utils/block_scaled.py) refuse and how their contexts behave where that needs no GPU."""
+import threading
+
+import pytest
+import torch
+import torch.nn as nn
+
+from medicaldetectiontoolkit_amd.utils import block_scaled as bs
+from medicaldetectiontoolkit_amd.utils import fused_epilogue as fe
+
+
+def box_net():
+    net, head = nn.Module(), nn.Module()
+    head.pool_size, head.mx4 = (3, 3), None
+    head.conv1, head.conv2 = fe.ConvBiasReLU(nn.Conv2d(2, 4, 3), nn.ReLU()), fe.ConvBiasReLU(nn.Conv2d(4, 4, 1), nn.ReLU())
+    net.classifier = head
+    return net
+
+
+def test_of_two_threads_one_enters_mx4_heads(monkeypatch):
+    """the second one raises also while the first one's filters are being rounded, and does not switch the head back"""
+    net = box_net()
+    rounding, go_on, inside, leave = threading.Event(), threading.Event(), threading.Event(), threading.Event()
+
+    def slow(w):
+        rounding.set()
+        assert go_on.wait(20)
+        return w
+    monkeypatch.setattr(bs, "mx4_quantize", slow)
+    errors = []
+
+    def first():
+        with bs.mx4_heads(net):
+            inside.set()
+            assert leave.wait(20)
+
+    def second():
+        try:
+            with bs.mx4_heads(net):
+                pass
+        except RuntimeError as e:
+            errors.append(str(e))
+    threads = [threading.Thread(target=first), threading.Thread(target=second)]
+    threads[0].start()
+    assert rounding.wait(20)
+    threads[1].start()                            # (it waits for the first one's rounding, or finds the head taken)
+    threads[1].join(0.2)
+    go_on.set()
+    assert inside.wait(20)
+    threads[1].join(20)
+    held = net.classifier.mx4
+    leave.set()
+    threads[0].join(20)
+    assert len(errors) == 1 and "already" in errors[0] and held is not None and net.classifier.mx4 is None
+
+
+def test_mx4_heads_leaves_the_head_free_when_rounding_fails(monkeypatch):
+    net = box_net()
+
+    def broken(w):
+        raise MemoryError
+    monkeypatch.setattr(bs, "mx4_quantize", broken)
+    with pytest.raises(MemoryError):
+        bs.mx4_heads(net).__enter__()
+    monkeypatch.setattr(bs, "mx4_quantize", lambda w: w)
+    with bs.mx4_heads(net):
+        assert net.classifier.mx4 is not None
+    assert net.classifier.mx4 is None
