@@ -24,6 +24,7 @@ import math
 import threading
 
 import torch
+import torch.nn as nn
 import torch.nn.functional as F
 from torch.autograd import Function
 from torch.autograd.function import once_differentiable
@@ -338,6 +339,8 @@ def conv_bias_act8(conv, x, x8=None, residual=None, relu=False, keep=True, subsa
     input was sub-sampled already): the autograd node keeps x8, x's 8-bit copy (None: one is made), and y's in place of x and y.  y8 is what the next
     layer takes as its x8; keep=False: there is none (an output that no further layer of this kind reads; None where there is no activation either).
     float32 maps on the GPU; a row-major x is copied to channels-last."""
+    if not isinstance(conv, (nn.Conv2d, nn.Conv3d)):
+        raise ValueError("conv_bias_act8: a Conv2d or Conv3d, not %s" % type(conv).__name__)
     for name, ok in (("a bias", conv.bias is not None), ("one group", conv.groups == 1), ("unit dilation", all(int(v) == 1 for v in conv.dilation)),
                      ("zero padding", conv.padding_mode == "zeros" and not isinstance(conv.padding, str)),
                      ("a size-preserving window", not isinstance(conv.padding, str) and all(2 * int(p) + 1 == int(k) for p, k in zip(conv.padding, conv.kernel_size))),

@@ -66,3 +66,11 @@ def test_mx4_heads_leaves_the_head_free_when_rounding_fails(monkeypatch):
     with bs.mx4_heads(net):
         assert net.classifier.mx4 is not None
     assert net.classifier.mx4 is None
+
+
+@pytest.mark.parametrize("conv", [nn.ConvTranspose3d(8, 8, 3, padding=1), nn.ConvTranspose2d(8, 8, 1), nn.Conv1d(8, 8, 1), nn.ConvTranspose1d(8, 8, 1)])
+def test_conv_bias_act8_takes_convolutions_in_2d_and_3d_only(conv):
+    """a transposed layer with as many channels out as in has the attributes and the filter's shape of a convolution, and another result"""
+    x = torch.zeros((1, 8) + (4,) * (conv.weight.dim() - 2))
+    with pytest.raises(ValueError, match="Conv2d or Conv3d"):
+        bs.conv_bias_act8(conv, x)
