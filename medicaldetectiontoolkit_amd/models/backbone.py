@@ -24,6 +24,10 @@ def _lateral(conv, x, top_down):
     return conv(x) + top_down
 
 
+def _hooked(module):
+    """whether the module or one inside it carries hooks, which run only where the module is called"""
+    return any(m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks for m in module.modules())
+
 
 class ResBlock(nn.Module):
     def __init__(self, start_filts, planes, conv, stride=1, downsample=None, norm=None, relu="relu"):
@@ -173,41 +177,62 @@ class FPN(nn.Module):
             if strided:
                 tap, x = fused_epilogue.stride_tap(x, blk.conv1[0].stride)
                 x_lat = tap if i == 0 else x_lat
-                x8 = block_scaled.checkpoint8(x, relu=True)
+                x8 = block_scaled.checkpoint8(x, relu=x8.relu)
             res = x if blk.downsample is None else conv8(blk.downsample, x, x8, keep=False, subsampled=strided)[0]
             h, h8 = conv8(blk.conv1[0], x, x8, relu=True, subsampled=strided)
             h, h8 = conv8(blk.conv2[0], h, h8, relu=True)
             x, x8 = conv8(blk.conv3, h, h8, residual=res, relu=True)
         return x, x8, x_lat
 
-    def _forward8(self, x):
-        """forward with cf.act8_checkpoints: the same values; the residual stages, the laterals and the P convolutions keep 8-bit copies for the backward pass"""
-        conv8, up = block_scaled.conv_bias_act8, fused_epilogue.upsample_nearest
-        c0_out = self._c0(x)
-        c1_out = None
-        if not self.operate_stride1 and fused_epilogue.stem_pool_fused_applies(self.C1, self.C2[0], c0_out):
-            h = fused_epilogue.conv_stem_bias_relu_pool(self.C1, c0_out)
-        else:
-            c1_out = self.C1(c0_out)
-            h = self.C2[0](c1_out)
+    @staticmethod
+    def _kept(h, relu):
+        """h in channels-last storage and its 8-bit copy (relu: h is a ReLU's output; what a hook returned may be anything)"""
         mf = torch.channels_last_3d if h.dim() == 5 else torch.channels_last
         if not h.is_contiguous(memory_format=mf):
             h = h.contiguous(memory_format=mf)
-        h8 = block_scaled.checkpoint8(h, relu=True)
+        return h, block_scaled.checkpoint8(h, relu=relu)
+
+    def _forward8(self, x):
+        """forward with cf.act8_checkpoints: the same values; the residual stages, the laterals and the P convolutions keep 8-bit copies for the backward pass.  These layers' modules
+        are not called: a stage or a P convolution with hooks runs as it does without the option, and keeps what it keeps there."""
+        conv8, up = block_scaled.conv_bias_act8, fused_epilogue.upsample_nearest
+        c0_out = self._c0(x)
+        c1_out = None
+        fused = not self.operate_stride1 and fused_epilogue.stem_pool_fused_applies(self.C1, self.C2[0], c0_out)
+        if fused:
+            h = fused_epilogue.conv_stem_bias_relu_pool(self.C1, c0_out)
+        else:
+            c1_out = self.C1(c0_out)
+        if not _hooked(self.C2):
+            h, h8 = self._kept(h, True) if fused else self._kept(self.C2[0](c1_out), not _hooked(self.C1))
+            h, h8, _ = self._stage8(list(self.C2)[1:], h, h8)
+        else:
+            if fused:
+                for blk in list(self.C2)[1:]:
+                    h = blk(h)
+            else:
+                h = self.C2(c1_out)
+            h, h8 = self._kept(h, False)
         levels = []                                     # (what the lateral reads, its copy) of C2 ...
-        for i, seq in enumerate([list(self.C2)[1:], self.C3, self.C4, self.C5] + ([self.C6] if self.sixth_pooling else [])):
-            below = (h8,)
-            h, h8, lat = self._stage8(seq, h, h8)
-            if i > 0:
-                levels.append((lat,) + below)
+        for seq in [self.C3, self.C4, self.C5] + ([self.C6] if self.sixth_pooling else []):
+            below = h8
+            if not _hooked(seq):
+                h, h8, lat = self._stage8(seq, h, h8)
+            else:
+                h, lat = self._stage(seq, h)
+                h, h8 = self._kept(h, False)
+            levels.append((lat, below))
         levels.append((h, h8))
         ones = [self.P2_conv1, self.P3_conv1, self.P4_conv1, self.P5_conv1] + ([self.P6_conv1] if self.sixth_pooling else [])
         threes = [self.P2_conv2, self.P3_conv2, self.P4_conv2, self.P5_conv2] + ([self.P6_conv2] if self.sixth_pooling else [])
-        pre, outs = None, []
-        for (c, c8), one, three in zip(reversed(levels), reversed(ones), reversed(threes)):
-            pre, pre8 = conv8(one, c, c8, residual=None if pre is None else up(pre, 2))
-            outs.append(conv8(three, pre, pre8, keep=False)[0])
-        outs = outs[::-1]
+        pre, pres = None, []
+        for (c, c8), one in zip(reversed(levels), reversed(ones)):
+            if not _hooked(one):
+                pre, pre8 = conv8(one, c, c8, residual=None if pre is None else up(pre, 2))
+            else:
+                pre, pre8 = one(c) if pre is None else _lateral_up(one, c, pre), None
+            pres.append((pre, pre8))
+        outs = [three(p) if _hooked(three) else conv8(three, p, p8, keep=False)[0] for three, (p, p8) in zip(threes, reversed(pres))]
         if self.operate_stride1:
             p1_pre_out = _lateral(self.P1_conv1, c1_out, self.P2_upsample(pre))
             p0_pre_out = _lateral(self.P0_conv1, c0_out, self.P1_upsample(p1_pre_out))

@@ -1,5 +1,5 @@
 """Block-scaled operators (utils/block_scaled.py) at their edges: layers whose passes run on several streams or inside a captured graph, every kernel of the 1x1 backward pass and
-of the 4-bit product, the ends of the number range, tensors of more than 2^31 values.
+of the 4-bit product, the ends of the number range, tensors of more than 2^31 values, backbones with hooks and in other forms.
 
 Compared on numbers whose products and sums are exact in fp32: equality."""
 import copy
@@ -13,7 +13,7 @@ from medicaldetectiontoolkit_amd import _lib
 from medicaldetectiontoolkit_amd.utils import block_scaled as bs
 from medicaldetectiontoolkit_amd.utils import fused_epilogue as fe
 from tests.test_block_scaled_gpu import BIG, DTYPES, f64, hard_values, kept4, kept8, layer, same
-from tests.test_block_scaled_models_gpu import int_layer
+from tests.test_block_scaled_models_gpu import int_layer, mf_of, rel, two_nets
 
 pytestmark = pytest.mark.gpu
 
@@ -419,3 +419,89 @@ def test_conv1x1_backward8_of_more_than_2_31_values(cuda, V, ci, co):
     del g
     y, ck = bs.bias_act_checkpoint8(gy, torch.full((co,), 2.0, device=cuda), relu=True)
     assert torch.equal(y[at], (gy[at] + 2).clamp(min=0)) and float(y[V // 2].min()) == 2.0 and int((ck.codes > 0).sum()) == int((y > 0).sum())
+
+
+# ---- the backbone: hooks, switches, other forms ----------------------------------------------------------------------------------------
+def pyramid(net, img):
+    fpn = net.Fpn if hasattr(net, "Fpn") else net.fpn
+    fpn.zero_grad(set_to_none=True)
+    outs = fpn(img)
+    gen = torch.Generator().manual_seed(2)
+    sum((o * torch.randn(o.shape, generator=gen).to(o.device)).sum() for o in outs).backward()
+    return fpn, [o.detach() for o in outs], {n: p.grad for n, p in fpn.named_parameters() if p.grad is not None}
+
+
+def image_of(net, kw, cuda):
+    img = torch.randn([kw["batch_size"], net.cf.n_channels] + kw["patch_size"], generator=torch.Generator().manual_seed(1)).to(cuda)
+    return img.contiguous(memory_format=mf_of(img)) if kw.get("channels_last") else img
+
+
+@pytest.fixture
+def repeatable(kw):
+    """MIOpen's 2D convolutions split sums over atomics: two passes of one net differ in their last bits, and a unit of a ReLU that is zero but for these bits has a gradient in the one and
+    none in the other.  Torch's own convolutions there (MIOpen's 3D ones are deterministic): the forward values of two nets are equal, and so are their masks"""
+    with torch.backends.cudnn.flags(enabled=kw["dim"] == 3):
+        yield
+
+
+def same_pyramids(a, b, img, kw):
+    """channels-last nets: the stages' outputs of the fp32 path bit for bit; bias gradients within 50 layers' roundings of a sum of either sign over all voxels, filters' gradients within what half a
+    step of a block allows.  Row-major nets run other kernels of the library with the option than without, so only their outputs are compared (see repeatable)"""
+    (_, o0, g0), (_, o1, g1) = a, b
+    assert len(o0) == len(o1) and set(g0) == set(g1)
+    if not kw.get("channels_last"):
+        assert all(p.shape == q.shape and rel(q, p) < 1e-6 for p, q in zip(o0, o1))
+        return
+    front = len(o0) - (5 if kw.get("sixth_pooling") else 4)          # levels behind the interpolations of a stride-1 pyramid, which have a kernel for each memory layout
+    assert all(torch.equal(p, q) for p, q in zip(o0[front:], o1[front:])) and all(rel(q, p) < 1e-6 for p, q in zip(o0[:front], o1[:front]))
+    bias_tol = 50 * 2.0 ** -24 * (img.numel() / img.shape[1]) ** 0.5
+    for n in g0:
+        assert rel(g1[n], g0[n]) < (bias_tol if n.endswith("bias") else 0.02), (n, rel(g1[n], g0[n]))
+
+
+HOOKED = [dict(dim=3, model="mrcnn", patch_size=[64, 64, 32], batch_size=1, channels_last=True), dict(dim=2, model="mrcnn", patch_size=[96, 64], batch_size=2, channels_last=True),
+          dict(dim=2, model="mrcnn", patch_size=[64, 64], batch_size=1)]
+
+
+@pytest.mark.parametrize("kw", HOOKED)
+def test_hooks_run_as_without_copies(cuda, repeatable, kw):
+    """hooks of every kind on every module: the same ones run, in the same order"""
+    seen, res = [], []
+    for net in two_nets(cuda, kw):
+        names = []
+        fpn = net.Fpn if hasattr(net, "Fpn") else net.fpn
+        for n, m in fpn.named_modules():
+            m.register_forward_hook(lambda m, i, o, n=n, names=names: names.append(n))
+            m.register_forward_pre_hook(lambda m, i, n=n, names=names: names.append("pre " + n))
+        img = image_of(net, kw, cuda)
+        res.append(pyramid(net, img))
+        seen.append(names)
+    assert seen[0] == seen[1] and any("C4.1.conv2" == n for n in seen[0]) and any("P2_conv2" == n for n in seen[0])
+    same_pyramids(*res, img, kw)
+
+
+@pytest.mark.parametrize("where", [("C1",), ("C2.0",), ("C2.1",), ("C3.0.conv2", "P5_conv1"), ("C4.2.conv3", "P3_conv2"), ("C5.1.conv1",), ("C5.2",), ("P2_conv2", "P4_conv2")])
+@pytest.mark.parametrize("kw", HOOKED[:2])
+def test_a_hook_that_changes_an_output(cuda, repeatable, kw, where):
+    """also to values of the other sign, behind a ReLU"""
+    res = []
+    for net in two_nets(cuda, kw):
+        fpn = net.Fpn if hasattr(net, "Fpn") else net.fpn
+        modules = dict(fpn.named_modules())
+        for n in where:
+            modules[n].register_forward_hook(lambda m, i, o: o * -1.5)
+        img = image_of(net, kw, cuda)
+        res.append(pyramid(net, img))
+    same_pyramids(*res, img, kw)
+
+
+@pytest.mark.parametrize("kw", [dict(dim=3, model="mrcnn", patch_size=[64, 64, 32], batch_size=1, channels_last=True, sixth_pooling=True),
+                                dict(dim=2, model="mrcnn", patch_size=[128, 96], batch_size=2, channels_last=True, res_architecture="resnet101"),
+                                dict(dim=2, model="retina_unet", patch_size=[96, 64], batch_size=2, channels_last=True), dict(dim=2, model="retina_unet", patch_size=[64, 64], batch_size=1)])
+def test_other_backbones_with_kept_copies(cuda, repeatable, kw):
+    """a sixth level, the deep architecture, the 2D pyramid at unit stride"""
+    res = []
+    for net in two_nets(cuda, kw):
+        img = image_of(net, kw, cuda)
+        res.append(pyramid(net, img))
+    same_pyramids(*res, img, kw)
