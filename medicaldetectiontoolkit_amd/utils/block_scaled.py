@@ -293,7 +293,7 @@ class _ConvBiasAct8(Function):
         one = math.prod(w.shape[2:]) == 1
         bias = bias.detach().contiguous()
         y = y8 = None
-        if one and x.numel() >= (1 << 20) and x.data_ptr() % 16 == 0 and w.stride()[:2] == (w.shape[1], 1) and _lib.lib().mdt_conv1x1_forward_supported(int(w.shape[1]), int(w.shape[0])):
+        if one and fused_epilogue.ENABLED and fused_epilogue.CONV1X1_FWD and x.numel() >= (1 << 20) and x.data_ptr() % 16 == 0 and w.stride()[:2] == (w.shape[1], 1) and _lib.lib().mdt_conv1x1_forward_supported(int(w.shape[1]), int(w.shape[0])):
             y = fused_epilogue._conv1x1_forward(x, w, bias, residual, relu)
         elif nd == 3 and residual is None and padding == (1, 1, 1) and not x.is_contiguous():
             y = fused_epilogue.conv3x3x3_small(x, w, bias, relu)

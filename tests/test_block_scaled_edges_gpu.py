@@ -495,6 +495,22 @@ def test_a_hook_that_changes_an_output(cuda, repeatable, kw, where):
     same_pyramids(*res, img, kw)
 
 
+def test_the_switch_of_the_1x1_kernel_holds(cuda, monkeypatch):
+    """a layer that the kernel would take, with and without it"""
+    conv, x0, gy, _ = int_layer(cuda, 3, 18, 72, 1, (64, 64, 32), 1, 9)
+    calls, real = [], fe._conv1x1_forward
+    monkeypatch.setattr(fe, "_conv1x1_forward", lambda *a: calls.append(1) or real(*a))
+    outs = []
+    for on, enabled in ((True, True), (False, True), (True, False)):
+        monkeypatch.setattr(fe, "CONV1X1_FWD", on)
+        monkeypatch.setattr(fe, "ENABLED", enabled)
+        x = x0.to(cuda).contiguous(memory_format=torch.channels_last_3d).requires_grad_()
+        y, y8 = bs.conv_bias_act8(conv, x, None, relu=True)
+        outs.append((y.detach(), y8.restore()) + torch.autograd.grad(y, [x, conv.weight, conv.bias], gy.to(cuda)))
+        assert len(calls) == 1
+    assert all(torch.equal(a, b) for o in outs[1:] for a, b in zip(o, outs[0]))
+
+
 @pytest.mark.parametrize("kw", [dict(dim=3, model="mrcnn", patch_size=[64, 64, 32], batch_size=1, channels_last=True, sixth_pooling=True),
                                 dict(dim=2, model="mrcnn", patch_size=[128, 96], batch_size=2, channels_last=True, res_architecture="resnet101"),
                                 dict(dim=2, model="retina_unet", patch_size=[96, 64], batch_size=2, channels_last=True), dict(dim=2, model="retina_unet", patch_size=[64, 64], batch_size=1)])
