@@ -36,14 +36,9 @@ BLOCK = 32
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
-_ENTRIES = {}       # the C entries that were called before, by name
-
-
 def _call(device, name, *args):
     """the C entry on `device`'s current stream"""
-    fn = _ENTRIES.get(name)
-    if fn is None:
-        fn = _ENTRIES[name] = getattr(_lib.lib(), name)
+    fn = getattr(_lib.lib(), name)
     idx = device.index
     if idx == torch._C._cuda_getDevice():                       # (a tensor on the GPU exists: no lazy initialisation to ask for)
         rc = fn(*args, torch._C._cuda_getCurrentRawStream(idx))

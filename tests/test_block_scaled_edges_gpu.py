@@ -521,3 +521,17 @@ def test_other_backbones_with_kept_copies(cuda, repeatable, kw):
         img = image_of(net, kw, cuda)
         res.append(pyramid(net, img))
     same_pyramids(*res, img, kw)
+
+
+def test_calls_are_counted_only_while_they_are(cuda):
+    """_lib.count_calls sees these operators' entries, whatever was called before, and nothing of it stays"""
+    x = torch.randn(64, device=cuda)
+    bs.checkpoint8(x).restore()
+    _lib.count_calls(True)
+    try:
+        bs.checkpoint8(x).restore()
+        seen = dict(_lib.CALLS)
+    finally:
+        _lib.count_calls(False)
+    bs.checkpoint8(x).restore()
+    assert seen == {"mdt_act8_quantize": 1, "mdt_act8_restore": 1} == _lib.CALLS
