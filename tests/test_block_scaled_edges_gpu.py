@@ -445,8 +445,8 @@ def repeatable(kw):
 
 
 def same_pyramids(a, b, img, kw):
-    """channels-last nets: the stages' outputs of the fp32 path bit for bit; bias gradients within 50 layers' roundings of a sum of either sign over all voxels, filters' gradients within what half a
-    step of a block allows.  Row-major nets run other kernels of the library with the option than without, so only their outputs are compared (see repeatable)"""
+    """channels-last nets: the stages' outputs of the fp32 path bit for bit; bias gradients within 50 layers' roundings of a sum of values of either sign over the map's voxels (2^-24 a layer of
+    the sum of magnitudes, sqrt(voxels) times the sum itself), filters' gradients within what half a step of a block allows.  Row-major nets run other kernels of the library with the option than without, so only their outputs are compared (see repeatable)"""
     (_, o0, g0), (_, o1, g1) = a, b
     assert len(o0) == len(o1) and set(g0) == set(g1)
     if not kw.get("channels_last"):
@@ -454,9 +454,10 @@ def same_pyramids(a, b, img, kw):
         return
     front = len(o0) - (5 if kw.get("sixth_pooling") else 4)          # levels behind the interpolations of a stride-1 pyramid, which have a kernel for each memory layout
     assert all(torch.equal(p, q) for p, q in zip(o0[front:], o1[front:])) and all(rel(q, p) < 1e-6 for p, q in zip(o0[:front], o1[:front]))
-    bias_tol = 50 * 2.0 ** -24 * (img.numel() / img.shape[1]) ** 0.5
     for n in g0:
-        assert rel(g1[n], g0[n]) < (bias_tol if n.endswith("bias") else 0.02), (n, rel(g1[n], g0[n]))
+        level = int(n[1])                                             # C3.0.conv1.0.bias, P5_conv2.weight
+        voxels = o0[front + level - 2][:, 0].numel() if level >= 2 else img[:, 0].numel()
+        assert rel(g1[n], g0[n]) < (50 * 2.0 ** -24 * voxels ** 0.5 if n.endswith("bias") else 0.02), (n, rel(g1[n], g0[n]))
 
 
 HOOKED = [dict(dim=3, model="mrcnn", patch_size=[64, 64, 32], batch_size=1, channels_last=True), dict(dim=2, model="mrcnn", patch_size=[96, 64], batch_size=2, channels_last=True),
@@ -512,15 +513,44 @@ def test_the_switch_of_the_1x1_kernel_holds(cuda, monkeypatch):
 
 
 @pytest.mark.parametrize("kw", [dict(dim=3, model="mrcnn", patch_size=[64, 64, 32], batch_size=1, channels_last=True, sixth_pooling=True),
+                                dict(dim=3, model="mrcnn", patch_size=[128, 128, 64], batch_size=2, channels_last=True),
                                 dict(dim=2, model="mrcnn", patch_size=[128, 96], batch_size=2, channels_last=True, res_architecture="resnet101"),
                                 dict(dim=2, model="retina_unet", patch_size=[96, 64], batch_size=2, channels_last=True), dict(dim=2, model="retina_unet", patch_size=[64, 64], batch_size=1)])
 def test_other_backbones_with_kept_copies(cuda, repeatable, kw):
-    """a sixth level, the deep architecture, the 2D pyramid at unit stride"""
+    """a sixth level, larger maps, the deep architecture, the 2D pyramid at unit stride"""
     res = []
     for net in two_nets(cuda, kw):
         img = image_of(net, kw, cuda)
         res.append(pyramid(net, img))
     same_pyramids(*res, img, kw)
+
+
+@pytest.mark.parametrize("k,size,B", [(1, (4, 4, 4), 0), (3, (4, 4, 4), 0), (1, (4, 6), 0), (3, (4, 6), 0), (1, (1, 1, 1), 1), (3, (1, 1, 1), 1), (3, (1, 1), 1)])
+@pytest.mark.parametrize("relu", [True, False])
+def test_layers_without_voxels_and_with_one(cuda, k, size, B, relu):
+    nd = len(size)
+    conv, x, gy, r = int_layer(cuda, nd, 6, 10, k, size, B, 3)
+    x, r = x.to(cuda).requires_grad_(), r.to(cuda).requires_grad_()
+    y, y8 = bs.conv_bias_act8(conv, x, None, residual=r, relu=relu)
+    got = torch.autograd.grad(y, [x, r, conv.weight, conv.bias], gy.to(cuda))
+    assert y.shape == gy.shape and y8.shape == tuple(gy.shape) and y8.restore().shape == gy.shape
+    xd, rd, w, b = (t.detach().cpu().double().requires_grad_() for t in (x, r, conv.weight, conv.bias))
+    h = (F.conv3d if nd == 3 else F.conv2d)(xd, w, b, padding=k // 2) + rd
+    want = torch.autograd.grad(h.relu() if relu else h, [xd, rd, w, b], gy.double())
+    assert all(p.shape == q.shape and torch.equal(p.cpu().double(), q) for p, q in zip(got, want))
+
+
+def test_a_map_without_extent_is_refused_as_by_any_convolution(cuda):
+    conv, x, _, _ = int_layer(cuda, 3, 6, 10, 1, (0, 4, 4), 2, 3)
+    for call in (lambda t: F.conv3d(t, conv.weight), lambda t: bs.conv_bias_act8(conv, t, None)):
+        with pytest.raises(RuntimeError, match="[Kk]ernel size"):
+            call(x.to(cuda))
+
+
+def test_checkpoint8_of_a_single_value_without_axes(cuda):
+    for v in (3.0, -0.75, 0.0):
+        back = bs.checkpoint8(torch.tensor(v, device=cuda)).restore()
+        assert back.shape == () and float(back) == v
 
 
 def test_calls_are_counted_only_while_they_are(cuda):
