@@ -723,7 +723,7 @@ int mdt_bias_act_act8_forward(float *y, const float *x, const float *bias, const
 /*
  * Backward pass of y = act(conv1x1(x, w) + bias (+ residual)) on channels-last rows from the 8-bit copies of x and y:
  *   g = gy * (y code > 0)  (y_codes NULL: g = gy),   gx[v][i] = sum_o g[v][o] * w[o][i],   gw[o][i] = sum_v g[v][o] * x^[v][i],   gbias[o] = sum_v g[v][o]
- * with fp32 products and sums in a fixed order (deterministic).  w: [c_out][c_in]; x_codes / x_scales: n_voxels * c_in values in storage order, x_relu their
+ * with fp32 products and sums in a fixed order (deterministic; gradients and filters below 2^-110 count to within 2^-133).  w: [c_out][c_in]; x_codes / x_scales: n_voxels * c_in values in storage order, x_relu their
  * kind; gx, gw, gbias, g may each be NULL (not wanted; without gx w may be NULL, without gw the codes and scales of x).  A non-finite gradient gives non-finite results (an infinity may become a NaN).
  */
 size_t mdt_conv1x1_act8_backward_workspace_bytes(long long n_voxels, int c_in, int c_out);

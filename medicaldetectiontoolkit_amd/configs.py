@@ -32,7 +32,7 @@ class Configs(object):
         self.n_latent_dims = 0
         self.operate_stride1 = False
         # training memory: the maps of the residual stages and of the pyramid kept for the backward pass in 8 bits (utils/block_scaled.py;
-        # fp32 steps of nets without norms and with ReLU; steps under autocast keep what they kept)
+        # fp32 steps of nets without norms and with ReLU.  Steps under autocast ignore it; so do stages and P convolutions that carry hooks)
         self.act8_checkpoints = False
         # optimiser / schedule (:104, 113-114, 219)
         self.num_epochs = 100

@@ -65,7 +65,7 @@ struct Args { const float *gy; const uint8_t *yc; const float *w; const uint8_t 
 // Both kernels cut what they load into bf16 pieces once, put the pieces into LDS with the summed axis innermost (32 entries and 8 of padding a row: the
 // 16-byte reads and writes of neighbouring rows fall into different banks) and hold the next step's loads in registers meanwhile.  4 waves, WM x WN of
 // them with TM x TN matrix tiles of 32 x 32 each.
-// 1620 voxels 1536 -> 384: 42 us, 410 TFLOP/s of the 9 products of pieces, and 5 us for the joining.  The cutting, which every tile repeats for its rows (a quarter of
+// 1620 voxels 1536 -> 384: 43 us, 400 TFLOP/s of the 9 products of pieces, and 5 us for the joining (both launches in a queue of calls: 43 - 47 us).  The cutting, which every tile repeats for its rows (a quarter of
 // the VALU's slots), and the waits at two workgroups a CU bound it.  Pieces cut once by a launch of their own and multiplied from L2 without LDS took 10 + 34 us
 // here and twice the time for long narrow maps.
 constexpr int KSTEP = 32, KROW = KSTEP + 8;
@@ -590,7 +590,7 @@ __host__ __device__ constexpr int fused_regions(int tiles) { return tiles <= 9 ?
 // and leaves as the contiguous run that it is, like g.
 // Used while gw takes at most 10 tiles of 32 x 32 of a side of at most 160 (what registers hold): narrow layers gain (100000 voxels 32 -> 160: 48 us, tiled 70; 36 -> 144: 59,
 // 67; 144 -> 36: 56, 68), square ones are equal (64 -> 64: 53, 50; 96 -> 64: 47, 45; 64 -> 96: 45, 48).
-// 1 M voxels 18 -> 72 with g: 163 us, 4.8 TB/s of its 155 us floor; 72 -> 18: 121 us, 3.9 TB/s (floor 95): memory, and the waits of a wave's chunk where no other wave covers
+// 1 M voxels 18 -> 72 with g: 163 us, 4.8 TB/s of its 155 us floor; 72 -> 18: 118 us, 4.0 TB/s (floor 95); 131072 voxels 36 -> 144 with g: 70 us (floor 39), 144 -> 36: 59 (24): memory, and the waits of a wave's chunk where no other wave covers
 // them.  A call of few voxels is one chunk's chain of loads, LDS and products: 32 voxels 8 us.
 // Loads and stores share one in-order counter: the next chunk's loads are issued before this chunk's stores and every chunk issues the same number of
 // stores, so that the wait for the loads does not wait for the stores behind them.
@@ -836,7 +836,8 @@ __global__ __launch_bounds__(THREADS, MT * NT <= 3 ? 2 : 1) void conv1x1_bwd_act
 // 264), else 128 x 64, or 64 x 64 where 128 would be padded (1620 voxels 1536 -> 384: 128 x 64 46 us, 64 x 64 52; 16384 voxels 72 -> 288: 31, 36; 6480 voxels 192 -> 768: 57,
 // 48); where even those leave CUs idle, the sum over co is split (at least 4 steps each; 400 voxels 1000 -> 1000: 30 us, unsplit 63, twice as many ranges 32) and joined with gw's.  gw: 64 or
 // 128 along each axis; its sum is split so that both products together fill whole rounds of the two workgroups that a CU holds, at least 128 of them and at least 128
-// voxels each (1620 voxels 1536 -> 384: 13 ranges 64 us, 11 of them 50; 6480 voxels 192 -> 768: 43 ranges 68 us, 17 52).
+// voxels each (1620 voxels 1536 -> 384: 13 ranges 64 us, 11 of them 50; 6480 voxels 192 -> 768: 43 ranges 68 us, 17 52).  Figures of whole calls, host work included.  The rules for both
+// sums hold at these sizes; 1300 voxels 1000 -> 1000 they cost 8 us (63 -> 71).
 struct Plan { int w_m, w_n, d_m, d_n; WgradGrid wg; DgradGrid dg; };
 inline Plan plan_of(long long V, int ci, int co)
 {

@@ -63,7 +63,7 @@ __device__ __forceinline__ unsigned group_max(unsigned v)
     return v;
 }
 
-// n / d for 0 <= n < 2^31 by a multiplication (d >= 1): m = floor(2^32 (2^s - d) / d) + 1 with s = ceil(log2 d)
+// n / d for 0 <= n < 2^31 by a multiplication (d >= 1), Granlund and Montgomery's division by an invariant integer: m = floor(2^32 (2^s - d) / d) + 1 with s = ceil(log2 d)
 struct FastDiv {
     unsigned d, mul, shift;
     __host__ explicit FastDiv(unsigned dd = 1) : d(dd)

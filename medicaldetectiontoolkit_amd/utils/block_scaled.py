@@ -4,8 +4,8 @@
 32 consecutive values share one power of two 2^e (scale byte e + 127), the smallest with which no value of the block is clipped:
 max|x| <= Q * 2^e with Q = 255 for the outputs of a ReLU, 127 for signed values in 8 bits, 6 for the magnitudes 0, .5, 1, 1.5, 2, 3, 4, 6 of 4 bits.
 Values are rounded to the nearest code, ties to the even one: a kept value is off by at most half a step of its block, max / 255 (ReLU), max / 127
-(signed).  A positive ReLU output keeps at least the code 1, so the codes hold the ReLU's mask exactly.  A block with an infinity or a NaN reads
-back as NaN.
+(signed).  A positive ReLU output keeps at least the code 1 (below half a step it is off by less than a whole one), so the codes hold the ReLU's mask
+exactly.  A block with an infinity or a NaN reads back as NaN.
 
   checkpoint8(x)                      -> Checkpoint8, .restore()      any float32 / bfloat16 / float16 tensor, 33 bytes for 32 values
   bias_act_checkpoint8(h, bias, res)  -> (y, Checkpoint8 of y)        the convolution epilogue of utils/fused_epilogue.bias_act that keeps the copy
@@ -18,7 +18,7 @@ What calls them: models/backbone.FPN with cf.act8_checkpoints (train.py --act8 1
 
 Like every operator of this package they run on the GPU only and are queued on the current stream of the tensors' device; a tensor that was made on
 another stream is the caller's to synchronise, as with any torch operator.  Their scratch memory comes from torch's allocator for each call, so
-calls on several streams and captured graphs do not share any."""
+calls on several streams and captured graphs do not share any.  (The backbone around them keeps its fp32 layers, whose buffers belong to one stream.)"""
 import contextlib
 import math
 import threading
@@ -277,7 +277,7 @@ def act_backward8(gy, y8=None):
 class _ConvBiasAct8(Function):
     """y = act(conv(x) + bias (+ residual)) whose backward pass finds x and y in 8 bits: a quarter of the memory that autograd would hold from the forward pass to the
     backward pass.  The forward values are those of the fp32 layer; the ReLU's mask, the input gradient and the bias gradient are exact, the weight
-    gradient is taken with the kept x (off by at most half a step of its block)."""
+    gradient is taken with the kept x."""
 
     @staticmethod
     def forward(ctx, x, w, bias, residual, x8, relu, keep, padding):

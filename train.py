@@ -48,7 +48,7 @@ def main():
                     "semantics and state-dict format); 0: torch.optim.Adam itself")
     ap.add_argument("--adam-absent-grad", default="skip", choices=["skip", "zero_after_first"], help="a parameter without a gradient in a step: skip it "
                     "(torch >= 2, default) or update it with a zero gradient once it has had one (torch 0.4.1, the reference's pinned version)")
-    ap.add_argument("--act8", type=int, default=0, help="1: the backbone's maps kept for the backward pass in 8 bits (cf.act8_checkpoints)")
+    ap.add_argument("--act8", type=int, default=0, help="1: the backbone's maps kept for the backward pass in 8 bits (cf.act8_checkpoints; fp32 steps)")
     args = ap.parse_args()
 
     world = int(os.environ.get("WORLD_SIZE", "1"))
