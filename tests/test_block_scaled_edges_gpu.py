@@ -112,7 +112,7 @@ def backward_variant(V, ci, co, need_gx=True, need_gw=True):
     mt, nt = -(-co // 32), -(-ci // 32)
     if need_gx and need_gw and co <= 160 and ci <= 160 and mt * nt <= 10:
         ks, wave = -(-co // 16), (32 * max(co, ci) + 32 * mt + (32 * ci + 32 * nt) // 2 + 3) // 4 * 4
-        lds = max(nt * ks * 3072 + 4 * wave * 4, (4 if mt * nt <= 9 else 2) * (1024 * mt * nt + 32 * mt) * 4)
+        lds = max(nt * ks * 3 * 1024 + 4 * wave * 4, (4 if mt * nt <= 9 else 2) * (1024 * mt * nt + 32 * mt) * 4)
         if lds <= 160 * 1024:
             return (mt, nt)
     gw = (128 if co > 64 else 64, 128 if ci > 64 else 64) if need_gw else None
