@@ -537,7 +537,11 @@ def test_layers_without_voxels_and_with_one(cuda, k, size, B, relu):
     xd, rd, w, b = (t.detach().cpu().double().requires_grad_() for t in (x, r, conv.weight, conv.bias))
     h = (F.conv3d if nd == 3 else F.conv2d)(xd, w, b, padding=k // 2) + rd
     want = torch.autograd.grad(h.relu() if relu else h, [xd, rd, w, b], gy.double())
-    assert all(p.shape == q.shape and torch.equal(p.cpu().double(), q) for p, q in zip(got, want))
+    # 1x1 layers are exact; the library may take a window through a minimal-filtering transform: sums of at most 10 * 3^3 products, and 64 times their rounding (see the window layers' test)
+    xa, ra, wa, ba = (t.detach().abs().requires_grad_() for t in (xd, rd, w, b))
+    mags = torch.autograd.grad((F.conv3d if nd == 3 else F.conv2d)(xa, wa, ba, padding=k // 2) + ra, [xa, ra, wa, ba], gy.double().abs())
+    tol = 0 if k == 1 else 64 * 270 * 2.0 ** -24
+    assert all(p.shape == q.shape and bool(((p.cpu().double() - q).abs() <= tol * m).all()) for p, q, m in zip(got, want, mags))
 
 
 def test_a_map_without_extent_is_refused_as_by_any_convolution(cuda):
